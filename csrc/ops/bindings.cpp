@@ -177,6 +177,35 @@ void jodie_project_bwd(const at::Tensor& roots, const at::Tensor& n_roots, const
                        const at::Tensor& dt, const at::Tensor& dz, at::Tensor& dw, at::Tensor& db,
                        const c10::optional<at::Tensor>& peer);
 
+// recurrence_ops.cpp
+std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& decay,
+                                       const c10::optional<at::Tensor>& h0, const c10::optional<at::Tensor>& mask,
+                                       const c10::optional<at::Tensor>& offsets, double rate, bool time_major,
+                                       bool keep_states, bool keep8);
+std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const c10::optional<at::Tensor>& scales,
+                                       const at::Tensor& states, const at::Tensor& decay,
+                                       const c10::optional<at::Tensor>& h0, const c10::optional<at::Tensor>& mask,
+                                       const c10::optional<at::Tensor>& offsets, const c10::optional<at::Tensor>& dh,
+                                       const c10::optional<at::Tensor>& dlast, double rate, bool time_major, bool bf16,
+                                       bool need_dh0);
+at::Tensor gated_scan_step(const at::Tensor& p, const at::Tensor& decay, at::Tensor& state,
+                           const c10::optional<at::Tensor>& rows, double rate);
+std::vector<at::Tensor> norm_residual_fwd(const at::Tensor& x, const c10::optional<at::Tensor>& u,
+                                          const c10::optional<at::Tensor>& gate,
+                                          const c10::optional<at::Tensor>& w_post,
+                                          const c10::optional<at::Tensor>& w_pre,
+                                          const c10::optional<at::Tensor>& scale, double eps, bool keep8);
+std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const c10::optional<at::Tensor>& u,
+                                          const c10::optional<at::Tensor>& gate,
+                                          const c10::optional<at::Tensor>& scales,
+                                          const c10::optional<at::Tensor>& w_post,
+                                          const c10::optional<at::Tensor>& w_pre,
+                                          const c10::optional<at::Tensor>& scale, double eps,
+                                          const c10::optional<at::Tensor>& dy, const c10::optional<at::Tensor>& dn,
+                                          bool bf16);
+std::vector<at::Tensor> quantize8(const at::Tensor& x);
+at::Tensor dequantize8(const at::Tensor& codes, const at::Tensor& scales, bool bf16);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "starry_unigraph sm_100a kernels (tcgen05 GEMMs, TGN step, DTDG ops, collectives)";
   m.def("status_read", &status_read, "read (and clear) the device status word", py::arg("clear") = true);
@@ -243,4 +272,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("halo"), py::arg("n_rows"), py::arg("plan") = py::none());
   m.def("lstm_fwd", &lstm_fwd);
   m.def("lstm_bwd", &lstm_bwd);
+  m.def("gated_scan_fwd", &gated_scan_fwd);
+  m.def("gated_scan_bwd", &gated_scan_bwd);
+  m.def("gated_scan_step", &gated_scan_step);
+  m.def("norm_residual_fwd", &norm_residual_fwd);
+  m.def("norm_residual_bwd", &norm_residual_bwd);
+  m.def("quantize8", &quantize8);
+  m.def("dequantize8", &dequantize8);
 }

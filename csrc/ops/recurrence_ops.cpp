@@ -1,0 +1,458 @@
+// Torch wrappers of the gated recurrent block's kernels: gated linear recurrence, norms
+// around a block, 8-bit activations.
+#include "host_common.h"
+#include "recurrence.h"
+
+using namespace su;
+
+namespace {
+
+using OptTensor = c10::optional<at::Tensor>;
+
+bool is_float_type(const at::Tensor& t) {
+  return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16;
+}
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// Numbers go into messages as text: an integer put into the stream of TORCH_CHECK crashes
+// where the interpreter brings a C++ library of its own.
+std::string str(int64_t v) { return std::to_string(v); }
+std::string str(at::IntArrayRef v) {
+  std::string s = "[";
+  for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
+  return s + "]";
+}
+
+// (of a tensor without values any stride will do: torch gives such tensors any)
+bool unit_last(const at::Tensor& t) { return t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1; }
+
+// rows that start on multiples of 4 values: base and strides of a tensor with unit last stride
+bool rows_of_four(const at::Tensor& t) {
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % (4 * t.element_size()) != 0) return false;
+  for (int64_t d = 0; d + 1 < t.dim(); ++d)
+    if (t.size(d) > 1 && t.stride(d) % 4 != 0) return false;
+  return t.size(-1) % 4 == 0;
+}
+
+void check_param(const at::Tensor& t, const char* name, int64_t width, const at::Device& dev) {
+  TORCH_CHECK(t.device() == dev, name, " must be on ", dev);
+  TORCH_CHECK(is_float_type(t), name, " must be float32 or bfloat16");
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == width && t.is_contiguous(), name, " must be a contiguous vector of ",
+              str(width));
+}
+
+void check_rows(const at::Tensor& t, const char* name, const at::Tensor& like) {
+  TORCH_CHECK(t.device() == like.device(), name, " must be on ", like.device());
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must be ", like.scalar_type());
+  TORCH_CHECK(t.sizes() == like.sizes(), name, " must have the shape ", str(like.sizes()), ", got ", str(t.sizes()));
+  TORCH_CHECK(unit_last(t), name, " must have unit stride along its last dimension");
+}
+
+struct ScanSizes {
+  bool packed;
+  int64_t batch, steps, width;
+};
+ScanSizes scan_sizes(at::IntArrayRef shape, const OptTensor& offsets, int64_t per_row) {
+  ScanSizes s;
+  s.packed = given(offsets);
+  TORCH_CHECK(static_cast<int64_t>(shape.size()) == (s.packed ? 2 : 3),
+              "gated_scan: p must be [batch, steps, 3H], or [rows, 3H] with offsets");
+  TORCH_CHECK(shape.back() > 0 && shape.back() % per_row == 0, "gated_scan: the last dimension of p must be 3H, H > 0");
+  s.width = shape.back() / per_row;
+  TORCH_CHECK(s.width <= (1 << 24), "gated_scan: H above 2^24");
+  s.steps = s.packed ? shape[0] : shape[1];
+  s.batch = s.packed ? offsets->size(0) - 1 : shape[0];
+  return s;
+}
+
+// what forward and backward share: sequences, mask, decay, first states, layout of the dense rows
+ScanArgs scan_args(const ScanSizes& z, const at::Tensor& decay, const OptTensor& h0, const OptTensor& mask,
+                   const OptTensor& offsets, double rate, bool time_major, const at::Device& dev) {
+  ScanArgs a;
+  a.batch = z.batch;
+  a.steps = z.steps;
+  a.width = static_cast<int>(z.width);
+  TORCH_CHECK(rate > 0 && std::isfinite(rate), "gated_scan: rate must be positive and finite");
+  a.rate = static_cast<float>(rate);
+  check_param(decay, "gated_scan: decay", z.width, dev);
+  a.decay = decay.data_ptr();
+  a.decay_bf16 = decay.scalar_type() == at::kBFloat16;
+  if (given(h0)) {
+    TORCH_CHECK(h0->device() == dev && h0->scalar_type() == at::kFloat && h0->is_contiguous(),
+                "gated_scan: h0 must be contiguous float32 on ", dev);
+    TORCH_CHECK(h0->dim() == 2 && h0->size(0) == z.batch && h0->size(1) == z.width, "gated_scan: h0 must be [",
+                str(z.batch), ", ", str(z.width), "]");
+    a.h0 = h0->data_ptr<float>();
+  }
+  if (z.packed) {
+    TORCH_CHECK(offsets->device() == dev && offsets->scalar_type() == at::kLong && offsets->dim() == 1 &&
+                    offsets->size(0) >= 1 && offsets->is_contiguous(),
+                "gated_scan: offsets must be a contiguous int64 vector of sequences + 1 on ", dev);
+    a.offsets = offsets->data_ptr<int64_t>();
+  }
+  if (given(mask)) {
+    TORCH_CHECK(mask->device() == dev && mask->scalar_type() == at::kBool, "gated_scan: mask must be bool on ", dev);
+    const bool fits = z.packed ? mask->dim() == 1 && mask->size(0) == z.steps
+                               : mask->dim() == 2 && mask->size(0) == z.batch && mask->size(1) == z.steps;
+    TORCH_CHECK(fits, "gated_scan: mask must have the shape of p without its last dimension");
+    a.mask = reinterpret_cast<const uint8_t*>(mask->data_ptr<bool>());
+    a.m_sb = z.packed ? 0 : mask->stride(0);
+    a.m_st = mask->stride(z.packed ? 0 : 1);
+  }
+  a.row_sb = z.packed ? 0 : (time_major ? 1 : z.steps);
+  a.row_st = z.packed ? 1 : (time_major ? z.batch : 1);
+  a.n_states = z.steps > 0 ? (z.steps - 1) / kStateEvery : 0;
+  a.status = device_status_ptr(dev.index());
+  return a;
+}
+
+// [batch, steps, width] (packed: [rows, width]) over dense rows in the order of the layout
+at::Tensor dense_rows(const ScanSizes& z, int64_t width, bool time_major, const at::TensorOptions& o) {
+  if (z.packed) return at::empty({z.steps, width}, o);
+  if (time_major) return at::empty({z.steps, z.batch, width}, o).transpose(0, 1);
+  return at::empty({z.batch, z.steps, width}, o);
+}
+
+int64_t groups_of(int64_t width) { return (width + kGroup8 - 1) / kGroup8; }
+
+}  // namespace
+
+// -> h, last state, kept states, codes, scales (the last three undefined where not kept)
+std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& decay, const OptTensor& h0,
+                                       const OptTensor& mask, const OptTensor& offsets, double rate, bool time_major,
+                                       bool keep_states, bool keep8) {
+  SU_CHECK_CUDA(p);
+  TORCH_CHECK(is_float_type(p), "gated_scan: p must be float32 or bfloat16");
+  const ScanSizes z = scan_sizes(p.sizes(), offsets, 3);
+  TORCH_CHECK(unit_last(p), "gated_scan: p must have unit stride along its last dimension");
+  c10::cuda::CUDAGuard guard(p.device());
+  ScanArgs a = scan_args(z, decay, h0, mask, offsets, rate, time_major, p.device());
+  a.bf16 = p.scalar_type() == at::kBFloat16;
+  a.p = p.data_ptr();
+  a.p_sb = z.packed ? 0 : p.stride(0);
+  a.p_st = p.stride(z.packed ? 0 : 1);
+  a.vec = rows_of_four(p) && z.width % 4 == 0;
+  const auto f32 = p.options().dtype(at::kFloat);
+  at::Tensor h = dense_rows(z, z.width, time_major, p.options());
+  at::Tensor last = at::empty({z.batch, z.width}, f32);
+  at::Tensor states, codes, scales;
+  a.h = h.data_ptr();
+  a.last = last.data_ptr<float>();
+  if (keep_states) {
+    states = at::empty({z.packed ? 1 : z.batch, a.n_states, z.width}, f32);
+    if (a.n_states > 0) a.states = states.data_ptr<float>();
+  }
+  if (keep8) {
+    codes = dense_rows(z, 3 * z.width, time_major, p.options().dtype(at::kChar));
+    scales = dense_rows(z, 3 * groups_of(z.width), time_major, f32);
+    a.codes = codes.data_ptr<int8_t>();
+    a.scales = scales.data_ptr<float>();
+  }
+  if (z.batch > 0) {
+    launch_scan_fwd(a, num_sms(p.get_device()), cur_stream());
+    SU_LAUNCH_CHECK();
+  }
+  return {h, last, states, codes, scales};
+}
+
+// `like`: p, or its 8-bit codes with `scales` (then the gradients have the type of h, `bf16`)
+// -> dp, ddecay, dh0
+std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptTensor& scales, const at::Tensor& states,
+                                       const at::Tensor& decay, const OptTensor& h0, const OptTensor& mask,
+                                       const OptTensor& offsets, const OptTensor& dh, const OptTensor& dlast,
+                                       double rate, bool time_major, bool bf16, bool need_dh0) {
+  SU_CHECK_CUDA(like);
+  const ScanSizes z = scan_sizes(like.sizes(), offsets, 3);
+  const auto dev = like.device();
+  c10::cuda::CUDAGuard guard(dev);
+  ScanArgs a = scan_args(z, decay, h0, mask, offsets, rate, time_major, dev);
+  const auto f32 = like.options().dtype(at::kFloat);
+  const auto type = bf16 ? at::kBFloat16 : at::kFloat;
+  a.bf16 = bf16;
+  a.vec = z.width % 4 == 0;
+  if (given(scales)) {
+    TORCH_CHECK(like.scalar_type() == at::kChar, "gated_scan: 8-bit codes must be int8");
+    a.codes = like.data_ptr<int8_t>();
+    a.scales = scales->data_ptr<float>();
+  } else {
+    TORCH_CHECK(like.scalar_type() == type, "gated_scan: p must have the type of h");
+    a.p = like.data_ptr();
+    a.p_sb = z.packed ? 0 : like.stride(0);
+    a.p_st = like.stride(z.packed ? 0 : 1);
+    a.vec = a.vec && rows_of_four(like);
+  }
+  TORCH_CHECK(states.numel() == (z.packed ? 1 : z.batch) * a.n_states * z.width, "gated_scan: kept states do not fit");
+  a.states = const_cast<float*>(states.data_ptr<float>());
+  if (given(dh)) {
+    TORCH_CHECK(dh->device() == dev && dh->scalar_type() == type && dh->dim() == like.dim() &&
+                    dh->size(-1) == z.width && unit_last(*dh),
+                "gated_scan: the gradient of h must have its type, shape and unit last stride");
+    a.dh = dh->data_ptr();
+    a.dh_sb = z.packed ? 0 : dh->stride(0);
+    a.dh_st = dh->stride(z.packed ? 0 : 1);
+    a.vec = a.vec && rows_of_four(*dh);
+  }
+  if (given(dlast)) {
+    TORCH_CHECK(dlast->scalar_type() == at::kFloat && dlast->is_contiguous() && dlast->numel() == z.batch * z.width,
+                "gated_scan: the gradient of the last state must be contiguous float32");
+    a.dlast = dlast->data_ptr<float>();
+  }
+  at::Tensor dp = dense_rows(z, 3 * z.width, time_major, like.options().dtype(type));
+  at::Tensor ddecay = at::empty_like(decay);
+  at::Tensor dh0 = need_dh0 ? at::empty({z.batch, z.width}, f32) : at::Tensor();
+  a.dp = dp.data_ptr();
+  a.dh0 = need_dh0 ? dh0.data_ptr<float>() : nullptr;
+  if (z.batch == 0) {
+    ddecay.zero_();
+    return {dp, ddecay, dh0};
+  }
+  const int sms = num_sms(like.get_device());
+  a.n_partial = scan_partials(a, sms);
+  at::Tensor partial = at::empty({a.n_partial, z.width}, f32);
+  a.partial = partial.data_ptr<float>();
+  launch_scan_bwd(a, sms, ddecay.data_ptr(), cur_stream());
+  SU_LAUNCH_CHECK();
+  return {dp, ddecay, dh0};
+}
+
+at::Tensor gated_scan_step(const at::Tensor& p, const at::Tensor& decay, at::Tensor& state, const OptTensor& rows,
+                           double rate) {
+  SU_CHECK_CUDA(p);
+  TORCH_CHECK(is_float_type(p), "gated_scan_step: p must be float32 or bfloat16");
+  TORCH_CHECK(p.dim() == 2 && p.size(1) > 0 && p.size(1) % 3 == 0 && unit_last(p),
+              "gated_scan_step: p must be [rows, 3H] with unit stride along its last dimension");
+  const int64_t n = p.size(0), H = p.size(1) / 3;
+  TORCH_CHECK(H <= (1 << 24), "gated_scan_step: H above 2^24");
+  TORCH_CHECK(rate > 0 && std::isfinite(rate), "gated_scan_step: rate must be positive and finite");
+  c10::cuda::CUDAGuard guard(p.device());
+  check_param(decay, "gated_scan_step: decay", H, p.device());
+  TORCH_CHECK(state.device() == p.device() && state.scalar_type() == at::kFloat && state.dim() == 2 &&
+                  state.size(1) == H && unit_last(state),
+              "gated_scan_step: state must be float32 [table rows, ", str(H), "] on ", p.device());
+  TORCH_CHECK(state.size(0) <= 1 || state.stride(0) >= H, "gated_scan_step: the rows of state must not overlap");
+  ScanStepArgs a;
+  if (given(rows)) {
+    TORCH_CHECK(rows->device() == p.device() && rows->scalar_type() == at::kLong && rows->dim() == 1 &&
+                    rows->size(0) == n && rows->is_contiguous(),
+                "gated_scan_step: rows must be a contiguous int64 vector, one place per row of p");
+    a.index = rows->data_ptr<int64_t>();
+  } else {
+    TORCH_CHECK(state.size(0) == n, "gated_scan_step: without rows, state must have one row per row of p");
+  }
+  at::Tensor h = at::empty({n, H}, p.options());
+  if (n == 0) return h;
+  a.bf16 = p.scalar_type() == at::kBFloat16;
+  a.rows = n;
+  a.table_rows = state.size(0);
+  a.width = static_cast<int>(H);
+  a.rate = static_cast<float>(rate);
+  a.p = p.data_ptr();
+  a.p_sb = p.stride(0);
+  a.decay = decay.data_ptr();
+  a.decay_bf16 = decay.scalar_type() == at::kBFloat16;
+  a.state = state.data_ptr<float>();
+  a.state_sb = state.stride(0);
+  a.h = h.data_ptr();
+  a.status = device_status_ptr(p.get_device());
+  launch_scan_step(a, cur_stream());
+  SU_LAUNCH_CHECK();
+  return h;
+}
+
+namespace {
+
+NormArgs norm_args(const at::Tensor& x, int64_t width, const OptTensor& w_post, const OptTensor& w_pre,
+                   const OptTensor& scale, double eps) {
+  TORCH_CHECK(width >= 1 && width <= kNormMaxWidth, "norm_residual: the width must be 1 to ", str(kNormMaxWidth));
+  TORCH_CHECK(eps > 0 && std::isfinite(eps), "norm_residual: eps must be positive and finite");
+  NormArgs a;
+  a.width = static_cast<int>(width);
+  a.eps = static_cast<float>(eps);
+  auto param = [&](const OptTensor& t, const char* name, const void*& ptr, int& bf16) {
+    if (!given(t)) return;
+    check_param(*t, name, width, x.device());
+    ptr = t->data_ptr();
+    bf16 = t->scalar_type() == at::kBFloat16;
+  };
+  param(w_post, "norm_residual: w_post", a.w_post, a.post_bf16);
+  param(w_pre, "norm_residual: w_pre", a.w_pre, a.pre_bf16);
+  param(scale, "norm_residual: scale", a.scale, a.scale_bf16);
+  return a;
+}
+
+}  // namespace
+
+// x, u, gate [rows, H] -> y (undefined without u), n (undefined without w_pre), codes, scales
+std::vector<at::Tensor> norm_residual_fwd(const at::Tensor& x, const OptTensor& u, const OptTensor& gate,
+                                          const OptTensor& w_post, const OptTensor& w_pre, const OptTensor& scale,
+                                          double eps, bool keep8) {
+  SU_CHECK_CUDA(x);
+  TORCH_CHECK(is_float_type(x) && x.dim() == 2, "norm_residual: x must be float32 or bfloat16 rows");
+  TORCH_CHECK(unit_last(x), "norm_residual: x must have unit stride along its last dimension");
+  c10::cuda::CUDAGuard guard(x.device());
+  NormArgs a = norm_args(x, x.size(1), w_post, w_pre, scale, eps);
+  a.bf16 = x.scalar_type() == at::kBFloat16;
+  a.rows = x.size(0);
+  a.x = x.data_ptr();
+  a.x_ld = x.stride(0);
+  a.vec = rows_of_four(x);
+  int64_t parts = 1;
+  if (given(u)) {
+    check_rows(*u, "norm_residual: u", x);
+    a.u = u->data_ptr();
+    a.u_ld = u->stride(0);
+    a.vec = a.vec && rows_of_four(*u);
+    ++parts;
+  }
+  if (given(gate)) {
+    TORCH_CHECK(given(u), "norm_residual: a gate needs u");
+    check_rows(*gate, "norm_residual: gate", x);
+    a.gate = gate->data_ptr();
+    a.gate_ld = gate->stride(0);
+    a.vec = a.vec && rows_of_four(*gate);
+    ++parts;
+  }
+  const int64_t H = a.width;
+  at::Tensor y, n, codes, scales;
+  // (an empty tensor's address is null: what takes part goes by the arguments)
+  if (given(u)) {
+    y = at::empty({a.rows, H}, x.options());
+    a.y = y.data_ptr();
+  }
+  if (given(w_pre)) {
+    n = at::empty({a.rows, H}, x.options());
+    a.n = n.data_ptr();
+  }
+  if (keep8) {
+    codes = at::empty({parts, a.rows, H}, x.options().dtype(at::kChar));
+    scales = at::empty({parts, a.rows, groups_of(H)}, x.options().dtype(at::kFloat));
+    a.codes = codes.data_ptr<int8_t>();
+    a.scales = scales.data_ptr<float>();
+  }
+  if (a.rows > 0) {
+    launch_norm_fwd(a, num_sms(x.get_device()), cur_stream());
+    SU_LAUNCH_CHECK();
+  }
+  return {y, n, codes, scales};
+}
+
+// x, u, gate: the forward's rows, or (keep8) undefined u and gate with x = codes and `scales`
+// -> dx, du, dgate, dw_post, dw_pre, dscale (undefined where there is nothing to differentiate)
+std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const OptTensor& u, const OptTensor& gate,
+                                          const OptTensor& scales, const OptTensor& w_post, const OptTensor& w_pre,
+                                          const OptTensor& scale, double eps, const OptTensor& dy, const OptTensor& dn,
+                                          bool bf16) {
+  SU_CHECK_CUDA(x);
+  c10::cuda::CUDAGuard guard(x.device());
+  NormArgs a = norm_args(x, x.size(-1), w_post, w_pre, scale, eps);
+  const int64_t H = a.width;
+  const auto type = bf16 ? at::kBFloat16 : at::kFloat;
+  const auto opt = x.options().dtype(type);
+  a.bf16 = bf16;
+  a.rows = x.size(-2);
+  a.vec = H % 4 == 0;
+  bool has_u, has_gate;
+  if (given(scales)) {
+    TORCH_CHECK(x.scalar_type() == at::kChar && x.dim() == 3, "norm_residual: malformed 8-bit inputs");
+    a.codes = x.data_ptr<int8_t>();
+    a.scales = scales->data_ptr<float>();
+    a.x = x.data_ptr();
+    has_u = x.size(0) > 1;
+    has_gate = x.size(0) > 2;
+    if (has_u) a.u = a.x;  // only whether they exist is read
+    if (has_gate) a.gate = a.x;
+  } else {
+    TORCH_CHECK(x.scalar_type() == type && x.dim() == 2, "norm_residual: x must have the type of y");
+    a.x = x.data_ptr();
+    a.x_ld = x.stride(0);
+    a.vec = a.vec && rows_of_four(x);
+    has_u = given(u);
+    has_gate = given(gate);
+    if (has_u) {
+      a.u = u->data_ptr();
+      a.u_ld = u->stride(0);
+      a.vec = a.vec && rows_of_four(*u);
+    }
+    if (has_gate) {
+      a.gate = gate->data_ptr();
+      a.gate_ld = gate->stride(0);
+      a.vec = a.vec && rows_of_four(*gate);
+    }
+  }
+  auto grad = [&](const OptTensor& t, const void*& ptr, int64_t& ld) {
+    if (!given(t)) return;
+    TORCH_CHECK(t->scalar_type() == type && t->dim() == 2 && t->size(0) == a.rows && t->size(1) == H && unit_last(*t),
+                "norm_residual: gradients must have the type and shape of the outputs and unit last stride");
+    ptr = t->data_ptr();
+    ld = t->stride(0);
+    a.vec = a.vec && rows_of_four(*t);
+  };
+  grad(dy, a.dy, a.dy_ld);
+  if (given(w_pre)) grad(dn, a.dn, a.dn_ld);
+  at::Tensor dx = at::empty({a.rows, H}, opt), du, dgate, dw_post, dw_pre, dscale;
+  a.dx = dx.data_ptr();
+  if (has_u) {
+    du = at::empty({a.rows, H}, opt);
+    a.du = du.data_ptr();
+  }
+  if (has_gate) {
+    dgate = at::empty({a.rows, H}, opt);
+    a.dgate = dgate.data_ptr();
+  }
+  auto param = [&](const OptTensor& t, bool used, at::Tensor& g, void*& ptr) {
+    if (!given(t) || !used) return;
+    g = at::empty_like(*t);
+    ptr = g.data_ptr();
+    if (a.rows == 0) g.zero_();
+  };
+  param(w_post, has_u, dw_post, a.dw_post);
+  param(w_pre, true, dw_pre, a.dw_pre);
+  param(scale, has_u, dscale, a.dscale);
+  if (a.rows > 0) {
+    const int sms = num_sms(x.get_device());
+    a.n_partial = norm_partials(a, sms);
+    at::Tensor partial = at::empty({a.n_partial, 3, H}, x.options().dtype(at::kFloat));
+    a.partial = partial.data_ptr<float>();
+    launch_norm_bwd(a, sms, cur_stream());
+    SU_LAUNCH_CHECK();
+  }
+  return {dx, du, dgate, dw_post, dw_pre, dscale};
+}
+
+// x [rows, H] -> codes [rows, H], scales [rows, ceil(H / 32)]
+std::vector<at::Tensor> quantize8(const at::Tensor& x) {
+  SU_CHECK_CUDA(x);
+  TORCH_CHECK(is_float_type(x) && x.dim() == 2 && x.size(1) > 0, "quantize8: x must be float32 or bfloat16 rows");
+  TORCH_CHECK(unit_last(x), "quantize8: x must have unit stride along its last dimension");
+  TORCH_CHECK(x.size(1) <= INT32_MAX, "quantize8: rows of at most 2^31 - 1 values");
+  c10::cuda::CUDAGuard guard(x.device());
+  const int64_t rows = x.size(0), H = x.size(1);
+  at::Tensor codes = at::empty({rows, H}, x.options().dtype(at::kChar));
+  at::Tensor scales = at::empty({rows, groups_of(H)}, x.options().dtype(at::kFloat));
+  if (rows == 0) return {codes, scales};
+  launch_quantize8(x.data_ptr(), x.scalar_type() == at::kBFloat16, x.stride(0), rows, static_cast<int>(H),
+                   codes.data_ptr<int8_t>(), scales.data_ptr<float>(), rows_of_four(x), cur_stream());
+  SU_LAUNCH_CHECK();
+  return {codes, scales};
+}
+
+at::Tensor dequantize8(const at::Tensor& codes, const at::Tensor& scales, bool bf16) {
+  SU_CHECK_CUDA(codes);
+  SU_CHECK_CUDA(scales);
+  SU_CHECK_CONTIG(codes);
+  SU_CHECK_CONTIG(scales);
+  SU_CHECK_F32(scales);
+  TORCH_CHECK(codes.scalar_type() == at::kChar && codes.dim() == 2, "dequantize8: codes must be int8 rows");
+  const int64_t rows = codes.size(0), H = codes.size(1);
+  TORCH_CHECK(scales.dim() == 2 && scales.size(0) == rows && scales.size(1) == groups_of(H) &&
+                  scales.device() == codes.device() && H <= INT32_MAX,
+              "dequantize8: one scale per row and group of ", str(kGroup8), " values");
+  c10::cuda::CUDAGuard guard(codes.device());
+  at::Tensor x = at::empty({rows, H}, codes.options().dtype(bf16 ? at::kBFloat16 : at::kFloat));
+  if (x.numel() == 0) return x;
+  const bool vec = H % 4 == 0 && reinterpret_cast<uintptr_t>(codes.data_ptr()) % 4 == 0;
+  launch_dequantize8(codes.data_ptr<int8_t>(), scales.data_ptr<float>(), rows, static_cast<int>(H), x.data_ptr(), bf16,
+                     vec, cur_stream());
+  SU_LAUNCH_CHECK();
+  return x;
+}

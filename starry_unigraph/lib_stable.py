@@ -10,11 +10,14 @@ from starry_unigraph.data.sample_config import SampleConfig
 from starry_unigraph.models.base import TemporalModel
 from starry_unigraph.models.task_head import EdgePredictHead, NodeClassifyHead, NodeRegressHead
 from starry_unigraph.models.wrapped import WrappedModel
+from starry_unigraph.ops.checkpoint8 import Packed8, quantize8, saved8
+from starry_unigraph.ops.norm import norm_residual, rms_norm
+from starry_unigraph.ops.recurrence import gated_scan, gated_scan_step
 from starry_unigraph.registry.task_adapter import TaskAdapter
 from starry_unigraph.registry.task_registry import TaskRegistry
 from starry_unigraph.runtime.backend import GraphBackend, StateManager
 from starry_unigraph.runtime.engine import PipelineEngine
-from starry_unigraph.runtime.modules import GCNStack, MatGRUCell, TimeEncode, _LSTMCell
+from starry_unigraph.runtime.modules import GatedRecurrentStack, GCNStack, MatGRUCell, TimeEncode, _LSTMCell
 from starry_unigraph.session import SchedulerSession
 
 __version__ = "0.2.0"
@@ -25,6 +28,7 @@ __all__ = [
     "ChunkAtomic", "NodeTemporalFeatureTable", "RawTemporalEvents", "GraphBackend", "StateManager", "TaskAdapter",
     "TemporalModel", "WrappedModel", "EdgePredictHead", "NodeRegressHead", "NodeClassifyHead", "TimeEncode",
     "GCNStack", "MatGRUCell", "_LSTMCell", "SchedulerSession", "PipelineEngine", "TaskRegistry",
+    "GatedRecurrentStack", "gated_scan", "gated_scan_step", "norm_residual", "rms_norm", "quantize8", "Packed8", "saved8",
 ]
 
 

@@ -1,0 +1,120 @@
+"""Activations kept in 8 bits between the forward and the backward pass.
+
+Format: groups of 32 neighbouring values of a row share one fp32 scale,
+``scale = amax / 127`` and ``code = rint(v * (127 / amax))`` (the division and the
+product by 1/127 each rounded once), 1.125 bytes a value. Rounding moves a value by at
+most half a scale. A group whose largest magnitude is below 2^-100 reads back as
+zeros; a group that holds a NaN or an infinity has the scale NaN and reads back as NaN,
+so that a broken activation shows in the gradients.
+
+* ``quantize8(x)`` -> ``Packed8``; ``Packed8.dequantize(dtype=None)`` back to x's type.
+* ``with saved8(): loss = model(...)``: every activation that an autograd node of the
+  block saves is kept in 8 bits (the framework's own ops and torch's alike) and restored
+  when its backward pass asks for it. Parameters, integer tensors, small tensors and
+  what an op marks as exact stay as they are. A saved ReLU output below half its group's
+  scale reads back as zero and passes no gradient.
+* ``gated_scan`` and ``norm_residual`` take ``checkpoint="int8"``: their own kernels write
+  the codes while they read the inputs and read the codes in the backward pass, with no
+  restored copy in between.
+
+On CPU tensors the same functions run the same arithmetic with torch operations.
+"""
+from __future__ import annotations
+
+from contextlib import contextmanager
+from dataclasses import dataclass
+
+import torch
+import torch.nn.functional as F
+
+from starry_unigraph.ops import cuda_ext
+
+GROUP = 32
+
+
+def check_checkpoint(value: str | None) -> bool:
+    """True for ``"int8"``, False for None."""
+    if value not in (None, "int8"):
+        raise ValueError(f'checkpoint must be None or "int8", got {value!r}')
+    return value == "int8"
+
+
+def _quantize_torch(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales of [rows, H] with torch operations (fp32; fp64 inputs stay fp64)."""
+    v = x if x.dtype == torch.float64 else x.float()
+    v = F.pad(v, (0, -x.size(1) % GROUP)).unflatten(1, (-1, GROUP))
+    top = v.abs().amax(2, keepdim=True)
+    tiny, bad = top < 2.0 ** -100, ~torch.isfinite(top)
+    zero = torch.zeros_like(top)
+    inv = torch.where(tiny | bad, zero, torch.full_like(top, 127.0) / top)
+    scale = torch.where(tiny, zero, torch.where(bad, torch.full_like(top, float("nan")), top * (1.0 / 127.0)))
+    codes = torch.nan_to_num(torch.round(v * inv), nan=0.0)
+    return codes.flatten(1)[:, : x.size(1)].to(torch.int8).contiguous(), scale.squeeze(2)
+
+
+def _dequantize_torch(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    wide = scales.repeat_interleave(GROUP, dim=1)[:, : codes.size(1)]
+    return (codes.to(wide.dtype) * wide).to(dtype)
+
+
+@dataclass
+class Packed8:
+    """8-bit codes [rows, H] and scales [rows, ceil(H / 32)] of a tensor of `shape` and `dtype`."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    shape: torch.Size
+    dtype: torch.dtype
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel() * self.scales.element_size()
+
+    def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        dtype = self.dtype if dtype is None else dtype
+        if self.codes.is_cuda:
+            if dtype not in (torch.float32, torch.bfloat16):
+                raise ValueError(f"dequantize: float32 or bfloat16 on CUDA, got {dtype}")
+            out = cuda_ext().dequantize8(self.codes, self.scales, dtype == torch.bfloat16)
+        else:
+            out = _dequantize_torch(self.codes, self.scales, dtype)
+        return out.view(self.shape)
+
+
+def quantize8(x: torch.Tensor) -> Packed8:
+    """8-bit codes of x along its last dimension (float32 or bfloat16; on CPU float64 too)."""
+    if x.dim() == 0 or x.size(-1) == 0:
+        raise ValueError("quantize8: x needs a last dimension of at least one value")
+    if not x.is_floating_point():
+        raise ValueError(f"quantize8: a floating tensor is wanted, got {x.dtype}")
+    rows = x.detach().reshape(-1, x.size(-1))
+    if rows.size(1) > 1 and rows.stride(1) != 1:
+        rows = rows.contiguous()
+    codes, scales = cuda_ext().quantize8(rows) if x.is_cuda else _quantize_torch(rows)
+    return Packed8(codes, scales, x.shape, x.dtype)
+
+
+def exact(t: torch.Tensor | None) -> torch.Tensor | None:
+    """Marks a tensor that an op saves for its backward pass as not to be kept in 8 bits."""
+    if t is not None:
+        t._su_exact = True
+    return t
+
+
+@contextmanager
+def saved8(min_numel: int = 1 << 16):
+    """Keep the activations that autograd saves inside the block in 8 bits: float32 and
+    bfloat16 tensors of at least two dimensions and `min_numel` values that are neither
+    parameters (leaves that require a gradient) nor marked by ``exact``."""
+
+    def pack(t: torch.Tensor):
+        if (t.dtype not in (torch.float32, torch.bfloat16) or t.dim() < 2 or t.numel() < max(1, min_numel)
+                or (t.is_leaf and t.requires_grad) or getattr(t, "_su_exact", False)):
+            return t
+        return quantize8(t)
+
+    def unpack(p):
+        return p.dequantize() if isinstance(p, Packed8) else p
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+        yield

@@ -1,4 +1,5 @@
 """Reusable layers (reference runtime/modules/__init__.py:15-27)."""
+from .gated_block import GatedRecurrentStack
 from .gcn_layers import GCNStack
 from .rnn_cells import MatGRUCell, _LSTMCell
 from .time_encode import TimeEncode
@@ -12,4 +13,5 @@ def __getattr__(name):
     raise AttributeError(name)
 
 
-__all__ = ["TimeEncode", "GCNStack", "MatGRUCell", "_LSTMCell", "TemporalTransformerConv"]
+__all__ = ["TimeEncode", "GCNStack", "MatGRUCell", "_LSTMCell", "TemporalTransformerConv",
+           "GatedRecurrentStack"]
