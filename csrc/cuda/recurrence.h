@@ -45,14 +45,20 @@ struct ScanArgs {
   void* dp = nullptr;           // dense rows of 3H
   float* dh0 = nullptr;         // [batch, H] or nullptr
   float* partial = nullptr;     // [n_partial, H] per-block sums of dz sigmoid(r)
-  int n_partial = 0;
   int vec = 1;                  // every row of p, dh, h, dp starts on a multiple of 4 values, H % 4 == 0
 };
 
-int scan_partials(const ScanArgs& a, int sms);  // rows of `partial` that launch_scan_bwd writes
-void launch_scan_fwd(const ScanArgs& a, int sms, cudaStream_t st);
+// Bytes of workspace that a call needs (16-byte aligned, no initial value).
+size_t scan_workspace(const ScanArgs& a, int sms);
+// Rows of `partial` that the backward pass writes, the ones it adds them up in included.
+int64_t scan_partials(const ScanArgs& a, int sms);
+void launch_scan_fwd(const ScanArgs& a, int sms, void* workspace, cudaStream_t st);
 // also adds `partial` up into ddecay [H] (in the type of decay)
-void launch_scan_bwd(const ScanArgs& a, int sms, void* ddecay, cudaStream_t st);
+void launch_scan_bwd(const ScanArgs& a, int sms, void* workspace, void* ddecay, cudaStream_t st);
+// the form that splits the steps into tiles (scan_tiles.cu)
+size_t scan_tiles_workspace(const ScanArgs& a);
+int64_t scan_tiles_partials(const ScanArgs& a);
+void launch_scan_tiles(const ScanArgs& a, bool bwd, void* workspace, cudaStream_t st);
 
 // One step of `rows` sequences whose fp32 states live in a table of table_rows rows;
 // index[i] (nullptr: i) is row i's place in the table.

@@ -7,21 +7,6 @@
 namespace su {
 namespace {
 
-// Where a thread's rows are: sequence s of a grid or of the packed axis.
-struct Seq {
-  int64_t begin, end;  // steps (packed: rows of the packed axis)
-  int64_t b;           // batch index of the strides (packed: 0)
-};
-__device__ __forceinline__ Seq seq_of(const ScanArgs& A, int64_t s) {
-  if (A.offsets == nullptr) return Seq{0, A.steps, s};
-  const int64_t lo = A.offsets[s], hi = A.offsets[s + 1];
-  if (lo < 0 || hi < lo || hi > A.steps) {  // skipped and reported
-    record_status(A.status, kBadIndex);
-    return Seq{0, 0, 0};
-  }
-  return Seq{lo, hi, 0};
-}
-
 // ---------------------------------------------------------------------------
 // A thread walks its V channels of one sequence after another.
 // ---------------------------------------------------------------------------
@@ -40,22 +25,21 @@ __global__ void __launch_bounds__(256) scan_rows_fwd_kernel(const ScanArgs A, co
   T* Hout = static_cast<T*>(A.h) + c;
   for (int64_t s = static_cast<int64_t>(blockIdx.x) * L.rows + y; s < A.batch;
        s += static_cast<int64_t>(gridDim.x) * L.rows) {
-    const Seq q = seq_of(A, s);
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = (live && A.h0 != nullptr) ? A.h0[s * H + c + v] : 0.f;
-    for (int64_t t0 = q.begin; t0 < q.end; t0 += U) {
+    for (int64_t t0 = 0; t0 < A.steps; t0 += U) {
       Pack<T, V> x[U], r[U], i[U];
       bool on[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const int64_t t = t0 + j;
-        on[j] = t < q.end && (A.mask == nullptr || A.mask[q.b * A.m_sb + t * A.m_st] != 0);
+        on[j] = t < A.steps && (A.mask == nullptr || A.mask[s * A.m_sb + t * A.m_st] != 0);
         x[j].zero();
         r[j].zero();
         i[j].zero();
         if (on[j] && live) {
-          const T* row = P + q.b * A.p_sb + t * A.p_st;
+          const T* row = P + s * A.p_sb + t * A.p_st;
           x[j].load(row);
           r[j].load(row + H);
           i[j].load(row + 2 * H);
@@ -64,9 +48,9 @@ __global__ void __launch_bounds__(256) scan_rows_fwd_kernel(const ScanArgs A, co
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const int64_t t = t0 + j;
-        if (t >= q.end) break;
-        if (A.states != nullptr && live && t > q.begin && t % kStateEvery == 0) {
-          float* to = A.states + (q.b * A.n_states + t / kStateEvery - 1) * H + c;
+        if (t >= A.steps) break;
+        if (A.states != nullptr && live && t > 0 && t % kStateEvery == 0) {
+          float* to = A.states + (s * A.n_states + t / kStateEvery - 1) * H + c;
 #pragma unroll
           for (int v = 0; v < V; ++v) to[v] = h[v];
         }
@@ -74,7 +58,7 @@ __global__ void __launch_bounds__(256) scan_rows_fwd_kernel(const ScanArgs A, co
         x[j].get(fx);
         r[j].get(fr);
         i[j].get(fi);
-        const int64_t row = q.b * A.row_sb + t * A.row_st;
+        const int64_t row = s * A.row_sb + t * A.row_st;
         if constexpr (CODES) {
           int8_t code[V];
           int8_t* to = A.codes + row * 3 * H + c;
@@ -132,31 +116,29 @@ __global__ void __launch_bounds__(256) scan_rows_bwd_kernel(const ScanArgs A, co
   if (live) {
     for (int64_t s = static_cast<int64_t>(blockIdx.x) * L.rows + y; s < A.batch;
          s += static_cast<int64_t>(gridDim.x) * L.rows) {
-      const Seq q = seq_of(A, s);
       float E[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) E[v] = A.dlast != nullptr ? A.dlast[s * H + c + v] : 0.f;
-      // chunks start at multiples of CH of the axis
-      for (int64_t tc = q.end > q.begin ? (q.end - 1) / CH * CH : q.begin - CH; tc > q.begin - CH; tc -= CH) {
+      for (int64_t tc = (A.steps + CH - 1) / CH * CH - CH; tc >= 0; tc -= CH) {
         float x[CH][V], r[CH][V], i[CH][V], d[CH][V], before[CH][V];
         bool in[CH], on[CH];
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
           const int64_t t = tc + j;
-          in[j] = t >= q.begin && t < q.end;
-          on[j] = in[j] && (A.mask == nullptr || A.mask[q.b * A.m_sb + t * A.m_st] != 0);
+          in[j] = t < A.steps;
+          on[j] = in[j] && (A.mask == nullptr || A.mask[s * A.m_sb + t * A.m_st] != 0);
 #pragma unroll
           for (int v = 0; v < V; ++v) x[j][v] = r[j][v] = i[j][v] = d[j][v] = 0.f;
           if (on[j]) {
             if constexpr (CODES) {
-              const int64_t row = q.b * A.row_sb + t * A.row_st;
+              const int64_t row = s * A.row_sb + t * A.row_st;
               const int8_t* from = A.codes + row * 3 * H + c;
               const float* sc = A.scales + row * 3 * G + c / kGroup8;
               load_codes(from, sc[0], x[j]);
               load_codes(from + H, sc[G], r[j]);
               load_codes(from + 2 * H, sc[2 * G], i[j]);
             } else {
-              const T* row = static_cast<const T*>(A.p) + q.b * A.p_sb + t * A.p_st + c;
+              const T* row = static_cast<const T*>(A.p) + s * A.p_sb + t * A.p_st + c;
               Pack<T, V> w;
               w.load(row);
               w.get(x[j]);
@@ -168,13 +150,13 @@ __global__ void __launch_bounds__(256) scan_rows_bwd_kernel(const ScanArgs A, co
           }
           if (in[j] && A.dh != nullptr) {
             Pack<T, V> w;
-            w.load(static_cast<const T*>(A.dh) + q.b * A.dh_sb + t * A.dh_st + c);
+            w.load(static_cast<const T*>(A.dh) + s * A.dh_sb + t * A.dh_st + c);
             w.get(d[j]);
           }
         }
         float h[V];
-        if (tc > q.begin) {
-          const float* from = A.states + (q.b * A.n_states + tc / kStateEvery - 1) * H + c;
+        if (tc > 0) {
+          const float* from = A.states + (s * A.n_states + tc / kStateEvery - 1) * H + c;
 #pragma unroll
           for (int v = 0; v < V; ++v) h[v] = from[v];
         } else {
@@ -195,7 +177,7 @@ __global__ void __launch_bounds__(256) scan_rows_bwd_kernel(const ScanArgs A, co
 #pragma unroll
         for (int j = CH - 1; j >= 0; --j) {
           if (!in[j]) continue;
-          const int64_t row = q.b * A.row_sb + (tc + j) * A.row_st;
+          const int64_t row = s * A.row_sb + (tc + j) * A.row_st;
           float dx[V], dr[V], di[V];
 #pragma unroll
           for (int v = 0; v < V; ++v) {
@@ -238,19 +220,26 @@ __global__ void __launch_bounds__(256) scan_rows_bwd_kernel(const ScanArgs A, co
   }
 }
 
-// ddecay = -c sigmoid(decay) * the partial sums in order: 32 channels x 32 shares per block
-__global__ void scan_decay_grad_kernel(const float* __restrict__ partial, int n, int H, const void* decay,
+// Rows k, k + m, k + 2m, ... of partial [n, H] added up in order into row k of out [m, H]:
+// 32 channels x 32 shares per block. `last`: out is ddecay, -c sigmoid(decay) times the sum.
+__global__ void scan_decay_grad_kernel(const float* __restrict__ partial, int64_t n, int H, bool last, const void* decay,
                                        int decay_bf16, float rate, void* out) {
   __shared__ float sum[32][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float t = 0.f;
-  if (c < H)
-    for (int w = threadIdx.y; w < n; w += 32) t += partial[static_cast<int64_t>(w) * H + c];
+  if (c < H) {
+#pragma unroll 4
+    for (int64_t w = blockIdx.y + static_cast<int64_t>(threadIdx.y) * gridDim.y; w < n; w += 32ll * gridDim.y)
+      t += partial[w * H + c];
+  }
   sum[threadIdx.y][threadIdx.x] = t;
   __syncthreads();
   if (threadIdx.y == 0 && c < H) {
     for (int w = 1; w < 32; ++w) t += sum[w][threadIdx.x];
-    param_store(out, decay_bf16, c, -rate * sigmoid_f(param_at(decay, decay_bf16, c)) * t);
+    if (last)
+      param_store(out, decay_bf16, c, -rate * sigmoid_f(param_at(decay, decay_bf16, c)) * t);
+    else
+      static_cast<float*>(out)[static_cast<int64_t>(blockIdx.y) * H + c] = t;
   }
 }
 
@@ -291,9 +280,8 @@ struct BwdShape {
 // 16 bytes of a channel per thread and step where the whole sequence is one short chunk,
 // 4 bytes where 16 steps of inputs and states have to stay in registers
 BwdShape bwd_shape(const ScanArgs& a) {
-  const bool one = a.offsets == nullptr;
-  if (one && a.steps <= 4) return {a.vec ? 4 : 1, 4};
-  if (one && a.steps <= 8) return {a.vec ? 2 : 1, 8};
+  if (a.steps <= 4) return {a.vec ? 4 : 1, 4};
+  if (a.steps <= 8) return {a.vec ? 2 : 1, 8};
   return {a.vec && a.bf16 ? 2 : 1, kStateEvery};
 }
 
@@ -332,13 +320,31 @@ void rows_bwd(const ScanArgs& a, int sms, cudaStream_t st) {
   }
 }
 
-}  // namespace
-
-int scan_partials(const ScanArgs& a, int sms) {
-  return row_blocks(a, lanes_of(a.width, bwd_shape(a).V, false, 256, 256), sms);
+// Tiles for packed sequences, and where a thread per sequence and 4 channels leaves the SMs
+// short of threads; a sequence of one chunk has nothing to split.
+bool in_tiles(const ScanArgs& a, int sms) {
+  if (a.offsets != nullptr) return true;
+  if (a.steps <= kStateEvery) return false;
+  return a.batch * ((a.width + (a.vec ? 3 : 0)) / (a.vec ? 4 : 1)) < static_cast<int64_t>(sms) * 512;
 }
 
-void launch_scan_fwd(const ScanArgs& a, int sms, cudaStream_t st) {
+constexpr int64_t kSumRows = 64;  // above it the partial sums are added up in two launches
+int64_t partial_rows(const ScanArgs& a, int sms) {
+  return in_tiles(a, sms) ? scan_tiles_partials(a)
+                          : row_blocks(a, lanes_of(a.width, bwd_shape(a).V, false, 256, 256), sms);
+}
+
+}  // namespace
+
+size_t scan_workspace(const ScanArgs& a, int sms) { return in_tiles(a, sms) ? scan_tiles_workspace(a) : 0; }
+
+int64_t scan_partials(const ScanArgs& a, int sms) {
+  const int64_t n = partial_rows(a, sms);
+  return n > 8 * kSumRows ? n + kSumRows : n;
+}
+
+void launch_scan_fwd(const ScanArgs& a, int sms, void* workspace, cudaStream_t st) {
+  if (in_tiles(a, sms)) return launch_scan_tiles(a, false, workspace, st);
   count_launch();
   const bool codes = a.codes != nullptr;
   if (a.bf16)
@@ -347,16 +353,31 @@ void launch_scan_fwd(const ScanArgs& a, int sms, cudaStream_t st) {
     codes ? rows_fwd<float, true>(a, sms, st) : rows_fwd<float, false>(a, sms, st);
 }
 
-void launch_scan_bwd(const ScanArgs& a, int sms, void* ddecay, cudaStream_t st) {
-  count_launch();
+void launch_scan_bwd(const ScanArgs& a, int sms, void* workspace, void* ddecay, cudaStream_t st) {
   const bool codes = a.codes != nullptr;
-  if (a.bf16)
-    codes ? rows_bwd<__nv_bfloat16, true>(a, sms, st) : rows_bwd<__nv_bfloat16, false>(a, sms, st);
-  else
-    codes ? rows_bwd<float, true>(a, sms, st) : rows_bwd<float, false>(a, sms, st);
+  if (in_tiles(a, sms)) {
+    launch_scan_tiles(a, true, workspace, st);
+  } else {
+    count_launch();
+    if (a.bf16)
+      codes ? rows_bwd<__nv_bfloat16, true>(a, sms, st) : rows_bwd<__nv_bfloat16, false>(a, sms, st);
+    else
+      codes ? rows_bwd<float, true>(a, sms, st) : rows_bwd<float, false>(a, sms, st);
+  }
+  int64_t n = partial_rows(a, sms);
+  const float* from = a.partial;
+  const int cols = (a.width + 31) / 32;
+  const dim3 threads(32, 32);
+  if (n > 8 * kSumRows) {
+    float* to = a.partial + n * a.width;
+    count_launch();
+    scan_decay_grad_kernel<<<dim3(cols, kSumRows), threads, 0, st>>>(from, n, a.width, false, a.decay, a.decay_bf16,
+                                                                     a.rate, to);
+    from = to;
+    n = kSumRows;
+  }
   count_launch();
-  scan_decay_grad_kernel<<<(a.width + 31) / 32, dim3(32, 32), 0, st>>>(a.partial, a.n_partial, a.width, a.decay,
-                                                                       a.decay_bf16, a.rate, ddecay);
+  scan_decay_grad_kernel<<<cols, threads, 0, st>>>(from, n, a.width, true, a.decay, a.decay_bf16, a.rate, ddecay);
 }
 
 void launch_scan_step(const ScanStepArgs& a, cudaStream_t st) {

@@ -113,6 +113,12 @@ at::Tensor dense_rows(const ScanSizes& z, int64_t width, bool time_major, const 
   return at::empty({z.batch, z.steps, width}, o);
 }
 
+// stream-ordered, as every temporary here: the caching allocator reuses it after the call
+at::Tensor scan_workspace_of(const ScanArgs& a, int sms, const at::TensorOptions& o) {
+  const size_t bytes = scan_workspace(a, sms);
+  return bytes == 0 ? at::Tensor() : at::empty({static_cast<int64_t>(bytes)}, o.dtype(at::kByte));
+}
+
 int64_t groups_of(int64_t width) { return (width + kGroup8 - 1) / kGroup8; }
 
 }  // namespace
@@ -149,7 +155,9 @@ std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& de
     a.scales = scales.data_ptr<float>();
   }
   if (z.batch > 0) {
-    launch_scan_fwd(a, num_sms(p.get_device()), cur_stream());
+    const int sms = num_sms(p.get_device());
+    at::Tensor work = scan_workspace_of(a, sms, p.options());
+    launch_scan_fwd(a, sms, work.defined() ? work.data_ptr() : nullptr, cur_stream());
     SU_LAUNCH_CHECK();
   }
   return {h, last, states, codes, scales};
@@ -207,10 +215,10 @@ std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptTensor& 
     return {dp, ddecay, dh0};
   }
   const int sms = num_sms(like.get_device());
-  a.n_partial = scan_partials(a, sms);
-  at::Tensor partial = at::empty({a.n_partial, z.width}, f32);
+  at::Tensor partial = at::empty({scan_partials(a, sms), z.width}, f32);
   a.partial = partial.data_ptr<float>();
-  launch_scan_bwd(a, sms, ddecay.data_ptr(), cur_stream());
+  at::Tensor work = scan_workspace_of(a, sms, like.options());
+  launch_scan_bwd(a, sms, work.defined() ? work.data_ptr() : nullptr, ddecay.data_ptr(), cur_stream());
   SU_LAUNCH_CHECK();
   return {dp, ddecay, dh0};
 }

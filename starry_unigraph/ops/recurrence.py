@@ -153,7 +153,7 @@ def gated_scan(p: torch.Tensor, decay: torch.Tensor, h0: torch.Tensor | None = N
     mask: bool ``[batch, steps]`` (packed ``[rows]``); a False step returns the state before
     it, reads nothing of p and gets no gradient. offsets: int64 ``[batch + 1]`` rising from 0
     to ``rows``; empty sequences return their first state. On CUDA, offsets that do not
-    rise or leave the rows are reported by ``check_status()``, and their sequences skipped.
+    rise or leave the rows are reported by ``check_status()``; results are then undefined.
     h has p's type and layout; ``last`` is the fp32 state after each sequence.
 
     checkpoint="int8" keeps p in 8 bits (``quantize8``'s format, each of x, r and i in groups
