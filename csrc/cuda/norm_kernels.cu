@@ -99,22 +99,22 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const NormArgs A, const 
       for (int j = 0; j < NV; ++j) {
         const int c = (j * M.size + lane) * V;
         const bool live = in && c < H;
-        int8_t code[V];
+        Codes<V> q;
         int8_t* to = A.codes + row * H + c;
         float* ts = A.scales + row * G + c / kGroup8;
         const int64_t part = A.rows * H, spart = A.rows * G;
         const bool first = live && c % kGroup8 == 0;
-        float s = encode8(x[j], code);
-        if (live) store_codes(to, code);
+        float s = encode8(x[j], q);
+        if (live) q.store(to);
         if (first) ts[0] = s;
         if (A.u != nullptr) {
-          s = encode8(u[j], code);
-          if (live) store_codes(to + part, code);
+          s = encode8(u[j], q);
+          if (live) q.store(to + part);
           if (first) ts[spart] = s;
         }
         if (A.gate != nullptr) {
-          s = encode8(g[j], code);
-          if (live) store_codes(to + 2 * part, code);
+          s = encode8(g[j], q);
+          if (live) q.store(to + 2 * part);
           if (first) ts[2 * spart] = s;
         }
       }
@@ -205,9 +205,17 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const 
           const int8_t* from = A.codes + row * H + c;
           const float* fs = A.scales + row * G + c / kGroup8;
           const int64_t part = A.rows * H, spart = A.rows * G;
-          load_codes(from, fs[0], x[j]);
-          if (A.u != nullptr) load_codes(from + part, fs[spart], u[j]);
-          if (A.gate != nullptr) load_codes(from + 2 * part, fs[2 * spart], g[j]);
+          Codes<V> q;
+          q.load(from);
+          q.get(fs[0], x[j]);
+          if (A.u != nullptr) {
+            q.load(from + part);
+            q.get(fs[spart], u[j]);
+          }
+          if (A.gate != nullptr) {
+            q.load(from + 2 * part);
+            q.get(fs[2 * spart], g[j]);
+          }
         } else {
           a.load(static_cast<const T*>(A.x) + row * A.x_ld + c);
           a.get(x[j]);

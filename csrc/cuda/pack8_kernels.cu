@@ -26,9 +26,9 @@ __global__ void __launch_bounds__(256) quantize8_kernel(const T* __restrict__ x,
     if (live) a.load(x + row * ld + c);
     float f[V];
     a.get(f);
-    int8_t code[V];
-    const float s = encode8(f, code);
-    if (live) store_codes(codes + row * H + c, code);
+    Codes<V> q;
+    const float s = encode8(f, q);
+    if (live) q.store(codes + row * H + c);
     if (lane == 0) scales[g] = s;
   }
 }
@@ -45,7 +45,9 @@ __global__ void __launch_bounds__(256) dequantize8_kernel(const int8_t* __restri
     const int64_t row = e / lanes;
     const int c = static_cast<int>(e - row * lanes) * V;
     float f[V];
-    load_codes(codes + row * H + c, scales[row * G + c / kGroup8], f);
+    Codes<V> q;
+    q.load(codes + row * H + c);
+    q.get(scales[row * G + c / kGroup8], f);
     Pack<T, V> o;
     o.set(f);
     o.store(x + row * H + c);

@@ -49,14 +49,14 @@ struct ScanArgs {
 };
 
 // Bytes of workspace that a call needs (16-byte aligned, no initial value).
-size_t scan_workspace(const ScanArgs& a, int sms);
+size_t scan_workspace(const ScanArgs& a, bool bwd, int sms);
 // Rows of `partial` that the backward pass writes, the ones it adds them up in included.
 int64_t scan_partials(const ScanArgs& a, int sms);
 void launch_scan_fwd(const ScanArgs& a, int sms, void* workspace, cudaStream_t st);
 // also adds `partial` up into ddecay [H] (in the type of decay)
 void launch_scan_bwd(const ScanArgs& a, int sms, void* workspace, void* ddecay, cudaStream_t st);
 // the form that splits the steps into tiles (scan_tiles.cu)
-size_t scan_tiles_workspace(const ScanArgs& a);
+size_t scan_tiles_workspace(const ScanArgs& a, bool bwd);
 int64_t scan_tiles_partials(const ScanArgs& a);
 void launch_scan_tiles(const ScanArgs& a, bool bwd, void* workspace, cudaStream_t st);
 

@@ -7,10 +7,9 @@
 namespace su {
 namespace {
 
-// ---------------------------------------------------------------------------
-// A thread walks its V channels of one sequence after another.
-// ---------------------------------------------------------------------------
-template <class T, int V, int U, bool CODES>
+// Forward by U steps: their inputs are loaded together, so that U x 3 loads of 4 V (fp32)
+// bytes are under way per thread.
+template <class T, int V, int U, bool CODES, bool MASK>
 __global__ void __launch_bounds__(256) scan_rows_fwd_kernel(const ScanArgs A, const Lanes L) {
   const int y = threadIdx.x / L.count;
   const int c = (blockIdx.y * L.count + threadIdx.x % L.count) * V;
@@ -18,76 +17,78 @@ __global__ void __launch_bounds__(256) scan_rows_fwd_kernel(const ScanArgs A, co
   if (!CODES && !live) return;
   const int H = A.width;
   const int G = (H + kGroup8 - 1) / kGroup8;
+  const int steps = static_cast<int>(A.steps);
   float k[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) k[v] = live ? decay_factor(param_at(A.decay, A.decay_bf16, c + v), A.rate) : 0.f;
-  const T* P = static_cast<const T*>(A.p) + c;
-  T* Hout = static_cast<T*>(A.h) + c;
   for (int64_t s = static_cast<int64_t>(blockIdx.x) * L.rows + y; s < A.batch;
        s += static_cast<int64_t>(gridDim.x) * L.rows) {
+    const T* in = static_cast<const T*>(A.p) + s * A.p_sb + c;
+    const uint8_t* valid = MASK ? A.mask + s * A.m_sb : nullptr;
+    T* out = static_cast<T*>(A.h) + s * A.row_sb * H + c;
+    int8_t* code = CODES ? A.codes + s * A.row_sb * 3 * H + c : nullptr;
+    float* scale = CODES ? A.scales + s * A.row_sb * 3 * G + c / kGroup8 : nullptr;
     float h[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = (live && A.h0 != nullptr) ? A.h0[s * H + c + v] : 0.f;
-    for (int64_t t0 = 0; t0 < A.steps; t0 += U) {
+    for (int t0 = 0; t0 < steps; t0 += U) {
       Pack<T, V> x[U], r[U], i[U];
       bool on[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int64_t t = t0 + j;
-        on[j] = t < A.steps && (A.mask == nullptr || A.mask[s * A.m_sb + t * A.m_st] != 0);
+        on[j] = t0 + j < steps && (!MASK || *valid != 0);
         x[j].zero();
         r[j].zero();
         i[j].zero();
         if (on[j] && live) {
-          const T* row = P + s * A.p_sb + t * A.p_st;
-          x[j].load(row);
-          r[j].load(row + H);
-          i[j].load(row + 2 * H);
+          x[j].load(in);
+          r[j].load(in + H);
+          i[j].load(in + 2 * H);
         }
+        in += A.p_st;
+        if (MASK && t0 + j + 1 < steps) valid += A.m_st;
+      }
+      if (A.states != nullptr && live && t0 > 0 && t0 % kStateEvery == 0) {  // U divides kStateEvery
+        float* to = A.states + (s * A.n_states + t0 / kStateEvery - 1) * H + c;
+#pragma unroll
+        for (int v = 0; v < V; ++v) to[v] = h[v];
       }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int64_t t = t0 + j;
-        if (t >= A.steps) break;
-        if (A.states != nullptr && live && t > 0 && t % kStateEvery == 0) {
-          float* to = A.states + (s * A.n_states + t / kStateEvery - 1) * H + c;
-#pragma unroll
-          for (int v = 0; v < V; ++v) to[v] = h[v];
-        }
+        if (t0 + j >= steps) break;
         float fx[V], fr[V], fi[V];
         x[j].get(fx);
         r[j].get(fr);
         i[j].get(fi);
-        const int64_t row = s * A.row_sb + t * A.row_st;
         if constexpr (CODES) {
-          int8_t code[V];
-          int8_t* to = A.codes + row * 3 * H + c;
-          float* sc = A.scales + (row * 3) * G + c / kGroup8;
-          const bool first = (c % kGroup8) == 0 && live;
-          const float s0 = encode8(fx, code);
-          if (live) store_codes(to, code);
-          const float s1 = encode8(fr, code);
-          if (live) store_codes(to + H, code);
-          const float s2 = encode8(fi, code);
-          if (live) store_codes(to + 2 * H, code);
-          if (first) {
-            sc[0] = s0;
-            sc[G] = s1;
-            sc[2 * G] = s2;
+          Codes<V> q[3];
+          const float s0 = encode8(fx, q[0]), s1 = encode8(fr, q[1]), s2 = encode8(fi, q[2]);
+          if (live) {
+            q[0].store(code);
+            q[1].store(code + H);
+            q[2].store(code + 2 * H);
+            if (c % kGroup8 == 0) {
+              scale[0] = s0;
+              scale[G] = s1;
+              scale[2 * G] = s2;
+            }
           }
+          code += A.row_st * 3 * H;
+          scale += A.row_st * 3 * G;
         }
-        if (on[j]) {
+        if (!MASK || on[j]) {
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const Step g = step_of(fr[v], fi[v], k[v]);
-            h[v] = fmaf(g.a, h[v], approx_sqrt(g.ss) * g.si * fx[v]);
+            const Step g = step_of(fx[v], fr[v], fi[v], k[v]);
+            h[v] = fmaf(g.a, h[v], g.add);
           }
         }
         if (live) {
           Pack<T, V> o;
           o.set(h);
-          o.store(Hout + row * H);
+          o.store(out);
         }
+        out += A.row_st * H;
       }
     }
     if (live) {
@@ -97,16 +98,19 @@ __global__ void __launch_bounds__(256) scan_rows_fwd_kernel(const ScanArgs A, co
   }
 }
 
-// Backwards by chunks of CH steps (kStateEvery, or fewer where the sequence has no more):
-// the states inside a chunk are recomputed from the state before it and kept in registers.
-template <class T, int V, int CH, bool CODES>
-__global__ void __launch_bounds__(256) scan_rows_bwd_kernel(const ScanArgs A, const Lanes L) {
+// Backwards by chunks of CH steps (kStateEvery, or fewer where the sequence has no more).
+// Every gradient of a step is g times a factor that the inputs and the state before the
+// step give: the chunk is walked forwards from its first state for the factors, which stay
+// in registers, and then backwards for g. The gates are evaluated once.
+template <class T, int V, int CH, bool CODES, bool MASK>
+__global__ void __launch_bounds__(256, 2) scan_rows_bwd_kernel(const ScanArgs A, const Lanes L) {
   const int y = threadIdx.x / L.count;
   const int lane_c = threadIdx.x % L.count;
   const int c = (blockIdx.y * L.count + lane_c) * V;
   const bool live = c < A.width;
   const int H = A.width;
   const int G = (H + kGroup8 - 1) / kGroup8;
+  const int steps = static_cast<int>(A.steps);
   float k[V], dl[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -119,84 +123,96 @@ __global__ void __launch_bounds__(256) scan_rows_bwd_kernel(const ScanArgs A, co
       float E[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) E[v] = A.dlast != nullptr ? A.dlast[s * H + c + v] : 0.f;
-      for (int64_t tc = (A.steps + CH - 1) / CH * CH - CH; tc >= 0; tc -= CH) {
-        float x[CH][V], r[CH][V], i[CH][V], d[CH][V], before[CH][V];
-        bool in[CH], on[CH];
+      for (int tc = (steps + CH - 1) / CH * CH - CH; tc >= 0; tc -= CH) {
+        const int64_t row = s * A.row_sb + tc * A.row_st;
+        Pack<T, V> x[CH], r[CH], i[CH], d[CH];
+        Codes<V> qx[CH], qr[CH], qi[CH];
+        float sx[CH], sr[CH], si[CH];
+        bool on[CH];
+        const T* in = CODES ? nullptr : static_cast<const T*>(A.p) + s * A.p_sb + tc * A.p_st + c;
+        const T* dh = static_cast<const T*>(A.dh) + (A.dh != nullptr ? s * A.dh_sb + tc * A.dh_st + c : 0);
+        const int8_t* code = CODES ? A.codes + row * 3 * H + c : nullptr;
+        const float* scale = CODES ? A.scales + row * 3 * G + c / kGroup8 : nullptr;
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
-          const int64_t t = tc + j;
-          in[j] = t < A.steps;
-          on[j] = in[j] && (A.mask == nullptr || A.mask[s * A.m_sb + t * A.m_st] != 0);
-#pragma unroll
-          for (int v = 0; v < V; ++v) x[j][v] = r[j][v] = i[j][v] = d[j][v] = 0.f;
-          if (on[j]) {
-            if constexpr (CODES) {
-              const int64_t row = s * A.row_sb + t * A.row_st;
-              const int8_t* from = A.codes + row * 3 * H + c;
-              const float* sc = A.scales + row * 3 * G + c / kGroup8;
-              load_codes(from, sc[0], x[j]);
-              load_codes(from + H, sc[G], r[j]);
-              load_codes(from + 2 * H, sc[2 * G], i[j]);
-            } else {
-              const T* row = static_cast<const T*>(A.p) + s * A.p_sb + t * A.p_st + c;
-              Pack<T, V> w;
-              w.load(row);
-              w.get(x[j]);
-              w.load(row + H);
-              w.get(r[j]);
-              w.load(row + 2 * H);
-              w.get(i[j]);
+          const bool inside = tc + j < steps;
+          on[j] = inside && (!MASK || A.mask[s * A.m_sb + (tc + j) * A.m_st] != 0);
+          d[j].zero();
+          if constexpr (CODES) {
+            qx[j].zero();
+            qr[j].zero();
+            qi[j].zero();
+            sx[j] = sr[j] = si[j] = 0.f;
+            if (on[j]) {
+              qx[j].load(code);
+              qr[j].load(code + H);
+              qi[j].load(code + 2 * H);
+              sx[j] = scale[0];
+              sr[j] = scale[G];
+              si[j] = scale[2 * G];
             }
+            code += A.row_st * 3 * H;
+            scale += A.row_st * 3 * G;
+          } else {
+            x[j].zero();
+            r[j].zero();
+            i[j].zero();
+            if (on[j]) {
+              x[j].load(in);
+              r[j].load(in + H);
+              i[j].load(in + 2 * H);
+            }
+            in += A.p_st;
           }
-          if (in[j] && A.dh != nullptr) {
-            Pack<T, V> w;
-            w.load(static_cast<const T*>(A.dh) + s * A.dh_sb + t * A.dh_st + c);
-            w.get(d[j]);
-          }
+          if (inside && A.dh != nullptr) d[j].load(dh);
+          dh += A.dh_st;
         }
         float h[V];
-        if (tc > 0) {
-          const float* from = A.states + (s * A.n_states + tc / kStateEvery - 1) * H + c;
+        const float* from = tc > 0 ? A.states + (s * A.n_states + tc / kStateEvery - 1) * H + c
+                                   : (A.h0 != nullptr ? A.h0 + s * H + c : nullptr);
 #pragma unroll
-          for (int v = 0; v < V; ++v) h[v] = from[v];
-        } else {
-#pragma unroll
-          for (int v = 0; v < V; ++v) h[v] = A.h0 != nullptr ? A.h0[s * H + c + v] : 0.f;
-        }
+        for (int v = 0; v < V; ++v) h[v] = from != nullptr ? from[v] : 0.f;
+        Slope f[CH][V];
 #pragma unroll
         for (int j = 0; j < CH; ++j) {
+          float fx[V], fr[V], fi[V];
+          if constexpr (CODES) {
+            qx[j].get(sx[j], fx);
+            qr[j].get(sr[j], fr);
+            qi[j].get(si[j], fi);
+          } else {
+            x[j].get(fx);
+            r[j].get(fr);
+            i[j].get(fi);
+          }
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            before[j][v] = h[v];
-            if (on[j]) {
-              const Step g = step_of(r[j][v], i[j][v], k[v]);
-              h[v] = fmaf(g.a, h[v], approx_sqrt(g.ss) * g.si * x[j][v]);
-            }
+            f[j][v] = slope_of(on[j] ? gate_of(fx[v], fr[v], fi[v], k[v]) : gate_shut(), h[v]);
           }
         }
+        T* out = static_cast<T*>(A.dp) + (row + CH * A.row_st) * 3 * H + c;
 #pragma unroll
         for (int j = CH - 1; j >= 0; --j) {
-          if (!in[j]) continue;
-          const int64_t row = s * A.row_sb + (tc + j) * A.row_st;
-          float dx[V], dr[V], di[V];
+          out -= A.row_st * 3 * H;
+          if (tc + j >= steps) continue;
+          float dy[V], dx[V], dr[V], di[V];
+          d[j].get(dy);
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const float g = d[j][v] + E[v];
-            if (on[j]) {
-              E[v] = step_grad(step_of(r[j][v], i[j][v], k[v]), x[j][v], before[j][v], g, dx[v], dr[v], di[v], dl[v]);
-            } else {
-              E[v] = g;
-              dx[v] = dr[v] = di[v] = 0.f;
-            }
+            const float g = dy[v] + E[v];
+            dx[v] = g * f[j][v].x;
+            dr[v] = g * f[j][v].r;
+            di[v] = g * f[j][v].i;
+            dl[v] = fmaf(g, f[j][v].l, dl[v]);
+            E[v] = g * f[j][v].a;
           }
-          T* to = static_cast<T*>(A.dp) + row * 3 * H + c;
           Pack<T, V> o;
           o.set(dx);
-          o.store(to);
+          o.store(out);
           o.set(dr);
-          o.store(to + H);
+          o.store(out + H);
           o.set(di);
-          o.store(to + 2 * H);
+          o.store(out + 2 * H);
         }
       }
       if (A.dh0 != nullptr) {
@@ -260,8 +276,8 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanStepArgs A) {
     record_status(A.status, kBadIndex);  // the row is left out
   } else {
     float* to = A.state + at * A.state_sb + c;
-    const Step g = step_of(r, i, k);
-    h = fmaf(g.a, *to, approx_sqrt(g.ss) * g.si * x);
+    const Step g = step_of(x, r, i, k);
+    h = fmaf(g.a, *to, g.add);
     *to = h;
   }
   static_cast<T*>(A.h)[e] = from_f32<T>(h);
@@ -277,26 +293,25 @@ int row_blocks(const ScanArgs& a, const Lanes& l, int sms) {
 struct BwdShape {
   int V, CH;
 };
-// 16 bytes of a channel per thread and step where the whole sequence is one short chunk,
-// 4 bytes where 16 steps of inputs and states have to stay in registers
+// 16 steps' factors of one channel fit the registers, so do 8 of two and 4 of four
 BwdShape bwd_shape(const ScanArgs& a) {
   if (a.steps <= 4) return {a.vec ? 4 : 1, 4};
   if (a.steps <= 8) return {a.vec ? 2 : 1, 8};
-  return {a.vec && a.bf16 ? 2 : 1, kStateEvery};
+  return {1, kStateEvery};
 }
 
-template <class T, bool CODES>
+template <class T, bool CODES, bool MASK>
 void rows_fwd(const ScanArgs& a, int sms, cudaStream_t st) {
   const Lanes l = lanes_of(a.width, a.vec ? 4 : 1, CODES, 256, 256);
   const dim3 grid(row_blocks(a, l, sms), l.blocks);
   const int threads = l.count * l.rows;
   if (a.vec)
-    scan_rows_fwd_kernel<T, 4, 4, CODES><<<grid, threads, 0, st>>>(a, l);
+    scan_rows_fwd_kernel<T, 4, 4, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
   else
-    scan_rows_fwd_kernel<T, 1, 8, CODES><<<grid, threads, 0, st>>>(a, l);
+    scan_rows_fwd_kernel<T, 1, 8, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
 }
 
-template <class T, bool CODES>
+template <class T, bool CODES, bool MASK>
 void rows_bwd(const ScanArgs& a, int sms, cudaStream_t st) {
   const BwdShape b = bwd_shape(a);
   const Lanes l = lanes_of(a.width, b.V, false, 256, 256);
@@ -304,31 +319,44 @@ void rows_bwd(const ScanArgs& a, int sms, cudaStream_t st) {
   const int threads = l.count * l.rows;
   if (b.CH == 4) {
     if (b.V == 4)
-      scan_rows_bwd_kernel<T, 4, 4, CODES><<<grid, threads, 0, st>>>(a, l);
+      scan_rows_bwd_kernel<T, 4, 4, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
     else
-      scan_rows_bwd_kernel<T, 1, 4, CODES><<<grid, threads, 0, st>>>(a, l);
+      scan_rows_bwd_kernel<T, 1, 4, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
   } else if (b.CH == 8) {
     if (b.V == 2)
-      scan_rows_bwd_kernel<T, 2, 8, CODES><<<grid, threads, 0, st>>>(a, l);
+      scan_rows_bwd_kernel<T, 2, 8, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
     else
-      scan_rows_bwd_kernel<T, 1, 8, CODES><<<grid, threads, 0, st>>>(a, l);
+      scan_rows_bwd_kernel<T, 1, 8, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
   } else {
-    if (b.V == 2)
-      scan_rows_bwd_kernel<T, 2, kStateEvery, CODES><<<grid, threads, 0, st>>>(a, l);
-    else
-      scan_rows_bwd_kernel<T, 1, kStateEvery, CODES><<<grid, threads, 0, st>>>(a, l);
+    scan_rows_bwd_kernel<T, 1, kStateEvery, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
   }
+}
+
+template <class T, bool CODES>
+void rows_run(const ScanArgs& a, bool bwd, int sms, cudaStream_t st) {
+  if (a.mask != nullptr)
+    bwd ? rows_bwd<T, CODES, true>(a, sms, st) : rows_fwd<T, CODES, true>(a, sms, st);
+  else
+    bwd ? rows_bwd<T, CODES, false>(a, sms, st) : rows_fwd<T, CODES, false>(a, sms, st);
+}
+void rows_launch(const ScanArgs& a, bool bwd, int sms, cudaStream_t st) {
+  count_launch();
+  const bool codes = a.codes != nullptr;
+  if (a.bf16)
+    codes ? rows_run<__nv_bfloat16, true>(a, bwd, sms, st) : rows_run<__nv_bfloat16, false>(a, bwd, sms, st);
+  else
+    codes ? rows_run<float, true>(a, bwd, sms, st) : rows_run<float, false>(a, bwd, sms, st);
 }
 
 // Tiles for packed sequences, and where a thread per sequence and 4 channels leaves the SMs
 // short of threads; a sequence of one chunk has nothing to split.
 bool in_tiles(const ScanArgs& a, int sms) {
-  if (a.offsets != nullptr) return true;
+  if (a.offsets != nullptr || a.steps > (1 << 30)) return true;
   if (a.steps <= kStateEvery) return false;
   return a.batch * ((a.width + (a.vec ? 3 : 0)) / (a.vec ? 4 : 1)) < static_cast<int64_t>(sms) * 512;
 }
 
-constexpr int64_t kSumRows = 64;  // above it the partial sums are added up in two launches
+constexpr int64_t kSumRows = 64;  // above 8 times it the partial sums are added up in two launches
 int64_t partial_rows(const ScanArgs& a, int sms) {
   return in_tiles(a, sms) ? scan_tiles_partials(a)
                           : row_blocks(a, lanes_of(a.width, bwd_shape(a).V, false, 256, 256), sms);
@@ -336,7 +364,9 @@ int64_t partial_rows(const ScanArgs& a, int sms) {
 
 }  // namespace
 
-size_t scan_workspace(const ScanArgs& a, int sms) { return in_tiles(a, sms) ? scan_tiles_workspace(a) : 0; }
+size_t scan_workspace(const ScanArgs& a, bool bwd, int sms) {
+  return in_tiles(a, sms) ? scan_tiles_workspace(a, bwd) : 0;
+}
 
 int64_t scan_partials(const ScanArgs& a, int sms) {
   const int64_t n = partial_rows(a, sms);
@@ -344,26 +374,17 @@ int64_t scan_partials(const ScanArgs& a, int sms) {
 }
 
 void launch_scan_fwd(const ScanArgs& a, int sms, void* workspace, cudaStream_t st) {
-  if (in_tiles(a, sms)) return launch_scan_tiles(a, false, workspace, st);
-  count_launch();
-  const bool codes = a.codes != nullptr;
-  if (a.bf16)
-    codes ? rows_fwd<__nv_bfloat16, true>(a, sms, st) : rows_fwd<__nv_bfloat16, false>(a, sms, st);
+  if (in_tiles(a, sms))
+    launch_scan_tiles(a, false, workspace, st);
   else
-    codes ? rows_fwd<float, true>(a, sms, st) : rows_fwd<float, false>(a, sms, st);
+    rows_launch(a, false, sms, st);
 }
 
 void launch_scan_bwd(const ScanArgs& a, int sms, void* workspace, void* ddecay, cudaStream_t st) {
-  const bool codes = a.codes != nullptr;
-  if (in_tiles(a, sms)) {
+  if (in_tiles(a, sms))
     launch_scan_tiles(a, true, workspace, st);
-  } else {
-    count_launch();
-    if (a.bf16)
-      codes ? rows_bwd<__nv_bfloat16, true>(a, sms, st) : rows_bwd<__nv_bfloat16, false>(a, sms, st);
-    else
-      codes ? rows_bwd<float, true>(a, sms, st) : rows_bwd<float, false>(a, sms, st);
-  }
+  else
+    rows_launch(a, true, sms, st);
   int64_t n = partial_rows(a, sms);
   const float* from = a.partial;
   const int cols = (a.width + 31) / 32;

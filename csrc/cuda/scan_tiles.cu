@@ -1,7 +1,7 @@
 // The gated linear recurrence split over its steps: for few or unequal sequences, whose
 // channels alone do not fill the GPU. One pass over the data.
 //
-// A tile is kStateEvery steps for each of `rows` neighbouring threads times 32 or fewer
+// A tile is kRun steps for each of `rows` neighbouring threads times 32 or fewer
 // lanes of channels; it is loaded once and stays in registers. A run of steps maps the
 // state before it to A h + B, and two runs compose to (A2 A1, A2 B1 + B2). A tile
 // composes its threads' runs in shared memory, publishes (A, B), obtains the state before
@@ -25,6 +25,7 @@
 namespace su {
 namespace {
 
+constexpr int kRun = 8;                        // steps per thread; divides kStateEvery by 2
 constexpr int kFan = 16;                       // tiles per group, groups per block
 constexpr long long kCarryBudget = 400000000;  // cycles, ~0.2 s
 
@@ -264,9 +265,10 @@ __device__ __forceinline__ void tile_carry(const TileShape& S, const TileWork& W
   for (int v = 0; v < V; ++v) h[v] = maps[p.y * width + p.x * V + v].x;
 }
 
-template <class T, int V, bool CODES>
-__global__ void __launch_bounds__(256, 2) scan_tiles_fwd_kernel(const ScanArgs A, const TileShape S, const TileWork W) {
-  constexpr int K = kStateEvery;
+template <class T, int V, bool CODES, bool PACKED, bool MASK>
+__global__ void __launch_bounds__(256, V == 1 ? 4 : 3)
+    scan_tiles_fwd_kernel(const ScanArgs A, const TileShape S, const TileWork W) {
+  constexpr int K = kRun;
   extern __shared__ float2 smem[];
   float2* maps = smem;
   int* first = reinterpret_cast<int*>(maps + S.l.rows * S.l.count * V);
@@ -276,70 +278,74 @@ __global__ void __launch_bounds__(256, 2) scan_tiles_fwd_kernel(const ScanArgs A
   const Place p = place_of<V>(S, W, H);
   const int64_t tile0 = p.j * S.l.rows * K;
   const int64_t t0 = tile0 + p.y * K;
-  const bool packed = A.offsets != nullptr;
+  const int n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(K), A.steps - t0)));
   Pack<T, V> x[K], r[K], i[K];
   unsigned on = 0;
+  {
+    const T* in = static_cast<const T*>(A.p) + p.b * A.p_sb + t0 * A.p_st + p.c;
+    const uint8_t* valid = MASK ? A.mask + p.b * A.m_sb + t0 * A.m_st : nullptr;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int64_t t = t0 + k;
-    x[k].zero();
-    r[k].zero();
-    i[k].zero();
-    if (t < A.steps && p.live && (A.mask == nullptr || A.mask[p.b * A.m_sb + t * A.m_st] != 0)) {
-      on |= 1u << k;
-      const T* row = static_cast<const T*>(A.p) + p.b * A.p_sb + t * A.p_st + p.c;
-      x[k].load(row);
-      r[k].load(row + H);
-      i[k].load(row + 2 * H);
+    for (int k = 0; k < K; ++k) {
+      x[k].zero();
+      r[k].zero();
+      i[k].zero();
+      if (k < n && p.live && (!MASK || *valid != 0)) {
+        on |= 1u << k;
+        x[k].load(in);
+        r[k].load(in + H);
+        i[k].load(in + 2 * H);
+      }
+      in += A.p_st;
+      if (MASK) valid += A.m_st;
     }
   }
-  if (packed) mark_sequences(A, tile0, S.l.rows * K, first, last);
+  if (PACKED) mark_sequences(A, tile0, S.l.rows * K, first, last);
   float kd[V], init[V], a[K][V], add[K][V], ra[V], rb[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     kd[v] = p.live ? decay_factor(param_at(A.decay, A.decay_bf16, p.c + v), A.rate) : 0.f;
-    init[v] = (!packed && p.live && A.h0 != nullptr) ? A.h0[p.b * H + p.c + v] : 0.f;
+    init[v] = (!PACKED && p.live && A.h0 != nullptr) ? A.h0[p.b * H + p.c + v] : 0.f;
     ra[v] = 1.f;
     rb[v] = 0.f;
   }
+  const int64_t row0 = p.b * A.row_sb + t0 * A.row_st;
+  int8_t* code = CODES ? A.codes + row0 * 3 * H + p.c : nullptr;
+  float* scale = CODES ? A.scales + row0 * 3 * G + p.c / kGroup8 : nullptr;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int64_t t = t0 + k;
     float fx[V], fr[V], fi[V];
     x[k].get(fx);
     r[k].get(fr);
     i[k].get(fi);
     if constexpr (CODES) {
-      if (t < A.steps) {  // the same for all lanes of a group
-        const int64_t row = p.b * A.row_sb + t * A.row_st;
-        int8_t code[V];
-        int8_t* to = A.codes + row * 3 * H + p.c;
-        float* sc = A.scales + row * 3 * G + p.c / kGroup8;
-        const bool head = p.live && p.c % kGroup8 == 0;
-        const float s0 = encode8(fx, code);
-        if (p.live) store_codes(to, code);
-        const float s1 = encode8(fr, code);
-        if (p.live) store_codes(to + H, code);
-        const float s2 = encode8(fi, code);
-        if (p.live) store_codes(to + 2 * H, code);
-        if (head) {
-          sc[0] = s0;
-          sc[G] = s1;
-          sc[2 * G] = s2;
+      if (k < n) {  // the same for all lanes of a group
+        Codes<V> q0, q1, q2;
+        const float s0 = encode8(fx, q0), s1 = encode8(fr, q1), s2 = encode8(fi, q2);
+        if (p.live) {
+          q0.store(code);
+          q1.store(code + H);
+          q2.store(code + 2 * H);
+          if (p.c % kGroup8 == 0) {
+            scale[0] = s0;
+            scale[G] = s1;
+            scale[2 * G] = s2;
+          }
         }
       }
+      code += A.row_st * 3 * H;
+      scale += A.row_st * 3 * G;
     }
-    const int from = packed && t < A.steps ? first[p.y * K + k] : -1;
+    const int from = PACKED ? first[p.y * K + k] : -1;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       a[k][v] = 1.f;
       add[k][v] = 0.f;
       if (on >> k & 1) {
-        const Step g = step_of(fr[v], fi[v], kd[v]);
+        const Step g = step_of(fx[v], fr[v], fi[v], kd[v]);
         a[k][v] = g.a;
-        add[k][v] = approx_sqrt(g.ss) * g.si * fx[v];
+        add[k][v] = g.add;
       }
-      if (from >= 0) {
+      if (PACKED && from >= 0) {
         ra[v] = 0.f;
         rb[v] = (p.live && A.h0 != nullptr) ? A.h0[static_cast<int64_t>(from) * H + p.c + v] : 0.f;
       }
@@ -350,265 +356,255 @@ __global__ void __launch_bounds__(256, 2) scan_tiles_fwd_kernel(const ScanArgs A
   float h[V];
   tile_carry<V>(S, W, p, ra, rb, init, maps, h, A.status);
   if (!p.live) return;
-  if (A.states != nullptr && t0 > 0 && t0 < A.steps) {
-    float* to = A.states + (p.b * A.n_states + t0 / K - 1) * H + p.c;
+  if (A.states != nullptr && t0 > 0 && t0 % kStateEvery == 0 && n > 0) {
+    float* to = A.states + (p.b * A.n_states + t0 / kStateEvery - 1) * H + p.c;
 #pragma unroll
     for (int v = 0; v < V; ++v) to[v] = h[v];
   }
+  T* out = static_cast<T*>(A.h) + row0 * H + p.c;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int64_t t = t0 + k;
-    if (t < A.steps) {
-      const int from = packed ? first[p.y * K + k] : -1;
+    if (k < n) {
+      const int from = PACKED ? first[p.y * K + k] : -1;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if (from >= 0) h[v] = A.h0 != nullptr ? A.h0[static_cast<int64_t>(from) * H + p.c + v] : 0.f;
+        if (PACKED && from >= 0) h[v] = A.h0 != nullptr ? A.h0[static_cast<int64_t>(from) * H + p.c + v] : 0.f;
         h[v] = fmaf(a[k][v], h[v], add[k][v]);
       }
       Pack<T, V> o;
       o.set(h);
-      o.store(static_cast<T*>(A.h) + (p.b * A.row_sb + t * A.row_st) * H + p.c);
-      const int64_t done = packed ? last[p.y * K + k] : (t == A.steps - 1 ? p.b : -1);
+      o.store(out);
+      const int64_t done = PACKED ? last[p.y * K + k] : (t0 + k == A.steps - 1 ? p.b : -1);
       if (done >= 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v) A.last[done * H + p.c + v] = h[v];
       }
     }
+    out += A.row_st * H;
   }
 }
 
 // Walks from the last step to the first: run y of tile j covers the steps that end
-// (j * rows + y) * K before the end of the last tile.
-template <class T, int V, bool CODES>
-__global__ void __launch_bounds__(256, 1) scan_tiles_bwd_kernel(const ScanArgs A, const TileShape S, const TileWork W) {
-  constexpr int K = kStateEvery;
+// (j * rows + y) * K before the end of the last tile. One channel per thread: the factors of
+// its steps' gradients, evaluated once, stay in registers.
+template <class T, bool CODES, bool PACKED, bool MASK>
+__global__ void __launch_bounds__(256, 2) scan_tiles_bwd_kernel(const ScanArgs A, const TileShape S, const TileWork W) {
+  constexpr int K = kRun;
   extern __shared__ float2 smem[];
   float2* maps = smem;
-  int* first = reinterpret_cast<int*>(maps + S.l.rows * S.l.count * V);
+  int* first = reinterpret_cast<int*>(maps + S.l.rows * S.l.count);
   int* last = first + S.l.rows * K;
   const int H = A.width;
   const int G = (H + kGroup8 - 1) / kGroup8;
-  const Place p = place_of<V>(S, W, H);
+  const Place p = place_of<1>(S, W, H);
   const int64_t tile = S.tiles - 1 - p.j;
   const int64_t tile0 = tile * S.l.rows * K;
   const int at0 = (S.l.rows - 1 - p.y) * K;  // inside the tile
   const int64_t t0 = tile0 + at0;
-  const bool packed = A.offsets != nullptr;
-  float x[K][V], r[K][V], i[K][V], d[K][V];
+  const int n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(K), A.steps - t0)));
+  const int64_t row0 = p.b * A.row_sb + t0 * A.row_st;
+  float x[K], r[K], i[K], d[K];
   unsigned on = 0;
+  {
+    const T* in = CODES ? nullptr : static_cast<const T*>(A.p) + p.b * A.p_sb + t0 * A.p_st + p.c;
+    const int8_t* code = CODES ? A.codes + row0 * 3 * H + p.c : nullptr;
+    const float* scale = CODES ? A.scales + row0 * 3 * G + p.c / kGroup8 : nullptr;
+    const T* dh = static_cast<const T*>(A.dh) + (A.dh != nullptr ? p.b * A.dh_sb + t0 * A.dh_st + p.c : 0);
+    const uint8_t* valid = MASK ? A.mask + p.b * A.m_sb + t0 * A.m_st : nullptr;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int64_t t = t0 + k;
-#pragma unroll
-    for (int v = 0; v < V; ++v) x[k][v] = r[k][v] = i[k][v] = d[k][v] = 0.f;
-    if (t < A.steps && p.live) {
-      if (A.mask == nullptr || A.mask[p.b * A.m_sb + t * A.m_st] != 0) {
-        on |= 1u << k;
-        if constexpr (CODES) {
-          const int64_t row = p.b * A.row_sb + t * A.row_st;
-          const int8_t* from = A.codes + row * 3 * H + p.c;
-          const float* sc = A.scales + row * 3 * G + p.c / kGroup8;
-          load_codes(from, sc[0], x[k]);
-          load_codes(from + H, sc[G], r[k]);
-          load_codes(from + 2 * H, sc[2 * G], i[k]);
-        } else {
-          const T* row = static_cast<const T*>(A.p) + p.b * A.p_sb + t * A.p_st + p.c;
-          Pack<T, V> w;
-          w.load(row);
-          w.get(x[k]);
-          w.load(row + H);
-          w.get(r[k]);
-          w.load(row + 2 * H);
-          w.get(i[k]);
+    for (int k = 0; k < K; ++k) {
+      x[k] = r[k] = i[k] = d[k] = 0.f;
+      if (k < n && p.live) {
+        if (!MASK || *valid != 0) {
+          on |= 1u << k;
+          if constexpr (CODES) {
+            Codes<1> q[3];
+            q[0].load(code);
+            q[1].load(code + H);
+            q[2].load(code + 2 * H);
+            float f[3][1];
+            q[0].get(scale[0], f[0]);
+            q[1].get(scale[G], f[1]);
+            q[2].get(scale[2 * G], f[2]);
+            x[k] = f[0][0];
+            r[k] = f[1][0];
+            i[k] = f[2][0];
+          } else {
+            x[k] = to_f32(__ldcs(in));
+            r[k] = to_f32(__ldcs(in + H));
+            i[k] = to_f32(__ldcs(in + 2 * H));
+          }
         }
+        if (A.dh != nullptr) d[k] = to_f32(__ldcs(dh));
       }
-      if (A.dh != nullptr) {
-        Pack<T, V> w;
-        w.load(static_cast<const T*>(A.dh) + p.b * A.dh_sb + t * A.dh_st + p.c);
-        w.get(d[k]);
-      }
-    }
-  }
-  float h[V];  // the state before the run
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    h[v] = 0.f;
-    if (p.live && t0 < A.steps) {
-      if (t0 > 0)
-        h[v] = A.states[(p.b * A.n_states + t0 / K - 1) * H + p.c + v];
-      else if (!packed && A.h0 != nullptr)
-        h[v] = A.h0[p.b * H + p.c + v];
-    }
-  }
-  if (packed) mark_sequences(A, tile0, S.l.rows * K, first, last);
-  float kd[V], init[V], ra[V], rb[V], dl[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    kd[v] = p.live ? decay_factor(param_at(A.decay, A.decay_bf16, p.c + v), A.rate) : 0.f;
-    init[v] = (!packed && p.live && A.dlast != nullptr) ? A.dlast[p.b * H + p.c + v] : 0.f;
-    ra[v] = 1.f;
-    rb[v] = 0.f;
-    dl[v] = 0.f;
-  }
-#pragma unroll
-  for (int k = K - 1; k >= 0; --k) {
-    if (t0 + k >= A.steps) continue;
-    const int to = packed ? last[at0 + k] : -1;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (to >= 0) {
-        ra[v] = 0.f;
-        rb[v] = (p.live && A.dlast != nullptr) ? A.dlast[static_cast<int64_t>(to) * H + p.c + v] : 0.f;
-      }
-      rb[v] += d[k][v];
-      if (on >> k & 1) {
-        const float a = 1.f - one_minus_exp(kd[v] * sigmoid_f(r[k][v]));
-        ra[v] *= a;
-        rb[v] *= a;
-      }
-    }
-  }
-  float E[V];
-  tile_carry<V>(S, W, p, ra, rb, init, maps, E, A.status);
-  float before[K][V];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    if (t0 + k >= A.steps) continue;
-    const int from = packed ? first[at0 + k] : -1;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (from >= 0) h[v] = (p.live && A.h0 != nullptr) ? A.h0[static_cast<int64_t>(from) * H + p.c + v] : 0.f;
-      before[k][v] = h[v];
-      if (on >> k & 1) {
-        const Step g = step_of(r[k][v], i[k][v], kd[v]);
-        h[v] = fmaf(g.a, h[v], approx_sqrt(g.ss) * g.si * x[k][v]);
-      }
-    }
-  }
-#pragma unroll
-  for (int k = K - 1; k >= 0; --k) {
-    const int64_t t = t0 + k;
-    if (t >= A.steps || !p.live) continue;
-    const int to = packed ? last[at0 + k] : -1;
-    float dx[V], dr[V], di[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      if (to >= 0) E[v] = A.dlast != nullptr ? A.dlast[static_cast<int64_t>(to) * H + p.c + v] : 0.f;
-      const float g = d[k][v] + E[v];
-      if (on >> k & 1) {
-        E[v] = step_grad(step_of(r[k][v], i[k][v], kd[v]), x[k][v], before[k][v], g, dx[v], dr[v], di[v], dl[v]);
+      if (CODES) {
+        code += A.row_st * 3 * H;
+        scale += A.row_st * 3 * G;
       } else {
-        E[v] = g;
-        dx[v] = dr[v] = di[v] = 0.f;
+        in += A.p_st;
       }
+      dh += A.dh_st;
+      if (MASK) valid += A.m_st;
     }
-    T* out = static_cast<T*>(A.dp) + (p.b * A.row_sb + t * A.row_st) * 3 * H + p.c;
-    Pack<T, V> o;
-    o.set(dx);
-    o.store(out);
-    o.set(dr);
-    o.store(out + H);
-    o.set(di);
-    o.store(out + 2 * H);
-    const int64_t begin = packed ? first[at0 + k] : (t == 0 ? p.b : -1);
-    if (begin >= 0 && A.dh0 != nullptr) {
+  }
+  // the state before the run: kept at every second run, handed on by the run before at the others
+  const bool kept = t0 % kStateEvery == 0;
+  float h = 0.f;
+  if (p.live && n > 0 && kept) {
+    if (t0 > 0)
+      h = A.states[(p.b * A.n_states + t0 / kStateEvery - 1) * H + p.c];
+    else if (!PACKED && A.h0 != nullptr)
+      h = A.h0[p.b * H + p.c];
+  }
+  if (PACKED) mark_sequences(A, tile0, S.l.rows * K, first, last);
+  const float kd = p.live ? decay_factor(param_at(A.decay, A.decay_bf16, p.c), A.rate) : 0.f;
+  Gate g[K];
 #pragma unroll
-      for (int v = 0; v < V; ++v) A.dh0[begin * H + p.c + v] = E[v];
+  for (int k = 0; k < K; ++k) g[k] = on >> k & 1 ? gate_of(x[k], r[k], i[k], kd) : gate_shut();
+  Slope f[K];
+  auto walk = [&]() {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int from = PACKED ? first[at0 + k] : -1;
+      if (PACKED && from >= 0) h = (p.live && A.h0 != nullptr) ? A.h0[static_cast<int64_t>(from) * H + p.c] : 0.f;
+      f[k] = slope_of(g[k], h);
+    }
+  };
+  float* handed = &maps[p.y * S.l.count + p.x].x;
+  if (kept) {
+    walk();
+    if (p.y > 0) handed[-2 * S.l.count] = h;  // the place of the run that follows in time
+  }
+  __syncthreads();
+  if (!kept) {
+    h = *handed;
+    walk();
+  }
+  float ra[1] = {1.f}, rb[1] = {0.f}, E[1];
+  const float init[1] = {(!PACKED && p.live && A.dlast != nullptr) ? A.dlast[p.b * H + p.c] : 0.f};
+#pragma unroll
+  for (int k = K - 1; k >= 0; --k) {
+    const int to = PACKED ? last[at0 + k] : -1;
+    if (PACKED && to >= 0) {
+      ra[0] = 0.f;
+      rb[0] = (p.live && A.dlast != nullptr) ? A.dlast[static_cast<int64_t>(to) * H + p.c] : 0.f;
+    }
+    ra[0] *= f[k].a;  // steps beyond the last: a = 1, d = 0
+    rb[0] = f[k].a * (rb[0] + d[k]);
+  }
+  tile_carry<1>(S, W, p, ra, rb, init, maps, E, A.status);
+  float dl = 0.f;
+  if (p.live) {
+    T* out = static_cast<T*>(A.dp) + (row0 + K * A.row_st) * 3 * H + p.c;
+#pragma unroll
+    for (int k = K - 1; k >= 0; --k) {
+      out -= A.row_st * 3 * H;
+      if (k >= n) continue;
+      const int to = PACKED ? last[at0 + k] : -1;
+      if (PACKED && to >= 0) E[0] = A.dlast != nullptr ? A.dlast[static_cast<int64_t>(to) * H + p.c] : 0.f;
+      const float e = d[k] + E[0];
+      __stcs(out, from_f32<T>(e * f[k].x));
+      __stcs(out + H, from_f32<T>(e * f[k].r));
+      __stcs(out + 2 * H, from_f32<T>(e * f[k].i));
+      dl = fmaf(e, f[k].l, dl);
+      E[0] = e * f[k].a;
+      const int64_t begin = PACKED ? first[at0 + k] : (t0 + k == 0 ? p.b : -1);
+      if (begin >= 0 && A.dh0 != nullptr) A.dh0[begin * H + p.c] = E[0];
     }
   }
   // the tile's share of sum dz sigmoid(r), its runs added up in order
   float* sum = reinterpret_cast<float*>(maps);
-  const int width = S.l.count * V;
   __syncthreads();
-#pragma unroll
-  for (int v = 0; v < V; ++v) sum[p.y * width + p.x * V + v] = dl[v];
+  sum[p.y * S.l.count + p.x] = dl;
   __syncthreads();
   if (p.y == 0 && p.live) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float t = 0.f;
-      for (int k = 0; k < S.l.rows; ++k) t += sum[k * width + p.x * V + v];
-      A.partial[(p.b * S.tiles + tile) * H + p.c + v] = t;
-    }
+    float t = 0.f;
+    for (int k = 0; k < S.l.rows; ++k) t += sum[k * S.l.count + p.x];
+    A.partial[(p.b * S.tiles + tile) * H + p.c] = t;
   }
 }
 
-// 4 bytes of channels per thread and step: 16 steps of three inputs, decays and additions
+// channels per thread: forward 4 bytes of them, backward one, whose 7 factors of 8 steps
 // have to fit its registers
-int vec_of(const ScanArgs& a) { return a.bf16 && a.vec ? 2 : 1; }
+int vec_of(const ScanArgs& a, bool bwd) { return !bwd && a.bf16 && a.vec ? 2 : 1; }
 
-TileShape shape_of(const ScanArgs& a, bool codes) {
+TileShape shape_of(const ScanArgs& a, bool bwd) {
   TileShape s;
-  s.l = lanes_of(a.width, vec_of(a), codes, 32, 256);
+  s.l = lanes_of(a.width, vec_of(a, bwd), a.codes != nullptr && !bwd, 32, 256);
   if (s.l.rows > 32) s.l.rows = 32;
-  const int64_t steps = static_cast<int64_t>(s.l.rows) * kStateEvery;
+  s.l.rows &= ~1;  // whole pairs of runs: a kept state for each
+  const int64_t steps = static_cast<int64_t>(s.l.rows) * kRun;
   s.tiles = (a.steps + steps - 1) / steps;
   s.chains = (a.offsets != nullptr ? 1 : a.batch) * s.l.blocks;
   return s;
 }
 
-int64_t flag_count(const TileShape& s) {
-  const int64_t groups = (s.tiles + kFan - 1) / kFan, blocks = (groups + kFan - 1) / kFan;
-  return s.chains * (s.tiles + groups + blocks);
+// workspace: ticket and flags (zeroed), then the maps
+struct WorkLayout {
+  int64_t groups, blocks, width, head, bytes;
+};
+WorkLayout layout_of(const ScanArgs& a, const TileShape& s, bool bwd) {
+  WorkLayout w;
+  w.groups = (s.tiles + kFan - 1) / kFan;
+  w.blocks = (w.groups + kFan - 1) / kFan;
+  w.width = s.l.count * vec_of(a, bwd);
+  w.head = (8 + 4 * s.chains * (s.tiles + w.groups + w.blocks) + 15) / 16 * 16;
+  w.bytes = w.head + s.chains * w.width * ((s.tiles + w.groups) * 8 + w.blocks * 4);
+  return w;
 }
 
-size_t smem_of(const ScanArgs& a, const TileShape& s) {
-  size_t b = static_cast<size_t>(s.l.rows) * s.l.count * vec_of(a) * sizeof(float2);
-  if (a.offsets != nullptr) b += static_cast<size_t>(s.l.rows) * kStateEvery * 2 * sizeof(int);
-  return b;
-}
-
-TileWork work_of(const ScanArgs& a, const TileShape& s, void* buf) {
-  const int64_t groups = (s.tiles + kFan - 1) / kFan, blocks = (groups + kFan - 1) / kFan;
-  const int64_t width = s.l.count * vec_of(a);
+TileWork work_of(const TileShape& s, const WorkLayout& l, void* buf) {
   TileWork w;
   w.ticket = static_cast<unsigned long long*>(buf);
   w.tile_flag = reinterpret_cast<int*>(w.ticket + 1);
   w.group_flag = w.tile_flag + s.chains * s.tiles;
-  w.block_flag = w.group_flag + s.chains * groups;
-  const int64_t head = (8 + 4 * flag_count(s) + 15) / 16 * 16;
-  w.tile_map = reinterpret_cast<float2*>(static_cast<char*>(buf) + head);
-  w.group_map = w.tile_map + s.chains * s.tiles * width;
-  w.block_state = reinterpret_cast<float*>(w.group_map + s.chains * groups * width);
-  (void)blocks;
+  w.block_flag = w.group_flag + s.chains * l.groups;
+  w.tile_map = reinterpret_cast<float2*>(static_cast<char*>(buf) + l.head);
+  w.group_map = w.tile_map + s.chains * s.tiles * l.width;
+  w.block_state = reinterpret_cast<float*>(w.group_map + s.chains * l.groups * l.width);
   return w;
+}
+
+template <class T, bool CODES, bool PACKED, bool MASK>
+void run_tiles(const ScanArgs& a, const TileShape& s, const TileWork& w, bool bwd, cudaStream_t st) {
+  const unsigned blocks = static_cast<unsigned>(s.tiles * s.chains);
+  const int threads = s.l.rows * s.l.count;
+  const size_t smem = static_cast<size_t>(threads) * vec_of(a, bwd) * sizeof(float2) +
+                      (PACKED ? static_cast<size_t>(s.l.rows) * kRun * 2 * sizeof(int) : 0);
+  if (bwd) {
+    scan_tiles_bwd_kernel<T, CODES, PACKED, MASK><<<blocks, threads, smem, st>>>(a, s, w);
+    return;
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (vec_of(a, bwd) == 2) {
+      scan_tiles_fwd_kernel<T, 2, CODES, PACKED, MASK><<<blocks, threads, smem, st>>>(a, s, w);
+      return;
+    }
+  }
+  scan_tiles_fwd_kernel<T, 1, CODES, PACKED, MASK><<<blocks, threads, smem, st>>>(a, s, w);
 }
 
 template <class T, bool CODES>
 void run_tiles(const ScanArgs& a, const TileShape& s, const TileWork& w, bool bwd, cudaStream_t st) {
-  const unsigned blocks = static_cast<unsigned>(s.tiles * s.chains);
-  const int threads = s.l.rows * s.l.count;
-  const size_t smem = smem_of(a, s);
-  if constexpr (sizeof(T) == 2) {
-    if (vec_of(a) == 2) {
-      if (bwd)
-        scan_tiles_bwd_kernel<T, 2, CODES><<<blocks, threads, smem, st>>>(a, s, w);
-      else
-        scan_tiles_fwd_kernel<T, 2, CODES><<<blocks, threads, smem, st>>>(a, s, w);
-      return;
-    }
-  }
-  if (bwd)
-    scan_tiles_bwd_kernel<T, 1, CODES><<<blocks, threads, smem, st>>>(a, s, w);
+  const bool mask = a.mask != nullptr;
+  if (a.offsets != nullptr)
+    mask ? run_tiles<T, CODES, true, true>(a, s, w, bwd, st) : run_tiles<T, CODES, true, false>(a, s, w, bwd, st);
   else
-    scan_tiles_fwd_kernel<T, 1, CODES><<<blocks, threads, smem, st>>>(a, s, w);
+    mask ? run_tiles<T, CODES, false, true>(a, s, w, bwd, st) : run_tiles<T, CODES, false, false>(a, s, w, bwd, st);
 }
 
 }  // namespace
 
 int64_t scan_tiles_partials(const ScanArgs& a) {
-  return (a.offsets != nullptr ? 1 : a.batch) * shape_of(a, a.codes != nullptr).tiles;
+  return (a.offsets != nullptr ? 1 : a.batch) * shape_of(a, true).tiles;
 }
 
-size_t scan_tiles_workspace(const ScanArgs& a) {
-  const TileShape s = shape_of(a, a.codes != nullptr);
-  const int64_t groups = (s.tiles + kFan - 1) / kFan, blocks = (groups + kFan - 1) / kFan;
-  const int64_t width = s.l.count * vec_of(a);
-  return (8 + 4 * flag_count(s) + 15) / 16 * 16 + s.chains * width * ((s.tiles + groups) * 8 + blocks * 4);
+size_t scan_tiles_workspace(const ScanArgs& a, bool bwd) {
+  return static_cast<size_t>(layout_of(a, shape_of(a, bwd), bwd).bytes);
 }
 
 void launch_scan_tiles(const ScanArgs& a, bool bwd, void* workspace, cudaStream_t st) {
-  const TileShape s = shape_of(a, a.codes != nullptr);
+  const TileShape s = shape_of(a, bwd);
   if (a.offsets != nullptr) {
     // what an empty sequence returns: its first state, or the gradient of its last
     float* to = bwd ? a.dh0 : a.last;
@@ -622,8 +618,9 @@ void launch_scan_tiles(const ScanArgs& a, bool bwd, void* workspace, cudaStream_
     }
   }
   if (s.tiles == 0) return;
-  cudaMemsetAsync(workspace, 0, 8 + 4 * flag_count(s), st);
-  const TileWork w = work_of(a, s, workspace);
+  const WorkLayout l = layout_of(a, s, bwd);
+  cudaMemsetAsync(workspace, 0, l.head, st);
+  const TileWork w = work_of(s, l, workspace);
   count_launch();
   const bool codes = a.codes != nullptr;
   if (a.bf16)

@@ -66,74 +66,113 @@ __device__ __forceinline__ void param_store(void* p, int is_bf16, int64_t i, flo
     static_cast<float*>(p)[i] = v;
 }
 
-// Logistic function: ex2 and reciprocal approximations, ~2e-7 relative. exp(-v) = inf gives 0.
-__device__ __forceinline__ float sigmoid_f(float v) { return __fdividef(1.f, 1.f + __expf(-v)); }
+// Single instructions of the special-function unit (each within 2 ulp or so), subnormals
+// flushed: the plain functions spend several instructions more on subnormals.
+__device__ __forceinline__ float ex2_f(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rcp_f(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float sqrt_f(float v) {
+  float r;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float rsqrt_f(float v) {
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Logistic function, ~3e-7 relative; exp(-v) = inf gives 0.
+__device__ __forceinline__ float sigmoid_f(float v) { return rcp_f(1.f + ex2_f(-kLog2e * v)); }
 
 // ---------------------------------------------------------------------------
 // 8-bit codes: per group of 32 values of a row, scale = amax / 127 and
-// code = rint(v * (127 / amax)). The largest magnitude is taken on the bits, so
-// NaN and infinity win; such a group gets the scale NaN (all of it reads back as
-// NaN), a group below 2^-100 the scale 0 (127 / amax would overflow).
+// code = rint(v * (127 / amax)). A NaN or an infinity wins the maximum; such a group gets
+// the scale NaN (all of it reads back as NaN) and codes 0, a group below 2^-100 the scale 0
+// (127 / amax would overflow).
+//
+// Rounding and conversion go through the FMA pipe: v + 1.5 * 2^23 rounds v to an integer
+// (to nearest even) and has it in its low bits; the conversion instructions run at the
+// special-function unit's rate, which the kernels that encode and decode need for
+// exponentials.
 // ---------------------------------------------------------------------------
 struct Scale8 {
   float inv;
   float scale;
+  bool bad;
 };
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
-__device__ __forceinline__ Scale8 scale8(uint32_t top) {
+__device__ __forceinline__ Scale8 scale8(float amax) {
   Scale8 s;
-  const float amax = __uint_as_float(top);
-  s.inv = __fdiv_rn(127.f, amax);
-  s.scale = __fmul_rn(amax, static_cast<float>(1.0 / 127.0));
-  if (top < 0x0d800000u) {  // 2^-100
-    s.inv = 0.f;
-    s.scale = 0.f;
-  } else if (top >= 0x7f800000u) {
-    s.inv = 0.f;
-    s.scale = __uint_as_float(0x7fc00000u);
-  }
+  s.bad = !(amax < __int_as_float(0x7f800000));
+  const bool tiny = amax < 7.888609052210118e-31f;  // 2^-100
+  s.inv = tiny ? 0.f : __fdiv_rn(127.f, amax);
+  s.scale = tiny ? 0.f : __fmul_rn(amax, static_cast<float>(1.0 / 127.0));
+  if (s.bad) s.scale = __int_as_float(0x7fc00000);
   return s;
 }
 
 // The largest magnitude of a group that LANES neighbouring lanes hold (LANES a power of
 // two, aligned inside the warp; every lane of the group calls).
 template <int LANES>
-__device__ __forceinline__ uint32_t group_top(uint32_t top) {
+__device__ __forceinline__ float group_top(float top) {
   const unsigned lane = threadIdx.x & 31;
   const unsigned mask = LANES == 32 ? 0xffffffffu : (((1u << LANES) - 1u) << (lane & ~(LANES - 1u)));
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(mask, top, o));
+  for (int o = LANES / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(mask, top, o));
   return top;
 }
 
-// codes and scale of V values per lane
+// V codes side by side, lowest address first
 template <int V>
-__device__ __forceinline__ float encode8(const float (&f)[V], int8_t (&code)[V]) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < V; ++i) top = max(top, abs_bits(f[i]));
-  const Scale8 s = scale8(group_top<kGroup8 / V>(top));
-  // inv = 0 and f = inf would be NaN, which converts to 0 as well
-#pragma unroll
-  for (int i = 0; i < V; ++i) code[i] = static_cast<int8_t>(__float2int_rn(__fmul_rn(f[i], s.inv)));
-  return s.scale;
-}
-
-template <int V>
-__device__ __forceinline__ void store_codes(int8_t* p, const int8_t (&code)[V]) {
+struct Codes {
   typename RawOf<V>::type raw;
-  int8_t* e = reinterpret_cast<int8_t*>(&raw);
+  __device__ __forceinline__ void store(int8_t* p) const { __stcs(reinterpret_cast<typename RawOf<V>::type*>(p), raw); }
+  __device__ __forceinline__ void load(const int8_t* p) { raw = __ldcs(reinterpret_cast<const typename RawOf<V>::type*>(p)); }
+  __device__ __forceinline__ void zero() { raw = 0; }
+  __device__ __forceinline__ void get(float scale, float (&f)[V]) const {
+    const uint32_t word = static_cast<uint32_t>(raw) ^ 0x80808080u;  // code + 128, 0 to 255
 #pragma unroll
-  for (int i = 0; i < V; ++i) e[i] = code[i];
-  __stcs(reinterpret_cast<typename RawOf<V>::type*>(p), raw);
-}
+    for (int i = 0; i < V; ++i) {
+      // 2^23 + (code + 128), exactly
+      const float t = __uint_as_float(__byte_perm(word, 0x4b000000u, 0x7440 + i));
+      f[i] = __fmul_rn(t - (8388608.f + 128.f), scale);
+    }
+  }
+};
+
+// codes of V values per lane; returns the group's scale
 template <int V>
-__device__ __forceinline__ void load_codes(const int8_t* p, float scale, float (&f)[V]) {
-  const typename RawOf<V>::type raw = __ldcs(reinterpret_cast<const typename RawOf<V>::type*>(p));
-  const int8_t* e = reinterpret_cast<const int8_t*>(&raw);
+__device__ __forceinline__ float encode8(const float (&f)[V], Codes<V>& code) {
+  float top = fabsf(f[0]);
 #pragma unroll
-  for (int i = 0; i < V; ++i) f[i] = __fmul_rn(static_cast<float>(e[i]), scale);
+  for (int i = 1; i < V; ++i) top = max_nan(top, fabsf(f[i]));
+  const Scale8 s = scale8(group_top<kGroup8 / V>(top));
+  uint32_t n[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) n[i] = __float_as_uint(__fadd_rn(__fmul_rn(f[i], s.inv), 12582912.f));
+  uint32_t word;
+  if constexpr (V == 4)
+    word = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+  else if constexpr (V == 2)
+    word = __byte_perm(n[0], n[1], 0x0040);
+  else
+    word = n[0];
+  code.raw = static_cast<typename RawOf<V>::type>(s.bad ? 0u : word);
+  return s.scale;
 }
 
 #endif  // __CUDACC__

@@ -114,8 +114,8 @@ at::Tensor dense_rows(const ScanSizes& z, int64_t width, bool time_major, const 
 }
 
 // stream-ordered, as every temporary here: the caching allocator reuses it after the call
-at::Tensor scan_workspace_of(const ScanArgs& a, int sms, const at::TensorOptions& o) {
-  const size_t bytes = scan_workspace(a, sms);
+at::Tensor scan_workspace_of(const ScanArgs& a, bool bwd, int sms, const at::TensorOptions& o) {
+  const size_t bytes = scan_workspace(a, bwd, sms);
   return bytes == 0 ? at::Tensor() : at::empty({static_cast<int64_t>(bytes)}, o.dtype(at::kByte));
 }
 
@@ -156,7 +156,7 @@ std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& de
   }
   if (z.batch > 0) {
     const int sms = num_sms(p.get_device());
-    at::Tensor work = scan_workspace_of(a, sms, p.options());
+    at::Tensor work = scan_workspace_of(a, false, sms, p.options());
     launch_scan_fwd(a, sms, work.defined() ? work.data_ptr() : nullptr, cur_stream());
     SU_LAUNCH_CHECK();
   }
@@ -217,7 +217,7 @@ std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptTensor& 
   const int sms = num_sms(like.get_device());
   at::Tensor partial = at::empty({scan_partials(a, sms), z.width}, f32);
   a.partial = partial.data_ptr<float>();
-  at::Tensor work = scan_workspace_of(a, sms, like.options());
+  at::Tensor work = scan_workspace_of(a, true, sms, like.options());
   launch_scan_bwd(a, sms, work.defined() ? work.data_ptr() : nullptr, ddecay.data_ptr(), cur_stream());
   SU_LAUNCH_CHECK();
   return {dp, ddecay, dh0};
