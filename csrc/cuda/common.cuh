@@ -29,7 +29,6 @@ enum StatusCode : int {
   kBadIndex = 5,        // an index was out of range (access skipped)
   kPeerTimeout = 6,     // a peer flag never arrived
   kTooLarge = 7,        // a size exceeded a compiled-in bound
-  kScanTimeout = 8,     // the state before a tile of a scan never arrived
 };
 
 // ~2 s at the B200 boost clock; far beyond any legitimate intra-kernel wait.

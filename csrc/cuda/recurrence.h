@@ -30,6 +30,7 @@ struct ScanArgs {
   int decay_bf16 = 0;
   const float* h0 = nullptr;    // [batch, H] or nullptr (zeros)
   const int64_t* offsets = nullptr;  // [batch + 1]
+  int* marks = nullptr;         // packed: [steps], first and last rows of the sequences (the forward pass writes it)
   int64_t row_sb = 0, row_st = 0;
   void* h = nullptr;            // dense rows of H
   float* last = nullptr;        // [batch, H]
@@ -49,16 +50,12 @@ struct ScanArgs {
 };
 
 // Bytes of workspace that a call needs (16-byte aligned, no initial value).
-size_t scan_workspace(const ScanArgs& a, bool bwd, int sms);
+size_t scan_workspace(const ScanArgs& a, int sms);
 // Rows of `partial` that the backward pass writes, the ones it adds them up in included.
 int64_t scan_partials(const ScanArgs& a, int sms);
 void launch_scan_fwd(const ScanArgs& a, int sms, void* workspace, cudaStream_t st);
 // also adds `partial` up into ddecay [H] (in the type of decay)
 void launch_scan_bwd(const ScanArgs& a, int sms, void* workspace, void* ddecay, cudaStream_t st);
-// the form that splits the steps into tiles (scan_tiles.cu)
-size_t scan_tiles_workspace(const ScanArgs& a, bool bwd);
-int64_t scan_tiles_partials(const ScanArgs& a);
-void launch_scan_tiles(const ScanArgs& a, bool bwd, void* workspace, cudaStream_t st);
 
 // One step of `rows` sequences whose fp32 states live in a table of table_rows rows;
 // index[i] (nullptr: i) is row i's place in the table.

@@ -1,239 +1,94 @@
-// Gated linear recurrence over node histories (formulas in scan_math.cuh): a thread walks
-// its channels of one sequence after another. Bound by bytes: forward reads the three
-// input rows and writes h, backward reads the three and dh and writes three.
-#include "kernels.h"
-#include "scan_math.cuh"
+// The gated recurrence's launches: segments, the states between them, packed sequences'
+// marks, the decay's gradient, and the form for one new token per row.
+//
+// Where the sequences and channels alone leave the SMs short of threads, the steps are cut
+// into segments that threads walk side by side. A run of steps maps the state before it to
+// A h + B, and two runs compose to (A2 A1, A2 B1 + B2): one pass over the inputs makes the
+// segments' maps, a short kernel walks the states through them, and the second pass starts
+// every segment from its state. The inputs are read twice (backwards only r and dh are),
+// which costs 7/4 of the bytes forward and 9/7 backward; nothing waits for another block.
+// Handing the states on inside one pass instead (each tile publishing its map and gathering
+// those before it) reads once, and was no faster at any size tried: 10 to 17 us a tile went
+// by in the exchange, 1.44 against 0.86 ms forward for 1,000,000 packed rows of 100 fp32.
+// Every sum and composition has a fixed order: results are the same every run.
+#include "scan_shape.cuh"
 
 namespace su {
 namespace {
 
-// Forward by U steps: their inputs are loaded together, so that U x 3 loads of 4 V (fp32)
-// bytes are under way per thread.
-template <class T, int V, int U, bool CODES, bool MASK>
-__global__ void __launch_bounds__(256) scan_rows_fwd_kernel(const ScanArgs A, const Lanes L) {
-  const int y = threadIdx.x / L.count;
-  const int c = (blockIdx.y * L.count + threadIdx.x % L.count) * V;
-  const bool live = c < A.width;
-  if (!CODES && !live) return;
-  const int H = A.width;
-  const int G = (H + kGroup8 - 1) / kGroup8;
-  const int steps = static_cast<int>(A.steps);
-  float k[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) k[v] = live ? decay_factor(param_at(A.decay, A.decay_bf16, c + v), A.rate) : 0.f;
-  for (int64_t s = static_cast<int64_t>(blockIdx.x) * L.rows + y; s < A.batch;
-       s += static_cast<int64_t>(gridDim.x) * L.rows) {
-    const T* in = static_cast<const T*>(A.p) + s * A.p_sb + c;
-    const uint8_t* valid = MASK ? A.mask + s * A.m_sb : nullptr;
-    T* out = static_cast<T*>(A.h) + s * A.row_sb * H + c;
-    int8_t* code = CODES ? A.codes + s * A.row_sb * 3 * H + c : nullptr;
-    float* scale = CODES ? A.scales + s * A.row_sb * 3 * G + c / kGroup8 : nullptr;
-    float h[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = (live && A.h0 != nullptr) ? A.h0[s * H + c + v] : 0.f;
-    for (int t0 = 0; t0 < steps; t0 += U) {
-      Pack<T, V> x[U], r[U], i[U];
-      bool on[U];
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        on[j] = t0 + j < steps && (!MASK || *valid != 0);
-        x[j].zero();
-        r[j].zero();
-        i[j].zero();
-        if (on[j] && live) {
-          x[j].load(in);
-          r[j].load(in + H);
-          i[j].load(in + 2 * H);
-        }
-        in += A.p_st;
-        if (MASK && t0 + j + 1 < steps) valid += A.m_st;
-      }
-      if (A.states != nullptr && live && t0 > 0 && t0 % kStateEvery == 0) {  // U divides kStateEvery
-        float* to = A.states + (s * A.n_states + t0 / kStateEvery - 1) * H + c;
-#pragma unroll
-        for (int v = 0; v < V; ++v) to[v] = h[v];
-      }
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        if (t0 + j >= steps) break;
-        float fx[V], fr[V], fi[V];
-        x[j].get(fx);
-        r[j].get(fr);
-        i[j].get(fi);
-        if constexpr (CODES) {
-          Codes<V> q[3];
-          const float s0 = encode8(fx, q[0]), s1 = encode8(fr, q[1]), s2 = encode8(fi, q[2]);
-          if (live) {
-            q[0].store(code);
-            q[1].store(code + H);
-            q[2].store(code + 2 * H);
-            if (c % kGroup8 == 0) {
-              scale[0] = s0;
-              scale[G] = s1;
-              scale[2 * G] = s2;
-            }
-          }
-          code += A.row_st * 3 * H;
-          scale += A.row_st * 3 * G;
-        }
-        if (!MASK || on[j]) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const Step g = step_of(fx[v], fr[v], fi[v], k[v]);
-            h[v] = fmaf(g.a, h[v], g.add);
-          }
-        }
-        if (live) {
-          Pack<T, V> o;
-          o.set(h);
-          o.store(out);
-        }
-        out += A.row_st * H;
-      }
+// Marks of the packed sequences' first and last rows; reports offsets that do not rise from
+// 0 to `rows`. `marks` holds -1 before.
+__global__ void scan_marks_kernel(const int64_t* __restrict__ offsets, int64_t batch, int64_t rows, int* marks,
+                                  int* status) {
+  for (int64_t s = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; s < batch;
+       s += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t lo = offsets[s], hi = offsets[s + 1];
+    if (lo < 0 || hi < lo || hi > rows || (s == 0 && lo != 0) || (s == batch - 1 && hi != rows)) {
+      record_status(status, kBadIndex);
+      continue;
     }
-    if (live) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) A.last[s * H + c + v] = h[v];
+    if (hi == lo) continue;
+    const int id = static_cast<int>(s) * 4;
+    if (hi - lo == 1) {
+      marks[lo] = id + kMarkFirst + kMarkLast;
+    } else {
+      marks[lo] = id + kMarkFirst;
+      marks[hi - 1] = id + kMarkLast;
     }
   }
 }
 
-// Backwards by chunks of CH steps (kStateEvery, or fewer where the sequence has no more).
-// Every gradient of a step is g times a factor that the inputs and the state before the
-// step give: the chunk is walked forwards from its first state for the factors, which stay
-// in registers, and then backwards for g. The gates are evaluated once.
-template <class T, int V, int CH, bool CODES, bool MASK>
-__global__ void __launch_bounds__(256, 2) scan_rows_bwd_kernel(const ScanArgs A, const Lanes L) {
-  const int y = threadIdx.x / L.count;
-  const int lane_c = threadIdx.x % L.count;
-  const int c = (blockIdx.y * L.count + lane_c) * V;
-  const bool live = c < A.width;
-  const int H = A.width;
-  const int G = (H + kGroup8 - 1) / kGroup8;
-  const int steps = static_cast<int>(A.steps);
-  float k[V], dl[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    k[v] = live ? decay_factor(param_at(A.decay, A.decay_bf16, c + v), A.rate) : 0.f;
-    dl[v] = 0.f;
-  }
+// carry[q] = the state before segment q (backwards: the gradient after it), from `start` through
+// the maps of the segments before it (after it). A block has 8 channels of one sequence (64
+// bytes of maps, two sectors); each of its 128 rows composes a share of the segments, the shares
+// meet in order, and the row walks its share again from the state it gets.
+constexpr int kShares = 128, kShareCols = 8;
+__global__ void __launch_bounds__(kShareCols * kShares) scan_carry_kernel(const float2* __restrict__ maps, const float* start,
+                                                                  int64_t n, int64_t batch, int H, bool bwd,
+                                                                  float* __restrict__ carry) {
+  __shared__ float2 part[kShares][kShareCols];
+  const int c = blockIdx.y * kShareCols + threadIdx.x;
+  const int64_t b = blockIdx.x;
+  const bool live = c < H;
+  const int64_t share = (n + kShares - 1) / kShares;
+  const int64_t lo = min(n, threadIdx.y * share), hi = min(n, lo + share);
+  const int64_t step = (bwd ? -1 : 1) * batch * H;
+  const int64_t at = ((bwd ? n - 1 - lo : lo) * batch + b) * H + c;
+  float A = 1.f, B = 0.f;
   if (live) {
-    for (int64_t s = static_cast<int64_t>(blockIdx.x) * L.rows + y; s < A.batch;
-         s += static_cast<int64_t>(gridDim.x) * L.rows) {
-      float E[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) E[v] = A.dlast != nullptr ? A.dlast[s * H + c + v] : 0.f;
-      for (int tc = (steps + CH - 1) / CH * CH - CH; tc >= 0; tc -= CH) {
-        const int64_t row = s * A.row_sb + tc * A.row_st;
-        Pack<T, V> x[CH], r[CH], i[CH], d[CH];
-        Codes<V> qx[CH], qr[CH], qi[CH];
-        float sx[CH], sr[CH], si[CH];
-        bool on[CH];
-        const T* in = CODES ? nullptr : static_cast<const T*>(A.p) + s * A.p_sb + tc * A.p_st + c;
-        const T* dh = static_cast<const T*>(A.dh) + (A.dh != nullptr ? s * A.dh_sb + tc * A.dh_st + c : 0);
-        const int8_t* code = CODES ? A.codes + row * 3 * H + c : nullptr;
-        const float* scale = CODES ? A.scales + row * 3 * G + c / kGroup8 : nullptr;
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          const bool inside = tc + j < steps;
-          on[j] = inside && (!MASK || A.mask[s * A.m_sb + (tc + j) * A.m_st] != 0);
-          d[j].zero();
-          if constexpr (CODES) {
-            qx[j].zero();
-            qr[j].zero();
-            qi[j].zero();
-            sx[j] = sr[j] = si[j] = 0.f;
-            if (on[j]) {
-              qx[j].load(code);
-              qr[j].load(code + H);
-              qi[j].load(code + 2 * H);
-              sx[j] = scale[0];
-              sr[j] = scale[G];
-              si[j] = scale[2 * G];
-            }
-            code += A.row_st * 3 * H;
-            scale += A.row_st * 3 * G;
-          } else {
-            x[j].zero();
-            r[j].zero();
-            i[j].zero();
-            if (on[j]) {
-              x[j].load(in);
-              r[j].load(in + H);
-              i[j].load(in + 2 * H);
-            }
-            in += A.p_st;
-          }
-          if (inside && A.dh != nullptr) d[j].load(dh);
-          dh += A.dh_st;
-        }
-        float h[V];
-        const float* from = tc > 0 ? A.states + (s * A.n_states + tc / kStateEvery - 1) * H + c
-                                   : (A.h0 != nullptr ? A.h0 + s * H + c : nullptr);
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = from != nullptr ? from[v] : 0.f;
-        Slope f[CH][V];
-#pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          float fx[V], fr[V], fi[V];
-          if constexpr (CODES) {
-            qx[j].get(sx[j], fx);
-            qr[j].get(sr[j], fr);
-            qi[j].get(si[j], fi);
-          } else {
-            x[j].get(fx);
-            r[j].get(fr);
-            i[j].get(fi);
-          }
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            f[j][v] = slope_of(on[j] ? gate_of(fx[v], fr[v], fi[v], k[v]) : gate_shut(), h[v]);
-          }
-        }
-        T* out = static_cast<T*>(A.dp) + (row + CH * A.row_st) * 3 * H + c;
-#pragma unroll
-        for (int j = CH - 1; j >= 0; --j) {
-          out -= A.row_st * 3 * H;
-          if (tc + j >= steps) continue;
-          float dy[V], dx[V], dr[V], di[V];
-          d[j].get(dy);
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const float g = dy[v] + E[v];
-            dx[v] = g * f[j][v].x;
-            dr[v] = g * f[j][v].r;
-            di[v] = g * f[j][v].i;
-            dl[v] = fmaf(g, f[j][v].l, dl[v]);
-            E[v] = g * f[j][v].a;
-          }
-          Pack<T, V> o;
-          o.set(dx);
-          o.store(out);
-          o.set(dr);
-          o.store(out + H);
-          o.set(di);
-          o.store(out + 2 * H);
-        }
-      }
-      if (A.dh0 != nullptr) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) A.dh0[s * H + c + v] = E[v];
-      }
+    const float2* m = maps + at;
+#pragma unroll 8
+    for (int64_t q = lo; q < hi; ++q, m += step) {
+      const float2 t = *m;
+      A *= t.x;
+      B = fmaf(t.x, B, t.y);
     }
   }
-  // the block's share of sum dz sigmoid(r), added up over its rows in order
-  __shared__ float sum[256 * V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) sum[threadIdx.x * V + v] = dl[v];
+  part[threadIdx.y][threadIdx.x] = make_float2(A, B);
   __syncthreads();
-  if (y == 0 && live) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      float t = 0.f;
-      for (int w = 0; w < L.rows; ++w) t += sum[(w * L.count + lane_c) * V + v];
-      A.partial[static_cast<int64_t>(blockIdx.x) * H + c + v] = t;
-    }
+  if (!live) return;
+  float h = start != nullptr ? start[b * H + c] : 0.f;
+#pragma unroll 8
+  for (int k = 0; k < static_cast<int>(threadIdx.y); ++k) {
+    const float2 t = part[k][threadIdx.x];
+    h = fmaf(t.x, h, t.y);
   }
+  const float2* m = maps + at;
+  float* to = carry + at;
+#pragma unroll 8
+  for (int64_t q = lo; q < hi; ++q, m += step, to += step) {
+    const float2 t = *m;
+    *to = h;
+    h = fmaf(t.x, h, t.y);
+  }
+}
+
+void launch_carry(const ScanArgs& a, const ScanPlan& p, bool bwd, cudaStream_t st) {
+  const int64_t batch = a.offsets != nullptr ? 1 : a.batch;
+  const float* start = a.offsets != nullptr ? nullptr : (bwd ? a.dlast : a.h0);
+  count_launch();
+  scan_carry_kernel<<<dim3(static_cast<unsigned>(batch), (a.width + kShareCols - 1) / kShareCols),
+                      dim3(kShareCols, kShares), 0, st>>>(p.maps, start, p.seg.n, batch, a.width, bwd, p.carry);
 }
 
 // Rows k, k + m, k + 2m, ... of partial [n, H] added up in order into row k of out [m, H]:
@@ -283,109 +138,81 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanStepArgs A) {
   static_cast<T*>(A.h)[e] = from_f32<T>(h);
 }
 
-// blocks over the sequences: every SM filled a few times, so that per-block sums stay few
-int row_blocks(const ScanArgs& a, const Lanes& l, int sms) {
-  const int64_t want = (a.batch + l.rows - 1) / l.rows;
-  const int64_t most = (static_cast<int64_t>(sms) * 8 + l.blocks - 1) / l.blocks;
-  return static_cast<int>(want < most ? want : most);
-}
-
-struct BwdShape {
-  int V, CH;
-};
-// 16 steps' factors of one channel fit the registers, so do 8 of two and 4 of four
-BwdShape bwd_shape(const ScanArgs& a) {
-  if (a.steps <= 4) return {a.vec ? 4 : 1, 4};
-  if (a.steps <= 8) return {a.vec ? 2 : 1, 8};
-  return {1, kStateEvery};
-}
-
-template <class T, bool CODES, bool MASK>
-void rows_fwd(const ScanArgs& a, int sms, cudaStream_t st) {
-  const Lanes l = lanes_of(a.width, a.vec ? 4 : 1, CODES, 256, 256);
-  const dim3 grid(row_blocks(a, l, sms), l.blocks);
-  const int threads = l.count * l.rows;
-  if (a.vec)
-    scan_rows_fwd_kernel<T, 4, 4, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
-  else
-    scan_rows_fwd_kernel<T, 1, 8, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
-}
-
-template <class T, bool CODES, bool MASK>
-void rows_bwd(const ScanArgs& a, int sms, cudaStream_t st) {
-  const BwdShape b = bwd_shape(a);
-  const Lanes l = lanes_of(a.width, b.V, false, 256, 256);
-  const dim3 grid(row_blocks(a, l, sms), l.blocks);
-  const int threads = l.count * l.rows;
-  if (b.CH == 4) {
-    if (b.V == 4)
-      scan_rows_bwd_kernel<T, 4, 4, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
-    else
-      scan_rows_bwd_kernel<T, 1, 4, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
-  } else if (b.CH == 8) {
-    if (b.V == 2)
-      scan_rows_bwd_kernel<T, 2, 8, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
-    else
-      scan_rows_bwd_kernel<T, 1, 8, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
-  } else {
-    scan_rows_bwd_kernel<T, 1, kStateEvery, CODES, MASK><<<grid, threads, 0, st>>>(a, l);
-  }
-}
-
-template <class T, bool CODES>
-void rows_run(const ScanArgs& a, bool bwd, int sms, cudaStream_t st) {
-  if (a.mask != nullptr)
-    bwd ? rows_bwd<T, CODES, true>(a, sms, st) : rows_fwd<T, CODES, true>(a, sms, st);
-  else
-    bwd ? rows_bwd<T, CODES, false>(a, sms, st) : rows_fwd<T, CODES, false>(a, sms, st);
-}
-void rows_launch(const ScanArgs& a, bool bwd, int sms, cudaStream_t st) {
-  count_launch();
-  const bool codes = a.codes != nullptr;
-  if (a.bf16)
-    codes ? rows_run<__nv_bfloat16, true>(a, bwd, sms, st) : rows_run<__nv_bfloat16, false>(a, bwd, sms, st);
-  else
-    codes ? rows_run<float, true>(a, bwd, sms, st) : rows_run<float, false>(a, bwd, sms, st);
-}
-
-// Tiles for packed sequences, and where a thread per sequence and 4 channels leaves the SMs
-// short of threads; a sequence of one chunk has nothing to split.
-bool in_tiles(const ScanArgs& a, int sms) {
-  if (a.offsets != nullptr || a.steps > (1 << 30)) return true;
-  if (a.steps <= kStateEvery) return false;
-  return a.batch * ((a.width + (a.vec ? 3 : 0)) / (a.vec ? 4 : 1)) < static_cast<int64_t>(sms) * 512;
-}
-
 constexpr int64_t kSumRows = 64;  // above 8 times it the partial sums are added up in two launches
-int64_t partial_rows(const ScanArgs& a, int sms) {
-  return in_tiles(a, sms) ? scan_tiles_partials(a)
-                          : row_blocks(a, lanes_of(a.width, bwd_shape(a).V, false, 256, 256), sms);
+
+// what an empty packed sequence returns: its first state, or the gradient of its last
+void fill_packed(const ScanArgs& a, float* to, const float* from, cudaStream_t st) {
+  if (to == nullptr) return;
+  const size_t bytes = static_cast<size_t>(a.batch) * a.width * sizeof(float);
+  if (from != nullptr)
+    cudaMemcpyAsync(to, from, bytes, cudaMemcpyDeviceToDevice, st);
+  else
+    cudaMemsetAsync(to, 0, bytes, st);
 }
 
 }  // namespace
 
-size_t scan_workspace(const ScanArgs& a, bool bwd, int sms) {
-  return in_tiles(a, sms) ? scan_tiles_workspace(a, bwd) : 0;
+// Segments: as many as give the SMs about 1024 threads each of forward lanes (4 channels where
+// rows are aligned), none shorter than 2 kStateEvery; at most 4096, whose states the carry
+// kernel walks in a few microseconds. Sequences that fill half of that by themselves are left whole:
+// the second read would cost more than the idle threads.
+ScanPlan scan_plan(const ScanArgs& a, int sms, void* workspace) {
+  const int64_t batch = a.offsets != nullptr ? 1 : a.batch;
+  const int64_t lanes = batch * ((a.width + (a.vec ? 3 : 0)) / (a.vec ? 4 : 1));
+  const int64_t want = static_cast<int64_t>(sms) * 1024;
+  ScanPlan p;
+  p.seg = {1, (a.steps + kStateEvery - 1) / kStateEvery * kStateEvery};
+  if (lanes * 2 < want && a.steps > 4 * kStateEvery) {
+    int64_t n = (want + lanes - 1) / lanes;
+    n = n < 4096 ? n : 4096;
+    int64_t len = (a.steps + n - 1) / n;
+    len = len > 2 * kStateEvery ? len : 2 * kStateEvery;
+    len = (len + kStateEvery - 1) / kStateEvery * kStateEvery;
+    p.seg = {(a.steps + len - 1) / len, len};
+  }
+  p.maps = static_cast<float2*>(workspace);
+  p.carry = reinterpret_cast<float*>(p.maps + p.seg.n * batch * a.width);
+  return p;
+}
+
+size_t scan_workspace(const ScanArgs& a, int sms) {
+  const ScanPlan p = scan_plan(a, sms, nullptr);
+  const int64_t batch = a.offsets != nullptr ? 1 : a.batch;
+  return p.seg.n > 1 ? static_cast<size_t>(p.seg.n * batch * a.width) * (sizeof(float2) + sizeof(float)) : 0;
 }
 
 int64_t scan_partials(const ScanArgs& a, int sms) {
-  const int64_t n = partial_rows(a, sms);
+  const int64_t n = scan_bwd_blocks(a, scan_plan(a, sms, nullptr), sms);
   return n > 8 * kSumRows ? n + kSumRows : n;
 }
 
 void launch_scan_fwd(const ScanArgs& a, int sms, void* workspace, cudaStream_t st) {
-  if (in_tiles(a, sms))
-    launch_scan_tiles(a, false, workspace, st);
-  else
-    rows_launch(a, false, sms, st);
+  const ScanPlan p = scan_plan(a, sms, workspace);
+  if (a.offsets != nullptr) {
+    cudaMemsetAsync(a.marks, 0xff, static_cast<size_t>(a.steps) * sizeof(int), st);
+    count_launch();
+    const int64_t blocks = (a.batch + 255) / 256;
+    scan_marks_kernel<<<static_cast<unsigned>(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(a.offsets, a.batch, a.steps,
+                                                                                           a.marks, a.status);
+    fill_packed(a, a.last, a.h0, st);
+  }
+  if (a.steps == 0 && a.offsets != nullptr) return;
+  if (p.seg.n > 1) {
+    scan_fwd_maps(a, p, sms, st);
+    launch_carry(a, p, false, st);
+  }
+  scan_fwd_rows(a, p, sms, st);
 }
 
 void launch_scan_bwd(const ScanArgs& a, int sms, void* workspace, void* ddecay, cudaStream_t st) {
-  if (in_tiles(a, sms))
-    launch_scan_tiles(a, true, workspace, st);
-  else
-    rows_launch(a, true, sms, st);
-  int64_t n = partial_rows(a, sms);
+  const ScanPlan p = scan_plan(a, sms, workspace);
+  if (a.offsets != nullptr) fill_packed(a, a.dh0, a.dlast, st);
+  if (p.seg.n > 1) {
+    scan_bwd_maps(a, p, sms, st);
+    launch_carry(a, p, true, st);
+  }
+  scan_bwd_rows(a, p, sms, st);
+  int64_t n = scan_bwd_blocks(a, p, sms);
   const float* from = a.partial;
   const int cols = (a.width + 31) / 32;
   const dim3 threads(32, 32);

@@ -1,5 +1,5 @@
 // Arithmetic of one step of the gated linear recurrence (forward and gradients), shared
-// by the kernels that walk whole sequences and those that split them into tiles.
+// by the kernels of both directions.
 //
 //   z = -c softplus(decay) sigmoid(r)      a = exp(z)          s = sqrt(1 - a^2)
 //   h_t = a h_{t-1} + s sigmoid(i) x
@@ -85,27 +85,6 @@ __device__ __forceinline__ Slope slope_of(const Gate& g, float& h) {
   const float f = g.a * (h - g.q);
   h = fmaf(g.a, h, g.add);
   return Slope{g.a, g.x, f * g.z, g.i, f * g.sr};
-}
-
-// A thread's V channels: lanes of a row side by side, rows over threadIdx / lanes.
-struct Lanes {
-  int count;   // lanes that one row takes in a block
-  int rows;    // rows side by side in a block
-  int blocks;  // blocks over the channels
-};
-
-// Lanes of H channels at V per lane, at most `most` lanes a row and `threads` threads a block;
-// with 8-bit codes every group of 32 channels gets its own aligned lanes, the last one's
-// beyond H included.
-inline Lanes lanes_of(int width, int V, bool codes, int most, int threads) {
-  const int unit = codes ? kGroup8 / V : 1;
-  const int all = codes ? (width + kGroup8 - 1) / kGroup8 * unit : (width + V - 1) / V;
-  Lanes l;
-  l.blocks = (all + most - 1) / most;
-  l.count = (all + l.blocks - 1) / l.blocks;
-  l.count = (l.count + unit - 1) / unit * unit;
-  l.rows = threads / l.count;
-  return l;
 }
 
 }  // namespace su

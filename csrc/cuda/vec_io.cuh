@@ -41,6 +41,8 @@ struct Pack {
   using Raw = typename RawOf<sizeof(T) * V>::type;
   Raw raw;
   __device__ __forceinline__ void load(const T* p) { raw = __ldcs(reinterpret_cast<const Raw*>(p)); }
+  // for values that a later pass reads again
+  __device__ __forceinline__ void load_keep(const T* p) { raw = __ldg(reinterpret_cast<const Raw*>(p)); }
   __device__ __forceinline__ void zero() { raw = Raw{}; }
   __device__ __forceinline__ void get(float (&f)[V]) const {
     const T* e = reinterpret_cast<const T*>(&raw);

@@ -185,7 +185,8 @@ std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& de
 std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const c10::optional<at::Tensor>& scales,
                                        const at::Tensor& states, const at::Tensor& decay,
                                        const c10::optional<at::Tensor>& h0, const c10::optional<at::Tensor>& mask,
-                                       const c10::optional<at::Tensor>& offsets, const c10::optional<at::Tensor>& dh,
+                                       const c10::optional<at::Tensor>& offsets,
+                                       const c10::optional<at::Tensor>& marks, const c10::optional<at::Tensor>& dh,
                                        const c10::optional<at::Tensor>& dlast, double rate, bool time_major, bool bf16,
                                        bool need_dh0);
 at::Tensor gated_scan_step(const at::Tensor& p, const at::Tensor& decay, at::Tensor& state,

@@ -114,8 +114,8 @@ at::Tensor dense_rows(const ScanSizes& z, int64_t width, bool time_major, const 
 }
 
 // stream-ordered, as every temporary here: the caching allocator reuses it after the call
-at::Tensor scan_workspace_of(const ScanArgs& a, bool bwd, int sms, const at::TensorOptions& o) {
-  const size_t bytes = scan_workspace(a, bwd, sms);
+at::Tensor scan_workspace_of(const ScanArgs& a, int sms, const at::TensorOptions& o) {
+  const size_t bytes = scan_workspace(a, sms);
   return bytes == 0 ? at::Tensor() : at::empty({static_cast<int64_t>(bytes)}, o.dtype(at::kByte));
 }
 
@@ -123,7 +123,8 @@ int64_t groups_of(int64_t width) { return (width + kGroup8 - 1) / kGroup8; }
 
 }  // namespace
 
-// -> h, last state, kept states, codes, scales (the last three undefined where not kept)
+// -> h, last state, kept states, codes, scales (those three undefined where not kept), marks of
+// packed sequences
 std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& decay, const OptTensor& h0,
                                        const OptTensor& mask, const OptTensor& offsets, double rate, bool time_major,
                                        bool keep_states, bool keep8) {
@@ -141,7 +142,7 @@ std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& de
   const auto f32 = p.options().dtype(at::kFloat);
   at::Tensor h = dense_rows(z, z.width, time_major, p.options());
   at::Tensor last = at::empty({z.batch, z.width}, f32);
-  at::Tensor states, codes, scales;
+  at::Tensor states, codes, scales, marks;
   a.h = h.data_ptr();
   a.last = last.data_ptr<float>();
   if (keep_states) {
@@ -154,21 +155,26 @@ std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& de
     a.codes = codes.data_ptr<int8_t>();
     a.scales = scales.data_ptr<float>();
   }
+  if (z.packed) {
+    TORCH_CHECK(z.batch < (1ll << 29), "gated_scan: 2^29 sequences or more");
+    marks = at::empty({z.steps}, p.options().dtype(at::kInt));
+    a.marks = marks.data_ptr<int>();
+  }
   if (z.batch > 0) {
     const int sms = num_sms(p.get_device());
-    at::Tensor work = scan_workspace_of(a, false, sms, p.options());
+    at::Tensor work = scan_workspace_of(a, sms, p.options());
     launch_scan_fwd(a, sms, work.defined() ? work.data_ptr() : nullptr, cur_stream());
     SU_LAUNCH_CHECK();
   }
-  return {h, last, states, codes, scales};
+  return {h, last, states, codes, scales, marks};
 }
 
 // `like`: p, or its 8-bit codes with `scales` (then the gradients have the type of h, `bf16`)
 // -> dp, ddecay, dh0
 std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptTensor& scales, const at::Tensor& states,
                                        const at::Tensor& decay, const OptTensor& h0, const OptTensor& mask,
-                                       const OptTensor& offsets, const OptTensor& dh, const OptTensor& dlast,
-                                       double rate, bool time_major, bool bf16, bool need_dh0) {
+                                       const OptTensor& offsets, const OptTensor& marks, const OptTensor& dh,
+                                       const OptTensor& dlast, double rate, bool time_major, bool bf16, bool need_dh0) {
   SU_CHECK_CUDA(like);
   const ScanSizes z = scan_sizes(like.sizes(), offsets, 3);
   const auto dev = like.device();
@@ -191,6 +197,10 @@ std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptTensor& 
   }
   TORCH_CHECK(states.numel() == (z.packed ? 1 : z.batch) * a.n_states * z.width, "gated_scan: kept states do not fit");
   a.states = const_cast<float*>(states.data_ptr<float>());
+  if (z.packed) {
+    TORCH_CHECK(given(marks) && marks->numel() == z.steps, "gated_scan: packed sequences need the forward's marks");
+    a.marks = marks->data_ptr<int>();
+  }
   if (given(dh)) {
     TORCH_CHECK(dh->device() == dev && dh->scalar_type() == type && dh->dim() == like.dim() &&
                     dh->size(-1) == z.width && unit_last(*dh),
@@ -217,7 +227,7 @@ std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptTensor& 
   const int sms = num_sms(like.get_device());
   at::Tensor partial = at::empty({scan_partials(a, sms), z.width}, f32);
   a.partial = partial.data_ptr<float>();
-  at::Tensor work = scan_workspace_of(a, true, sms, like.options());
+  at::Tensor work = scan_workspace_of(a, sms, like.options());
   launch_scan_bwd(a, sms, work.defined() ? work.data_ptr() : nullptr, ddecay.data_ptr(), cur_stream());
   SU_LAUNCH_CHECK();
   return {dp, ddecay, dh0};

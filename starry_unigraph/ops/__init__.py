@@ -57,7 +57,7 @@ def check_status(clear: bool = True) -> None:
     if code != 0:
         names = {1: "operand stage wait timed out", 2: "free stage wait timed out", 3: "accumulator wait timed out",
                  4: "TMEM drain wait timed out", 5: "index out of range", 6: "peer flag wait timed out",
-                 7: "size above compiled bound", 8: "scan carry wait timed out"}
+                 7: "size above compiled bound"}
         raise RuntimeError(f"device status {code}: {names.get(code, 'unknown')}")
 
 

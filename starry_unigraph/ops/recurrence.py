@@ -32,10 +32,10 @@ STATE_EVERY = 16  # steps between the fp32 states kept for the backward pass
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, p, decay, h0, mask, offsets, rate, time_major, keep8):
-        h, last, states, codes, scales = cuda_ext().gated_scan_fwd(p, decay, h0, mask, offsets, rate, time_major, True,
-                                                                   keep8)
+        h, last, states, codes, scales, marks = cuda_ext().gated_scan_fwd(p, decay, h0, mask, offsets, rate, time_major,
+                                                                          True, keep8)
         ctx.save_for_backward(exact(codes) if keep8 else p, exact(scales), exact(states), decay,
-                              None if h0 is None else exact(h0.detach()), mask, offsets)
+                              None if h0 is None else exact(h0.detach()), mask, offsets, marks)
         ctx.meta = (rate, time_major, p.dtype == torch.bfloat16)
         ctx.set_materialize_grads(False)
         return h, last
@@ -43,14 +43,14 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, dlast):
-        like, scales, states, decay, h0, mask, offsets = ctx.saved_tensors
+        like, scales, states, decay, h0, mask, offsets, marks = ctx.saved_tensors
         rate, time_major, bf16 = ctx.meta
         if dh is not None and dh.stride(-1) != 1:
             dh = dh.contiguous()
         if dlast is not None:
             dlast = dlast.contiguous()
-        dp, ddecay, dh0 = cuda_ext().gated_scan_bwd(like, scales, states, decay, h0, mask, offsets, dh, dlast, rate,
-                                                    time_major, bf16, ctx.needs_input_grad[2])
+        dp, ddecay, dh0 = cuda_ext().gated_scan_bwd(like, scales, states, decay, h0, mask, offsets, marks, dh, dlast,
+                                                    rate, time_major, bf16, ctx.needs_input_grad[2])
         return dp, ddecay, dh0, None, None, None, None, None
 
 
@@ -185,8 +185,7 @@ def gated_scan(p: torch.Tensor, decay: torch.Tensor, h0: torch.Tensor | None = N
     time_major = offsets is None and p.stride(1) > p.stride(0)
     if torch.is_grad_enabled() and (p.requires_grad or decay.requires_grad or (h0 is not None and h0.requires_grad)):
         return _GatedScan.apply(p, decay, h0, mask, offsets, float(rate), time_major, keep8)
-    h, last, _, _, _ = cuda_ext().gated_scan_fwd(p, decay, h0, mask, offsets, float(rate), time_major, False, False)
-    return h, last
+    return tuple(cuda_ext().gated_scan_fwd(p, decay, h0, mask, offsets, float(rate), time_major, False, False)[:2])
 
 
 def gated_scan_step(p: torch.Tensor, decay: torch.Tensor, state: torch.Tensor, rows: torch.Tensor | None = None, *,
