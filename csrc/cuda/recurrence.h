@@ -7,9 +7,11 @@
 
 namespace su {
 
-// Steps between the fp32 states that the recurrence's forward pass keeps for its
-// backward pass (which recomputes the steps in between).
+// Steps between the fp32 states that the recurrence's forward pass keeps for its backward
+// pass, which recomputes the steps in between: 16 with 8-bit inputs (the gradients'
+// definition has them), else 8, whose factors of two channels fit a thread's registers.
 constexpr int kStateEvery = 16;
+constexpr int kStateShort = 8;
 
 constexpr int kGroup8 = 32;  // values of a row that share one scale in the 8-bit format
 
@@ -34,7 +36,8 @@ struct ScanArgs {
   int64_t row_sb = 0, row_st = 0;
   void* h = nullptr;            // dense rows of H
   float* last = nullptr;        // [batch, H]
-  float* states = nullptr;      // state before step k * kStateEvery, k >= 1: [batch, n_states, H] (packed: [n_states, H])
+  int state_every = kStateShort;
+  float* states = nullptr;      // state before step k * state_every, k >= 1: [batch, n_states, H] (packed: [n_states, H])
   int64_t n_states = 0;
   int8_t* codes = nullptr;      // dense rows of 3H: the inputs in 8 bits (nullptr: not kept)
   float* scales = nullptr;      // dense rows of 3 * ceil(H / 32)

@@ -5,182 +5,276 @@
 namespace su {
 namespace {
 
-// V values of each of x, r and i of one step: the inputs, or their 8-bit codes and scales.
-template <class T, int V, bool CODES>
-struct Inputs;
-template <class T, int V>
-struct Inputs<T, V, false> {
-  Pack<T, V> v[3];
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int w = 0; w < 3; ++w) v[w].zero();
-  }
-  __device__ __forceinline__ void load(const T* p, const float*, int H, int) {
-#pragma unroll
-    for (int w = 0; w < 3; ++w) v[w].load(p + w * static_cast<int64_t>(H));
-  }
-  __device__ __forceinline__ void get(int w, float (&f)[V]) const { v[w].get(f); }
-};
-template <class T, int V>
-struct Inputs<T, V, true> {
-  Codes<V> v[3];
-  float scale[3];
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int w = 0; w < 3; ++w) {
-      v[w].zero();
-      scale[w] = 0.f;
-    }
-  }
-  __device__ __forceinline__ void load(const int8_t* p, const float* s, int H, int G) {
-#pragma unroll
-    for (int w = 0; w < 3; ++w) {
-      v[w].load(p + w * static_cast<int64_t>(H));
-      scale[w] = s[w * static_cast<int64_t>(G)];
-    }
-  }
-  __device__ __forceinline__ void get(int w, float (&f)[V]) const { v[w].get(scale[w], f); }
+// Where a unit of work (one chunk of one segment) lies.
+struct Unit {
+  int64_t q, b, begin;  // segment, sequence, the segment's first step
+  int steps, tc;        // of the segment; the chunk's first step inside it
 };
 
-// Chunks of CH steps (kStateEvery, or fewer where the sequence has no more). Every gradient
-// of a step is g times a factor that the inputs and the state before the step give: the
-// chunk is walked forwards from its first state for the factors, which stay in registers,
-// and then backwards for g. The gates are evaluated once.
+// A chunk's x, r, i and dh on their way to registers. In flight they are copies into slots of
+// shared memory that belong to the thread, so the next chunk's loads are under way while
+// this one is worked on and no barrier is needed.
+template <class T, int V, int CH>
+struct Slots {
+  static constexpr int kBytes = sizeof(T) * V;
+  using Raw = typename RawOf<kBytes>::type;
+  Raw* at;  // [2][CH][4][threads], at this thread's place
+  int ld;   // threads
+
+  __device__ __forceinline__ Raw* slot(int buf, int j, int w) const { return at + ((buf * CH + j) * 4 + w) * ld; }
+  __device__ __forceinline__ void fetch(const ScanArgs& A, const Unit& u, int c, int buf) const {
+    const int64_t t0 = u.begin + u.tc;
+    const T* in = static_cast<const T*>(A.p) + u.b * A.p_sb + t0 * A.p_st + c;
+    const T* dh = static_cast<const T*>(A.dh) + (A.dh != nullptr ? u.b * A.dh_sb + t0 * A.dh_st + c : 0);
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      if (u.tc + j < u.steps) {
+        copy_async<kBytes>(slot(buf, j, 0), in);
+        copy_async<kBytes>(slot(buf, j, 1), in + A.width);
+        copy_async<kBytes>(slot(buf, j, 2), in + 2 * static_cast<int64_t>(A.width));
+        if (A.dh != nullptr) copy_async<kBytes>(slot(buf, j, 3), dh);
+      }
+      in += A.p_st;
+      dh += A.dh_st;
+    }
+  }
+  __device__ __forceinline__ void get(int buf, int j, int w, float (&f)[V]) const {
+    Pack<T, V> p;
+    p.raw = *slot(buf, j, w);
+    p.get(f);
+  }
+};
+
+// The same values in registers: narrow rows (single bf16 values) and 8-bit codes.
+template <class T, int V, int CH, bool CODES>
+struct Held {
+  Pack<T, V> v[CODES ? 1 : CH][3], d[CH];
+  Codes<V> q[CODES ? CH : 1][3];
+  float scale[CODES ? CH : 1][3];
+
+  __device__ __forceinline__ void fetch(const ScanArgs& A, const Unit& u, int c, unsigned on) {
+    const int H = A.width, G = (H + kGroup8 - 1) / kGroup8;
+    const int64_t t0 = u.begin + u.tc;
+    const int64_t row = u.b * A.row_sb + t0 * A.row_st;
+    const T* in = CODES ? nullptr : static_cast<const T*>(A.p) + u.b * A.p_sb + t0 * A.p_st + c;
+    const int8_t* code = CODES ? A.codes + row * 3 * H + c : nullptr;
+    const float* sc = CODES ? A.scales + row * 3 * G + c / kGroup8 : nullptr;
+    const T* dh = static_cast<const T*>(A.dh) + (A.dh != nullptr ? u.b * A.dh_sb + t0 * A.dh_st + c : 0);
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+#pragma unroll
+      for (int w = 0; w < 3; ++w) {
+        if constexpr (CODES) {
+          q[j][w].zero();
+          scale[j][w] = 0.f;
+          if (on >> j & 1) {
+            q[j][w].load(code + w * static_cast<int64_t>(H));
+            scale[j][w] = sc[w * static_cast<int64_t>(G)];
+          }
+        } else {
+          v[j][w].zero();
+          if (on >> j & 1) v[j][w].load(in + w * static_cast<int64_t>(H));
+        }
+      }
+      d[j].zero();
+      if (u.tc + j < u.steps && A.dh != nullptr) d[j].load(dh);
+      if (CODES) {
+        code += A.row_st * 3 * H;
+        sc += A.row_st * 3 * G;
+      } else {
+        in += A.p_st;
+      }
+      dh += A.dh_st;
+    }
+  }
+  __device__ __forceinline__ void get(int j, int w, float (&f)[V]) const {
+    if constexpr (CODES)
+      q[j][w].get(scale[j][w], f);
+    else
+      v[j][w].get(f);
+  }
+};
+
+// Chunks of CH steps (those between kept states, or the whole of a short sequence). Every
+// gradient of a step is g times a factor that the inputs and the state before the step give:
+// the chunk is walked forwards from its first state for the factors, which stay in
+// registers, and then backwards for g. The gates are evaluated once.
+constexpr int kBwdThreads = 128;
 template <class T, int V, int CH, bool CODES, int KIND>
-__global__ void __launch_bounds__(256, 2) scan_bwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {
+__global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {
+  constexpr bool kAsync = !CODES && sizeof(T) * V >= 4;
+  extern __shared__ uint4 smem[];
   const int y = threadIdx.x / L.count;
   const int lane_c = threadIdx.x % L.count;
   const int c = (blockIdx.y * L.count + lane_c) * V;
   const bool live = c < A.width;
   const int H = A.width;
-  const int G = (H + kGroup8 - 1) / kGroup8;
   const int64_t batch = KIND == kPacked ? 1 : A.batch;
   const int64_t rows = live ? batch * P.seg.n : 0;
-  float k[V], dl[V];
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * L.rows;
+  float k[V], dl[V], E[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     k[v] = live ? decay_factor(param_at(A.decay, A.decay_bf16, c + v), A.rate) : 0.f;
-    dl[v] = 0.f;
+    dl[v] = E[v] = 0.f;
   }
-  for (int64_t rr = static_cast<int64_t>(blockIdx.x) * L.rows + y; rr < rows;
-       rr += static_cast<int64_t>(gridDim.x) * L.rows) {
+  // units in the order of work: a row's chunks from the last to the first, then the next row;
+  // false behind the last one. Rows without steps have one empty chunk.
+  auto place = [&](int64_t rr, Unit& u) {
+    if (rr >= rows) return false;
     const SegRow s = seg_row(rr, batch, P.seg, false);
-    const int64_t begin = s.q * P.seg.len;
-    const int steps = static_cast<int>(min(P.seg.len, A.steps - begin));
-    float E[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      E[v] = 0.f;
-      if (P.seg.n > 1)
-        E[v] = P.carry[(s.q * batch + s.b) * H + c + v];
-      else if (KIND != kPacked && A.dlast != nullptr)
-        E[v] = A.dlast[s.b * H + c + v];
+    u.q = s.q;
+    u.b = s.b;
+    u.begin = s.q * P.seg.len;
+    u.steps = static_cast<int>(min(P.seg.len, A.steps - u.begin));
+    u.tc = u.steps > 0 ? (u.steps - 1) / CH * CH : 0;
+    return true;
+  };
+  int64_t rr = static_cast<int64_t>(blockIdx.x) * L.rows + y;
+  Unit u;
+  bool more = place(rr, u);
+  Slots<T, V, CH> slots;
+  if constexpr (kAsync) {
+    slots.at = reinterpret_cast<typename Slots<T, V, CH>::Raw*>(smem) + threadIdx.x;
+    slots.ld = blockDim.x;
+    if (more) slots.fetch(A, u, c, 0);
+    commit_copies();
+  }
+  bool fresh = true;
+  int buf = 0;
+  while (more) {
+    Unit next = u;
+    bool more_next;
+    if (u.tc > 0) {
+      next.tc -= CH;
+      more_next = true;
+    } else {
+      rr += stride;
+      more_next = place(rr, next);
     }
-    for (int tc = (steps + CH - 1) / CH * CH - CH; tc >= 0; tc -= CH) {
-      const int64_t t0 = begin + tc;
-      const int64_t row = s.b * A.row_sb + t0 * A.row_st;
-      Inputs<T, V, CODES> w[CH];
-      Pack<T, V> d[CH];
-      unsigned on = 0, firsts = 0, lasts = 0;
-      {
-        const auto* in = [&] {
-          if constexpr (CODES)
-            return A.codes + row * 3 * H + c;
-          else
-            return static_cast<const T*>(A.p) + s.b * A.p_sb + t0 * A.p_st + c;
-        }();
-        const int64_t in_st = CODES ? A.row_st * 3 * H : A.p_st;
-        const float* scale = CODES ? A.scales + row * 3 * G + c / kGroup8 : nullptr;
-        const T* dh = static_cast<const T*>(A.dh) + (A.dh != nullptr ? s.b * A.dh_sb + t0 * A.dh_st + c : 0);
-        const uint8_t* valid = A.mask != nullptr ? A.mask + s.b * A.m_sb + t0 * A.m_st : nullptr;
+    const int64_t t0 = u.begin + u.tc;
+    const int64_t row = u.b * A.row_sb + t0 * A.row_st;
+    const int64_t at = (u.q * batch + u.b) * H + c;
+    if (fresh) {
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-          const bool inside = tc + j < steps;
-          bool step = inside;
-          if (KIND == kMasked || (KIND == kPacked && valid != nullptr)) {
-            if (inside) step = *valid != 0;
-            valid += A.m_st;
-          }
-          if (KIND == kPacked) {
-            const int mk = inside ? A.marks[t0 + j] : -1;
-            if (mk >= 0) {
-              firsts |= static_cast<unsigned>(mk & kMarkFirst) << j;
-              lasts |= static_cast<unsigned>((mk & kMarkLast) >> 1) << j;
-            }
-          }
-          if (step) on |= 1u << j;
-          w[j].zero();
-          if (step) w[j].load(in, scale, H, G);
-          in += in_st;
-          if (CODES) scale += A.row_st * 3 * G;
-          d[j].zero();
-          if (inside && A.dh != nullptr) d[j].load(dh);
-          dh += A.dh_st;
-        }
+      for (int v = 0; v < V; ++v) {
+        E[v] = 0.f;
+        if (P.seg.n > 1)
+          E[v] = P.carry[at + v];
+        else if (KIND != kPacked && A.dlast != nullptr)
+          E[v] = A.dlast[u.b * H + c + v];
       }
-      float h[V];
-      const float* from = t0 > 0 ? A.states + (s.b * A.n_states + t0 / kStateEvery - 1) * H + c
-                                 : (KIND != kPacked && A.h0 != nullptr ? A.h0 + s.b * H + c : nullptr);
+    }
+    float h[V];
+    const float* from = t0 > 0 ? A.states + (u.b * A.n_states + t0 / A.state_every - 1) * H + c
+                               : (KIND != kPacked && A.h0 != nullptr ? A.h0 + u.b * H + c : nullptr);
 #pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = from != nullptr ? from[v] : 0.f;
-      Slope f[CH][V];
+    for (int v = 0; v < V; ++v) h[v] = from != nullptr ? from[v] : 0.f;
+    unsigned on = 0, firsts = 0, lasts = 0;
+    if (KIND == kPlain) {
+      const int n = u.steps - u.tc;
+      on = n >= CH ? (1u << CH) - 1u : (1u << n) - 1u;
+    } else {
+      const uint8_t* valid = A.mask != nullptr ? A.mask + u.b * A.m_sb + t0 * A.m_st : nullptr;
 #pragma unroll
       for (int j = 0; j < CH; ++j) {
-        if (KIND == kPacked && (firsts >> j & 1)) {
-          const int64_t q = A.marks[t0 + j] >> 2;
-#pragma unroll
-          for (int v = 0; v < V; ++v) h[v] = A.h0 != nullptr ? A.h0[q * H + c + v] : 0.f;
-        }
-        float fx[V], fr[V], fi[V];
-        w[j].get(0, fx);
-        w[j].get(1, fr);
-        w[j].get(2, fi);
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          f[j][v] = slope_of(on >> j & 1 ? gate_of(fx[v], fr[v], fi[v], k[v]) : gate_shut(), h[v]);
-      }
-      T* out = static_cast<T*>(A.dp) + (row + CH * A.row_st) * 3 * H + c;
-#pragma unroll
-      for (int j = CH - 1; j >= 0; --j) {
-        out -= A.row_st * 3 * H;
-        if (tc + j >= steps) continue;
-        if (KIND == kPacked && (lasts >> j & 1)) {
-          const int64_t q = A.marks[t0 + j] >> 2;
-#pragma unroll
-          for (int v = 0; v < V; ++v) E[v] = A.dlast != nullptr ? A.dlast[q * H + c + v] : 0.f;
-        }
-        float dy[V], dx[V], dr[V], di[V];
-        d[j].get(dy);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float g = dy[v] + E[v];
-          dx[v] = g * f[j][v].x;
-          dr[v] = g * f[j][v].r;
-          di[v] = g * f[j][v].i;
-          dl[v] = fmaf(g, f[j][v].l, dl[v]);
-          E[v] = g * f[j][v].a;
-        }
-        Pack<T, V> o;
-        o.set(dx);
-        o.store(out);
-        o.set(dr);
-        o.store(out + H);
-        o.set(di);
-        o.store(out + 2 * H);
-        if (KIND == kPacked && (firsts >> j & 1) && A.dh0 != nullptr) {
-          const int64_t q = A.marks[t0 + j] >> 2;
-#pragma unroll
-          for (int v = 0; v < V; ++v) A.dh0[q * H + c + v] = E[v];
+        if (u.tc + j >= u.steps) continue;
+        if (valid == nullptr || valid[j * A.m_st] != 0) on |= 1u << j;
+        if (KIND == kPacked) {
+          const int mk = A.marks[t0 + j];
+          if (mk >= 0) {
+            firsts |= static_cast<unsigned>(mk & kMarkFirst) << j;
+            lasts |= static_cast<unsigned>((mk & kMarkLast) >> 1) << j;
+          }
         }
       }
     }
-    if (KIND != kPacked && s.q == 0 && A.dh0 != nullptr) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) A.dh0[s.b * H + c + v] = E[v];
+    Held<T, V, CH, CODES> held;
+    if constexpr (kAsync) {
+      if (more_next) slots.fetch(A, next, c, buf ^ 1);
+      commit_copies();
+      wait_copies<1>();
+    } else {
+      held.fetch(A, u, c, on);
     }
+    Slope f[CH][V];
+#pragma unroll
+    for (int j = 0; j < CH; ++j) {
+      if (KIND == kPacked && (firsts >> j & 1)) {
+        const int64_t q = A.marks[t0 + j] >> 2;
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = A.h0 != nullptr ? A.h0[q * H + c + v] : 0.f;
+      }
+      float fx[V], fr[V], fi[V];
+      if constexpr (kAsync) {
+        slots.get(buf, j, 0, fx);
+        slots.get(buf, j, 1, fr);
+        slots.get(buf, j, 2, fi);
+      } else {
+        held.get(j, 0, fx);
+        held.get(j, 1, fr);
+        held.get(j, 2, fi);
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        Gate g = gate_of(fx[v], fr[v], fi[v], k[v]);  // of whatever the slot holds where the step does not count
+        if (!(on >> j & 1)) g = gate_shut();
+        f[j][v] = slope_of(g, h[v]);
+      }
+    }
+    T* out = static_cast<T*>(A.dp) + (row + CH * A.row_st) * 3 * H + c;
+#pragma unroll
+    for (int j = CH - 1; j >= 0; --j) {
+      out -= A.row_st * 3 * H;
+      if (u.tc + j >= u.steps) continue;
+      if (KIND == kPacked && (lasts >> j & 1)) {
+        const int64_t q = A.marks[t0 + j] >> 2;
+#pragma unroll
+        for (int v = 0; v < V; ++v) E[v] = A.dlast != nullptr ? A.dlast[q * H + c + v] : 0.f;
+      }
+      float dy[V], dx[V], dr[V], di[V];
+      if constexpr (kAsync) {
+        slots.get(buf, j, 3, dy);
+        if (A.dh == nullptr) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) dy[v] = 0.f;
+        }
+      } else {
+        held.d[j].get(dy);
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float g = dy[v] + E[v];
+        dx[v] = g * f[j][v].x;
+        dr[v] = g * f[j][v].r;
+        di[v] = g * f[j][v].i;
+        dl[v] = fmaf(g, f[j][v].l, dl[v]);
+        E[v] = g * f[j][v].a;
+      }
+      Pack<T, V> o;
+      o.set(dx);
+      o.store(out);
+      o.set(dr);
+      o.store(out + H);
+      o.set(di);
+      o.store(out + 2 * H);
+      if (KIND == kPacked && (firsts >> j & 1) && A.dh0 != nullptr) {
+        const int64_t q = A.marks[t0 + j] >> 2;
+#pragma unroll
+        for (int v = 0; v < V; ++v) A.dh0[q * H + c + v] = E[v];
+      }
+    }
+    fresh = u.tc == 0;
+    if (KIND != kPacked && fresh && u.q == 0 && A.dh0 != nullptr) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) A.dh0[u.b * H + c + v] = E[v];
+    }
+    u = next;
+    more = more_next;
+    buf ^= 1;
   }
   // the block's share of sum dz sigmoid(r), added up over its rows in order
-  __shared__ float sum[256 * V];
+  __shared__ float sum[kBwdThreads * V];
 #pragma unroll
   for (int v = 0; v < V; ++v) sum[threadIdx.x * V + v] = dl[v];
   __syncthreads();
@@ -290,38 +384,41 @@ struct BwdShape {
 // 16 steps' factors of one channel fit the registers, so do 8 of two and 4 of four
 BwdShape bwd_shape(const ScanArgs& a) {
   if (a.offsets == nullptr && a.steps <= 4) return {a.vec ? 4 : 1, 4};
-  if (a.offsets == nullptr && a.steps <= 8) return {a.vec ? 2 : 1, 8};
+  if (a.state_every == kStateShort || (a.offsets == nullptr && a.steps <= 8)) return {a.vec ? 2 : 1, 8};
   return {1, kStateEvery};
+}
+Lanes bwd_lanes(const ScanArgs& a) { return lanes_of(a.width, bwd_shape(a).V, false, kBwdThreads); }
+
+template <class T, int V, int CH, bool CODES, int KIND>
+void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
+  const Lanes l = bwd_lanes(a);
+  const dim3 grid(scan_bwd_blocks(a, p, sms), l.blocks);
+  const int threads = l.count * l.rows;
+  const bool async = !CODES && sizeof(T) * V >= 4;
+  const size_t smem = async ? static_cast<size_t>(threads) * 2 * CH * 4 * sizeof(T) * V : 0;
+  auto kernel = scan_bwd_kernel<T, V, CH, CODES, KIND>;
+  if (smem > 40 * 1024)
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  kernel<<<grid, threads, smem, st>>>(a, p, l);
 }
 
 template <class T, bool CODES, int KIND>
 void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
   const BwdShape b = bwd_shape(a);
-  const Lanes l = lanes_of(a.width, b.V, false);
-  const dim3 grid(scan_bwd_blocks(a, p, sms), l.blocks);
-  const int threads = l.count * l.rows;
-  if constexpr (KIND != kPacked) {
-    if (b.CH == 4) {
-      if (b.V == 4)
-        scan_bwd_kernel<T, 4, 4, CODES, KIND><<<grid, threads, 0, st>>>(a, p, l);
-      else
-        scan_bwd_kernel<T, 1, 4, CODES, KIND><<<grid, threads, 0, st>>>(a, p, l);
-      return;
-    }
-    if (b.CH == 8) {
-      if (b.V == 2)
-        scan_bwd_kernel<T, 2, 8, CODES, KIND><<<grid, threads, 0, st>>>(a, p, l);
-      else
-        scan_bwd_kernel<T, 1, 8, CODES, KIND><<<grid, threads, 0, st>>>(a, p, l);
-      return;
-    }
+  if (b.CH == 4) {
+    if constexpr (KIND != kPacked)
+      b.V == 4 ? run<T, 4, 4, CODES, KIND>(a, p, sms, st) : run<T, 1, 4, CODES, KIND>(a, p, sms, st);
+  } else if (b.CH == 8) {
+    if constexpr (KIND != kPacked || !CODES)
+      b.V == 2 ? run<T, 2, 8, CODES, KIND>(a, p, sms, st) : run<T, 1, 8, CODES, KIND>(a, p, sms, st);
+  } else {
+    if constexpr (CODES) run<T, 1, kStateEvery, CODES, KIND>(a, p, sms, st);
   }
-  scan_bwd_kernel<T, 1, kStateEvery, CODES, KIND><<<grid, threads, 0, st>>>(a, p, l);
 }
 
 template <class T, bool CODES, int KIND>
 void run_maps(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
-  const Lanes l = lanes_of(a.width, a.vec ? 4 : 1, false);
+  const Lanes l = lanes_of(a.width, a.vec ? 4 : 1, false, 256);
   const int64_t rows = (a.offsets != nullptr ? 1 : a.batch) * p.seg.n;
   const dim3 grid(row_blocks(rows, l, sms), l.blocks);
   const int threads = l.count * l.rows;
@@ -354,7 +451,7 @@ void run(const ScanArgs& a, const ScanPlan& p, bool maps, int sms, cudaStream_t 
 }  // namespace
 
 int scan_bwd_blocks(const ScanArgs& a, const ScanPlan& p, int sms) {
-  return row_blocks((a.offsets != nullptr ? 1 : a.batch) * p.seg.n, lanes_of(a.width, bwd_shape(a).V, false), sms);
+  return row_blocks((a.offsets != nullptr ? 1 : a.batch) * p.seg.n, bwd_lanes(a), sms);
 }
 void scan_bwd_maps(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) { run(a, p, true, sms, st); }
 void scan_bwd_rows(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) { run(a, p, false, sms, st); }

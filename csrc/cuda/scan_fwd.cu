@@ -32,7 +32,7 @@ struct Inputs {
 // Steps are taken U at a time: their inputs are loaded together, U x 3 loads of V values
 // under way per thread.
 template <class T, int V, int U, bool MAPS, bool CODES, int KIND>
-__global__ void __launch_bounds__(256) scan_fwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {
+__global__ void __launch_bounds__(256, 3) scan_fwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {
   const int y = threadIdx.x / L.count;
   const int c = (blockIdx.y * L.count + threadIdx.x % L.count) * V;
   const bool live = c < A.width;
@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(const ScanArgs A, const S
         in += A.p_st;
       }
       if (KIND == kPacked) mark += U;
-      if (!MAPS && A.states != nullptr && live && begin + t0 > 0 && t0 % kStateEvery == 0) {  // U divides kStateEvery
-        float* to = A.states + (s.b * A.n_states + (begin + t0) / kStateEvery - 1) * H + c;
+      if (!MAPS && A.states != nullptr && live && begin + t0 > 0 && t0 % A.state_every == 0) {  // U divides it
+        float* to = A.states + (s.b * A.n_states + (begin + t0) / A.state_every - 1) * H + c;
 #pragma unroll
         for (int v = 0; v < V; ++v) to[v] = h[v];
       }
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(256) scan_fwd_kernel(const ScanArgs A, const S
 
 template <class T, bool MAPS, bool CODES, int KIND>
 void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
-  const Lanes l = lanes_of(a.width, a.vec ? 4 : 1, CODES);
+  const Lanes l = lanes_of(a.width, a.vec ? 4 : 1, CODES, 256);
   const int64_t rows = (a.offsets != nullptr ? 1 : a.batch) * p.seg.n;
   const dim3 grid(row_blocks(rows, l, sms), l.blocks);
   const int threads = l.count * l.rows;

@@ -14,16 +14,16 @@ struct Lanes {
   int blocks;  // blocks over the channels
 };
 
-// Lanes of H channels at V per lane in blocks of up to 256 threads; with 8-bit codes every
-// group of 32 channels gets its own aligned lanes, the last one's beyond H included.
-inline Lanes lanes_of(int width, int V, bool codes) {
+// Lanes of H channels at V per lane in blocks of up to `threads` threads; with 8-bit codes
+// every group of 32 channels gets its own aligned lanes, the last one's beyond H included.
+inline Lanes lanes_of(int width, int V, bool codes, int threads) {
   const int unit = codes ? kGroup8 / V : 1;
   const int all = codes ? (width + kGroup8 - 1) / kGroup8 * unit : (width + V - 1) / V;
   Lanes l;
-  l.blocks = (all + 255) / 256;
+  l.blocks = (all + threads - 1) / threads;
   l.count = (all + l.blocks - 1) / l.blocks;
   l.count = (l.count + unit - 1) / unit * unit;
-  l.rows = 256 / l.count;
+  l.rows = threads / l.count;
   return l;
 }
 
@@ -59,7 +59,7 @@ inline ScanKind kind_of(const ScanArgs& a) {
 // blocks over `rows` rows of threads: every SM filled a few times, so that per-block sums stay few
 inline int row_blocks(int64_t rows, const Lanes& l, int sms) {
   const int64_t want = (rows + l.rows - 1) / l.rows;
-  const int64_t most = (static_cast<int64_t>(sms) * 8 + l.blocks - 1) / l.blocks;
+  const int64_t most = (static_cast<int64_t>(sms) * 12 + l.blocks - 1) / l.blocks;
   return static_cast<int>(want < most ? want : most);
 }
 

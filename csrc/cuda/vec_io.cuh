@@ -57,6 +57,22 @@ struct Pack {
   __device__ __forceinline__ void store(T* p) const { __stcs(reinterpret_cast<Raw*>(p), raw); }
 };
 
+// Copies of 4, 8 or 16 bytes from global to shared memory that the thread does not wait for:
+// committed in groups, of which wait_copies leaves the newest N under way. What a thread
+// copied is its own to read after that.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* smem, const void* p) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(smem)), "l"(p) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(smem)), "l"(p), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // one value of a parameter vector held in fp32 or bf16
 __device__ __forceinline__ float param_at(const void* p, int is_bf16, int64_t i) {
   return is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]) : static_cast<const float*>(p)[i];

@@ -67,7 +67,7 @@ ScanSizes scan_sizes(at::IntArrayRef shape, const OptTensor& offsets, int64_t pe
 
 // what forward and backward share: sequences, mask, decay, first states, layout of the dense rows
 ScanArgs scan_args(const ScanSizes& z, const at::Tensor& decay, const OptTensor& h0, const OptTensor& mask,
-                   const OptTensor& offsets, double rate, bool time_major, const at::Device& dev) {
+                   const OptTensor& offsets, double rate, bool time_major, bool codes, const at::Device& dev) {
   ScanArgs a;
   a.batch = z.batch;
   a.steps = z.steps;
@@ -101,7 +101,8 @@ ScanArgs scan_args(const ScanSizes& z, const at::Tensor& decay, const OptTensor&
   }
   a.row_sb = z.packed ? 0 : (time_major ? 1 : z.steps);
   a.row_st = z.packed ? 1 : (time_major ? z.batch : 1);
-  a.n_states = z.steps > 0 ? (z.steps - 1) / kStateEvery : 0;
+  a.state_every = codes ? kStateEvery : kStateShort;
+  a.n_states = z.steps > 0 ? (z.steps - 1) / a.state_every : 0;
   a.status = device_status_ptr(dev.index());
   return a;
 }
@@ -133,7 +134,7 @@ std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& de
   const ScanSizes z = scan_sizes(p.sizes(), offsets, 3);
   TORCH_CHECK(unit_last(p), "gated_scan: p must have unit stride along its last dimension");
   c10::cuda::CUDAGuard guard(p.device());
-  ScanArgs a = scan_args(z, decay, h0, mask, offsets, rate, time_major, p.device());
+  ScanArgs a = scan_args(z, decay, h0, mask, offsets, rate, time_major, keep8, p.device());
   a.bf16 = p.scalar_type() == at::kBFloat16;
   a.p = p.data_ptr();
   a.p_sb = z.packed ? 0 : p.stride(0);
@@ -179,7 +180,7 @@ std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptTensor& 
   const ScanSizes z = scan_sizes(like.sizes(), offsets, 3);
   const auto dev = like.device();
   c10::cuda::CUDAGuard guard(dev);
-  ScanArgs a = scan_args(z, decay, h0, mask, offsets, rate, time_major, dev);
+  ScanArgs a = scan_args(z, decay, h0, mask, offsets, rate, time_major, given(scales), dev);
   const auto f32 = like.options().dtype(at::kFloat);
   const auto type = bf16 ? at::kBFloat16 : at::kFloat;
   a.bf16 = bf16;

@@ -26,7 +26,7 @@ from torch.autograd.function import once_differentiable
 from starry_unigraph.ops import cuda_ext
 from starry_unigraph.ops.checkpoint8 import _dequantize_torch, _quantize_torch, check_checkpoint, exact
 
-STATE_EVERY = 16  # steps between the fp32 states kept for the backward pass
+STATE_EVERY = 16  # checkpoint="int8": steps between the fp32 states kept for the backward pass
 
 
 class _GatedScan(torch.autograd.Function):
@@ -158,8 +158,8 @@ def gated_scan(p: torch.Tensor, decay: torch.Tensor, h0: torch.Tensor | None = N
 
     checkpoint="int8" keeps p in 8 bits (``quantize8``'s format, each of x, r and i in groups
     of its own) for the backward pass instead of p itself: gradients are those at the
-    values of the codes. Either way fp32 states are kept every 16 steps and the ones in
-    between recomputed."""
+    values of the codes, the states between fp32 ones that are kept every 16 steps (packed: rows of
+    the packed axis) recomputed from them."""
     keep8 = check_checkpoint(checkpoint)
     if p.dim() != (3 if offsets is None else 2) or p.size(-1) == 0 or p.size(-1) % 3:
         raise ValueError("gated_scan: p must be [batch, steps, 3H], or [rows, 3H] with offsets")
