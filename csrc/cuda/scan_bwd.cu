@@ -1,5 +1,7 @@
 // Gated linear recurrence, backward (formulas in scan_math.cuh): a thread walks its channels
 // through one segment of one sequence, last step to first.
+#include <type_traits>
+
 #include "scan_shape.cuh"
 
 namespace su {
@@ -197,73 +199,80 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
     } else {
       held.fetch(A, u, c, on);
     }
-    Slope f[CH][V];
+    // WHOLE: every step of the chunk is inside the sequence and counts
+    auto work = [&](auto whole) {
+      constexpr bool WHOLE = decltype(whole)::value;
+      Slope f[CH][V];
 #pragma unroll
-    for (int j = 0; j < CH; ++j) {
-      if (KIND == kPacked && (firsts >> j & 1)) {
-        const int64_t q = A.marks[t0 + j] >> 2;
+      for (int j = 0; j < CH; ++j) {
+        if (KIND == kPacked && (firsts >> j & 1)) {
+          const int64_t q = A.marks[t0 + j] >> 2;
 #pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = A.h0 != nullptr ? A.h0[q * H + c + v] : 0.f;
-      }
-      float fx[V], fr[V], fi[V];
-      if constexpr (kAsync) {
-        slots.get(buf, j, 0, fx);
-        slots.get(buf, j, 1, fr);
-        slots.get(buf, j, 2, fi);
-      } else {
-        held.get(j, 0, fx);
-        held.get(j, 1, fr);
-        held.get(j, 2, fi);
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        Gate g = gate_of(fx[v], fr[v], fi[v], k[v]);  // of whatever the slot holds where the step does not count
-        if (!(on >> j & 1)) g = gate_shut();
-        f[j][v] = slope_of(g, h[v]);
-      }
-    }
-    T* out = static_cast<T*>(A.dp) + (row + CH * A.row_st) * 3 * H + c;
-#pragma unroll
-    for (int j = CH - 1; j >= 0; --j) {
-      out -= A.row_st * 3 * H;
-      if (u.tc + j >= u.steps) continue;
-      if (KIND == kPacked && (lasts >> j & 1)) {
-        const int64_t q = A.marks[t0 + j] >> 2;
-#pragma unroll
-        for (int v = 0; v < V; ++v) E[v] = A.dlast != nullptr ? A.dlast[q * H + c + v] : 0.f;
-      }
-      float dy[V], dx[V], dr[V], di[V];
-      if constexpr (kAsync) {
-        slots.get(buf, j, 3, dy);
-        if (A.dh == nullptr) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) dy[v] = 0.f;
+          for (int v = 0; v < V; ++v) h[v] = A.h0 != nullptr ? A.h0[q * H + c + v] : 0.f;
         }
-      } else {
-        held.d[j].get(dy);
-      }
+        float fx[V], fr[V], fi[V];
+        if constexpr (kAsync) {
+          slots.get(buf, j, 0, fx);
+          slots.get(buf, j, 1, fr);
+          slots.get(buf, j, 2, fi);
+        } else {
+          held.get(j, 0, fx);
+          held.get(j, 1, fr);
+          held.get(j, 2, fi);
+        }
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const float g = dy[v] + E[v];
-        dx[v] = g * f[j][v].x;
-        dr[v] = g * f[j][v].r;
-        di[v] = g * f[j][v].i;
-        dl[v] = fmaf(g, f[j][v].l, dl[v]);
-        E[v] = g * f[j][v].a;
+        for (int v = 0; v < V; ++v) {
+          if (!WHOLE && !(on >> j & 1)) shut(fx[v], fr[v], fi[v]);
+          f[j][v] = slope_of(gate_of(fx[v], fr[v], fi[v], k[v]), h[v]);
+        }
       }
-      Pack<T, V> o;
-      o.set(dx);
-      o.store(out);
-      o.set(dr);
-      o.store(out + H);
-      o.set(di);
-      o.store(out + 2 * H);
-      if (KIND == kPacked && (firsts >> j & 1) && A.dh0 != nullptr) {
-        const int64_t q = A.marks[t0 + j] >> 2;
+      T* out = static_cast<T*>(A.dp) + (row + CH * A.row_st) * 3 * H + c;
 #pragma unroll
-        for (int v = 0; v < V; ++v) A.dh0[q * H + c + v] = E[v];
+      for (int j = CH - 1; j >= 0; --j) {
+        out -= A.row_st * 3 * H;
+        if (!WHOLE && u.tc + j >= u.steps) continue;
+        if (KIND == kPacked && (lasts >> j & 1)) {
+          const int64_t q = A.marks[t0 + j] >> 2;
+#pragma unroll
+          for (int v = 0; v < V; ++v) E[v] = A.dlast != nullptr ? A.dlast[q * H + c + v] : 0.f;
+        }
+        float dy[V], dx[V], dr[V], di[V];
+        if constexpr (kAsync) {
+          slots.get(buf, j, 3, dy);
+          if (A.dh == nullptr) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) dy[v] = 0.f;
+          }
+        } else {
+          held.d[j].get(dy);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float g = dy[v] + E[v];
+          dx[v] = g * f[j][v].x;
+          dr[v] = g * f[j][v].r;
+          di[v] = g * f[j][v].i;
+          dl[v] = fmaf(g, f[j][v].l, dl[v]);
+          E[v] = g * f[j][v].a;
+        }
+        Pack<T, V> o;
+        o.set(dx);
+        o.store(out);
+        o.set(dr);
+        o.store(out + H);
+        o.set(di);
+        o.store(out + 2 * H);
+        if (KIND == kPacked && (firsts >> j & 1) && A.dh0 != nullptr) {
+          const int64_t q = A.marks[t0 + j] >> 2;
+#pragma unroll
+          for (int v = 0; v < V; ++v) A.dh0[q * H + c + v] = E[v];
+        }
       }
-    }
+    };
+    if (on == (1u << CH) - 1u)
+      work(std::true_type{});
+    else
+      work(std::false_type{});
     fresh = u.tc == 0;
     if (KIND != kPacked && fresh && u.q == 0 && A.dh0 != nullptr) {
 #pragma unroll

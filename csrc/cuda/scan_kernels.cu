@@ -152,18 +152,19 @@ void fill_packed(const ScanArgs& a, float* to, const float* from, cudaStream_t s
 
 }  // namespace
 
-// Segments: as many as give the SMs about 1024 threads each of forward lanes (4 channels where
-// rows are aligned), none shorter than 2 kStateEvery; at most 4096, whose states the carry
-// kernel walks in a few microseconds. Sequences that fill half of that by themselves are left whole:
-// the second read would cost more than the idle threads.
+// Segments: as many as fill the SMs once with the forward kernels' 768 threads each (lanes of 4
+// channels where rows are aligned; the backward kernel takes that in four whole rounds), none
+// shorter than 2 kStateEvery; at most 4096, whose states the carry kernel walks in a few
+// microseconds. Sequences that fill half of that by themselves are left whole: the second
+// read would cost more than the idle threads.
 ScanPlan scan_plan(const ScanArgs& a, int sms, void* workspace) {
   const int64_t batch = a.offsets != nullptr ? 1 : a.batch;
   const int64_t lanes = batch * ((a.width + (a.vec ? 3 : 0)) / (a.vec ? 4 : 1));
-  const int64_t want = static_cast<int64_t>(sms) * 1024;
+  const int64_t want = static_cast<int64_t>(sms) * 768;
   ScanPlan p;
   p.seg = {1, (a.steps + kStateEvery - 1) / kStateEvery * kStateEvery};
   if (lanes * 2 < want && a.steps > 4 * kStateEvery) {
-    int64_t n = (want + lanes - 1) / lanes;
+    int64_t n = want / lanes;
     n = n < 4096 ? n : 4096;
     int64_t len = (a.steps + n - 1) / n;
     len = len > 2 * kStateEvery ? len : 2 * kStateEvery;

@@ -75,7 +75,12 @@ __device__ __forceinline__ Gate gate_of(float x, float r, float i, float k) {
   g.z = fmaf(-z, g.sr, z);
   return g;
 }
-__device__ __forceinline__ Gate gate_shut() { return Gate{1.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
+// Inputs of a step that leaves the state as it is: sigmoid(r) = 0, so a = 1 and s = 0.
+__device__ __forceinline__ void shut(float& x, float& r, float& i) {
+  x = 0.f;
+  r = -1e30f;
+  i = 0.f;
+}
 
 struct Slope {
   float a, x, r, i, l;
