@@ -111,6 +111,7 @@ struct NormArgs {
   void* dw_pre = nullptr;
   void* dscale = nullptr;
   int vec = 1;                  // every row starts on a multiple of 4 values, H % 4 == 0
+  int vec8 = 0;                 // the same of 8
 };
 constexpr int kNormMaxWidth = 16384;
 int norm_partials(const NormArgs& a, int sms);
@@ -119,8 +120,8 @@ void launch_norm_bwd(const NormArgs& a, int sms, cudaStream_t st);
 
 // 8-bit codes of dense rows
 void launch_quantize8(const void* x, int bf16, int64_t ld, int64_t rows, int width, int8_t* codes, float* scales,
-                      int vec, cudaStream_t st);
+                      int vec, int sms, cudaStream_t st);
 void launch_dequantize8(const int8_t* codes, const float* scales, int64_t rows, int width, void* x, int bf16, int vec,
-                        cudaStream_t st);
+                        int sms, cudaStream_t st);
 
 }  // namespace su

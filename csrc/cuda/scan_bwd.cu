@@ -220,11 +220,14 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
           held.get(j, 1, fr);
           held.get(j, 2, fi);
         }
+        if (!WHOLE && !(on >> j & 1)) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          if (!WHOLE && !(on >> j & 1)) shut(fx[v], fr[v], fi[v]);
-          f[j][v] = slope_of(gate_of(fx[v], fr[v], fi[v], k[v]), h[v]);
+          for (int v = 0; v < V; ++v) shut(fx[v], fr[v], fi[v]);
         }
+        Gate g[V];
+        gates_of(fx, fr, fi, k, g);
+#pragma unroll
+        for (int v = 0; v < V; ++v) f[j][v] = slope_of(g[v], h[v]);
       }
       T* out = static_cast<T*>(A.dp) + (row + CH * A.row_st) * 3 * H + c;
 #pragma unroll
@@ -322,38 +325,49 @@ __global__ void __launch_bounds__(256) scan_bwd_maps_kernel(const ScanArgs A, co
       m[v] = 1.f;
       E[v] = 0.f;
     }
-    for (int tc = (steps + U - 1) / U * U - U; tc >= 0; tc -= U) {
-      const int64_t t0 = begin + tc;
+    int tc = (steps + U - 1) / U * U;
+    const int64_t end = s.b * A.row_sb + (begin + tc) * A.row_st;
+    const T* in = CODES ? nullptr : static_cast<const T*>(A.p) + s.b * A.p_sb + (begin + tc) * A.p_st + H + c;
+    const int8_t* code = CODES ? A.codes + end * 3 * H + H + c : nullptr;
+    const float* sc = CODES ? A.scales + end * 3 * G + G + c / kGroup8 : nullptr;
+    const T* dh = static_cast<const T*>(A.dh) + (A.dh != nullptr ? s.b * A.dh_sb + (begin + tc) * A.dh_st + c : 0);
+    const uint8_t* valid = A.mask != nullptr ? A.mask + s.b * A.m_sb + (begin + tc) * A.m_st : nullptr;
+    while (tc > 0) {
+      tc -= U;
       Pack<T, V> r[U], d[U];
       Codes<V> q[U];
       float scale[U];
       bool on[U];
       int mk[U];
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int64_t t = t0 + j;
+      for (int j = U - 1; j >= 0; --j) {
         const bool inside = tc + j < steps;
         on[j] = inside;
-        if (KIND == kMasked || (KIND == kPacked && A.mask != nullptr))
-          on[j] = inside && A.mask[s.b * A.m_sb + t * A.m_st] != 0;
+        if (KIND == kMasked || (KIND == kPacked && A.mask != nullptr)) {
+          valid -= A.m_st;
+          if (inside) on[j] = *valid != 0;
+        }
         mk[j] = -1;
         if (KIND == kPacked) {
-          if (inside) mk[j] = A.marks[t];
+          if (inside) mk[j] = A.marks[begin + tc + j];
         }
         r[j].zero();
         q[j].zero();
         scale[j] = 0.f;
-        if (on[j]) {
-          if constexpr (CODES) {
-            const int64_t row = s.b * A.row_sb + t * A.row_st;
-            q[j].load(A.codes + row * 3 * H + H + c);
-            scale[j] = A.scales[row * 3 * G + G + c / kGroup8];
-          } else {
-            r[j].load_keep(static_cast<const T*>(A.p) + s.b * A.p_sb + t * A.p_st + H + c);
+        if constexpr (CODES) {
+          code -= A.row_st * 3 * H;
+          sc -= A.row_st * 3 * G;
+          if (on[j]) {
+            q[j].load(code);
+            scale[j] = *sc;
           }
+        } else {
+          in -= A.p_st;
+          if (on[j]) r[j].load_keep(in);
         }
         d[j].zero();
-        if (inside && A.dh != nullptr) d[j].load_keep(static_cast<const T*>(A.dh) + s.b * A.dh_sb + t * A.dh_st + c);
+        dh -= A.dh_st;
+        if (inside && A.dh != nullptr) d[j].load_keep(dh);
       }
 #pragma unroll
       for (int j = U - 1; j >= 0; --j) {
@@ -371,14 +385,16 @@ __global__ void __launch_bounds__(256) scan_bwd_maps_kernel(const ScanArgs A, co
           q[j].get(scale[j], fr);
         else
           r[j].get(fr);
+        float a[V];
+        if (!on[j]) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) fr[v] = -1e30f;  // a = 1; dh is 0 beyond the last step
+        }
+        decays_of(fr, k, a);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          E[v] += fd[v];
-          if (on[j]) {
-            const float a = decay_of(fr[v], k[v]);
-            E[v] *= a;
-            m[v] *= a;
-          }
+          E[v] = a[v] * (E[v] + fd[v]);
+          m[v] *= a[v];
         }
       }
     }

@@ -127,13 +127,16 @@ __global__ void __launch_bounds__(256, 3) scan_fwd_kernel(const ScanArgs A, cons
             m[v] = 0.f;
           }
         }
-        if (KIND == kPlain || on[j]) {
+        if (KIND != kPlain && !on[j]) {
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const Step g = step_of(fx[v], fr[v], fi[v], k[v]);
-            h[v] = fmaf(g.a, h[v], g.add);
-            if (MAPS) m[v] *= g.a;
-          }
+          for (int v = 0; v < V; ++v) shut(fx[v], fr[v], fi[v]);
+        }
+        Step g[V];
+        steps_of(fx, fr, fi, k, g);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          h[v] = fmaf(g[v].a, h[v], g[v].add);
+          if (MAPS) m[v] *= g[v].a;
         }
         if (!MAPS) {
           if (live) {

@@ -123,16 +123,17 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanStepArgs A) {
   const int64_t row = e / A.width;
   const int c = static_cast<int>(e - row * A.width);
   const T* p = static_cast<const T*>(A.p) + row * A.p_sb + c;
-  const float x = to_f32(p[0]), r = to_f32(p[A.width]), i = to_f32(p[2 * static_cast<int64_t>(A.width)]);
-  const float k = decay_factor(param_at(A.decay, A.decay_bf16, c), A.rate);
+  const float x[1] = {to_f32(p[0])}, r[1] = {to_f32(p[A.width])}, i[1] = {to_f32(p[2 * static_cast<int64_t>(A.width)])};
+  const float k[1] = {decay_factor(param_at(A.decay, A.decay_bf16, c), A.rate)};
   const int64_t at = A.index != nullptr ? A.index[row] : row;
   float h = 0.f;
   if (at < 0 || at >= A.table_rows) {
     record_status(A.status, kBadIndex);  // the row is left out
   } else {
     float* to = A.state + at * A.state_sb + c;
-    const Step g = step_of(x, r, i, k);
-    h = fmaf(g.a, *to, g.add);
+    Step g[1];
+    steps_of(x, r, i, k, g);
+    h = fmaf(g[0].a, *to, g[0].add);
     *to = h;
   }
   static_cast<T*>(A.h)[e] = from_f32<T>(h);

@@ -21,18 +21,30 @@
 
 namespace su {
 
-// 1 - exp(z) for z <= 0. Taylor's series up to z^6 where |z| <= 0.25 (remainder below
-// 0.25^6 / 7! = 5e-8 of the result), else the difference, which cancels at most two bits.
-// The exponential is issued only where some lane of the warp needs it.
-__device__ __forceinline__ float one_minus_exp(float z) {
-  float t = fmaf(z, 1.f / 720.f, 1.f / 120.f);
-  t = fmaf(z, t, 1.f / 24.f);
-  t = fmaf(z, t, 1.f / 6.f);
-  t = fmaf(z, t, 0.5f);
-  t = fmaf(z, t, 1.f);
-  float em = -z * t;
-  if (z < -0.25f) em = 1.f - ex2_f(kLog2e * z);
-  return em;
+// 1 - exp(z) for V values z <= 0. Taylor's series up to z^6 where |z| <= 0.25 (remainder below
+// 0.25^6 / 7! = 5e-8 of the result), else the difference, which cancels at most two bits. A
+// thread whose V values are all small, the rule for a memory of many steps, branches past
+// the exponentials: the special-function unit is what bounds bf16 inputs.
+template <int V>
+__device__ __forceinline__ void one_minus_exp(const float (&z)[V], float (&em)[V]) {
+  float least = z[0];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float t = fmaf(z[v], 1.f / 720.f, 1.f / 120.f);
+    t = fmaf(z[v], t, 1.f / 24.f);
+    t = fmaf(z[v], t, 1.f / 6.f);
+    t = fmaf(z[v], t, 0.5f);
+    t = fmaf(z[v], t, 1.f);
+    em[v] = -z[v] * t;
+    least = fminf(least, z[v]);
+  }
+  if (least < -0.25f) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const float e = 1.f - ex2_f(kLog2e * z[v]);
+      em[v] = z[v] < -0.25f ? e : em[v];
+    }
+  }
 }
 
 // -c softplus(decay)
@@ -44,14 +56,28 @@ __device__ __forceinline__ float decay_factor(float decay, float rate) {
 struct Step {
   float a, add;
 };
-__device__ __forceinline__ Step step_of(float x, float r, float i, float k) {
-  const float em = one_minus_exp(k * sigmoid_f(r));
-  Step g;
-  g.a = 1.f - em;
-  g.add = sqrt_f(em * (1.f + g.a)) * sigmoid_f(i) * x;
-  return g;
+template <int V>
+__device__ __forceinline__ void steps_of(const float (&x)[V], const float (&r)[V], const float (&i)[V],
+                                         const float (&k)[V], Step (&g)[V]) {
+  float z[V], em[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) z[v] = k[v] * sigmoid_f(r[v]);
+  one_minus_exp(z, em);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    g[v].a = 1.f - em[v];
+    g[v].add = sqrt_f(em[v] * (1.f + g[v].a)) * sigmoid_f(i[v]) * x[v];
+  }
 }
-__device__ __forceinline__ float decay_of(float r, float k) { return 1.f - one_minus_exp(k * sigmoid_f(r)); }
+template <int V>
+__device__ __forceinline__ void decays_of(const float (&r)[V], const float (&k)[V], float (&a)[V]) {
+  float z[V], em[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) z[v] = k[v] * sigmoid_f(r[v]);
+  one_minus_exp(z, em);
+#pragma unroll
+  for (int v = 0; v < V; ++v) a[v] = 1.f - em[v];
+}
 
 // One step's gradients are products with g, the gradient at h_t: dx = g x, dr = g r,
 // di = g i, the share of ddecay's sum is g l and a g goes on to h_{t-1}. `Gate` is what the
@@ -59,21 +85,28 @@ __device__ __forceinline__ float decay_of(float r, float k) { return 1.f - one_m
 struct Gate {
   float a, x, i, add, q, z, sr;
 };
-__device__ __forceinline__ Gate gate_of(float x, float r, float i, float k) {
-  Gate g;
-  g.sr = sigmoid_f(r);
-  const float si = sigmoid_f(i);
-  const float z = k * g.sr;
-  const float em = one_minus_exp(z);
-  g.a = 1.f - em;
-  const float ss = em * (1.f + g.a);
-  const float rs = rsqrt_f(fmaxf(ss, 1.2e-38f));  // finite where the gate is closed; s and z are 0 there
-  g.x = ss * rs * si;
-  g.add = g.x * x;
-  g.i = fmaf(-g.add, si, g.add);
-  g.q = g.a * rs * (si * x);
-  g.z = fmaf(-z, g.sr, z);
-  return g;
+template <int V>
+__device__ __forceinline__ void gates_of(const float (&x)[V], const float (&r)[V], const float (&i)[V],
+                                         const float (&k)[V], Gate (&g)[V]) {
+  float z[V], em[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    g[v].sr = sigmoid_f(r[v]);
+    z[v] = k[v] * g[v].sr;
+  }
+  one_minus_exp(z, em);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const float si = sigmoid_f(i[v]);
+    g[v].a = 1.f - em[v];
+    const float ss = em[v] * (1.f + g[v].a);
+    const float rs = rsqrt_f(fmaxf(ss, 1.2e-38f));  // finite where the gate is closed; s and z are 0 there
+    g[v].x = ss * rs * si;
+    g[v].add = g[v].x * x[v];
+    g[v].i = fmaf(-g[v].add, si, g[v].add);
+    g[v].q = g[v].a * rs * (si * x[v]);
+    g[v].z = fmaf(-z[v], g[v].sr, z[v]);
+  }
 }
 // Inputs of a step that leaves the state as it is: sigmoid(r) = 0, so a = 1 and s = 0.
 __device__ __forceinline__ void shut(float& x, float& r, float& i) {

@@ -26,13 +26,14 @@ std::string str(at::IntArrayRef v) {
 // (of a tensor without values any stride will do: torch gives such tensors any)
 bool unit_last(const at::Tensor& t) { return t.numel() == 0 || t.size(-1) == 1 || t.stride(-1) == 1; }
 
-// rows that start on multiples of 4 values: base and strides of a tensor with unit last stride
-bool rows_of_four(const at::Tensor& t) {
-  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % (4 * t.element_size()) != 0) return false;
+// rows that start on multiples of n values: base and strides of a tensor with unit last stride
+bool rows_of(int n, const at::Tensor& t) {
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % (n * t.element_size()) != 0) return false;
   for (int64_t d = 0; d + 1 < t.dim(); ++d)
-    if (t.size(d) > 1 && t.stride(d) % 4 != 0) return false;
-  return t.size(-1) % 4 == 0;
+    if (t.size(d) > 1 && t.stride(d) % n != 0) return false;
+  return t.size(-1) % n == 0;
 }
+bool rows_of_four(const at::Tensor& t) { return rows_of(4, t); }
 
 void check_param(const at::Tensor& t, const char* name, int64_t width, const at::Device& dev) {
   TORCH_CHECK(t.device() == dev, name, " must be on ", dev);
@@ -315,12 +316,14 @@ std::vector<at::Tensor> norm_residual_fwd(const at::Tensor& x, const OptTensor& 
   a.x = x.data_ptr();
   a.x_ld = x.stride(0);
   a.vec = rows_of_four(x);
+  a.vec8 = rows_of(8, x);
   int64_t parts = 1;
   if (given(u)) {
     check_rows(*u, "norm_residual: u", x);
     a.u = u->data_ptr();
     a.u_ld = u->stride(0);
     a.vec = a.vec && rows_of_four(*u);
+    a.vec8 = a.vec8 && rows_of(8, *u);
     ++parts;
   }
   if (given(gate)) {
@@ -329,6 +332,7 @@ std::vector<at::Tensor> norm_residual_fwd(const at::Tensor& x, const OptTensor& 
     a.gate = gate->data_ptr();
     a.gate_ld = gate->stride(0);
     a.vec = a.vec && rows_of_four(*gate);
+    a.vec8 = a.vec8 && rows_of(8, *gate);
     ++parts;
   }
   const int64_t H = a.width;
@@ -370,6 +374,7 @@ std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const OptTensor& 
   a.bf16 = bf16;
   a.rows = x.size(-2);
   a.vec = H % 4 == 0;
+  a.vec8 = H % 8 == 0;
   bool has_u, has_gate;
   if (given(scales)) {
     TORCH_CHECK(x.scalar_type() == at::kChar && x.dim() == 3, "norm_residual: malformed 8-bit inputs");
@@ -385,17 +390,20 @@ std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const OptTensor& 
     a.x = x.data_ptr();
     a.x_ld = x.stride(0);
     a.vec = a.vec && rows_of_four(x);
+    a.vec8 = a.vec8 && rows_of(8, x);
     has_u = given(u);
     has_gate = given(gate);
     if (has_u) {
       a.u = u->data_ptr();
       a.u_ld = u->stride(0);
       a.vec = a.vec && rows_of_four(*u);
+      a.vec8 = a.vec8 && rows_of(8, *u);
     }
     if (has_gate) {
       a.gate = gate->data_ptr();
       a.gate_ld = gate->stride(0);
       a.vec = a.vec && rows_of_four(*gate);
+      a.vec8 = a.vec8 && rows_of(8, *gate);
     }
   }
   auto grad = [&](const OptTensor& t, const void*& ptr, int64_t& ld) {
@@ -405,6 +413,7 @@ std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const OptTensor& 
     ptr = t->data_ptr();
     ld = t->stride(0);
     a.vec = a.vec && rows_of_four(*t);
+    a.vec8 = a.vec8 && rows_of(8, *t);
   };
   grad(dy, a.dy, a.dy_ld);
   if (given(w_pre)) grad(dn, a.dn, a.dn_ld);
@@ -450,7 +459,7 @@ std::vector<at::Tensor> quantize8(const at::Tensor& x) {
   at::Tensor scales = at::empty({rows, groups_of(H)}, x.options().dtype(at::kFloat));
   if (rows == 0) return {codes, scales};
   launch_quantize8(x.data_ptr(), x.scalar_type() == at::kBFloat16, x.stride(0), rows, static_cast<int>(H),
-                   codes.data_ptr<int8_t>(), scales.data_ptr<float>(), rows_of_four(x), cur_stream());
+                   codes.data_ptr<int8_t>(), scales.data_ptr<float>(), rows_of_four(x), num_sms(x.get_device()), cur_stream());
   SU_LAUNCH_CHECK();
   return {codes, scales};
 }
@@ -471,7 +480,7 @@ at::Tensor dequantize8(const at::Tensor& codes, const at::Tensor& scales, bool b
   if (x.numel() == 0) return x;
   const bool vec = H % 4 == 0 && reinterpret_cast<uintptr_t>(codes.data_ptr()) % 4 == 0;
   launch_dequantize8(codes.data_ptr<int8_t>(), scales.data_ptr<float>(), rows, static_cast<int>(H), x.data_ptr(), bf16,
-                     vec, cur_stream());
+                     vec, num_sms(codes.get_device()), cur_stream());
   SU_LAUNCH_CHECK();
   return x;
 }
