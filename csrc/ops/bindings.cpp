@@ -178,32 +178,16 @@ void jodie_project_bwd(const at::Tensor& roots, const at::Tensor& n_roots, const
                        const c10::optional<at::Tensor>& peer);
 
 // recurrence_ops.cpp
-std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& decay,
-                                       const c10::optional<at::Tensor>& h0, const c10::optional<at::Tensor>& mask,
-                                       const c10::optional<at::Tensor>& offsets, double rate, bool time_major,
-                                       bool keep_states, bool keep8);
-std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const c10::optional<at::Tensor>& scales,
-                                       const at::Tensor& states, const at::Tensor& decay,
-                                       const c10::optional<at::Tensor>& h0, const c10::optional<at::Tensor>& mask,
-                                       const c10::optional<at::Tensor>& offsets,
-                                       const c10::optional<at::Tensor>& marks, const c10::optional<at::Tensor>& dh,
-                                       const c10::optional<at::Tensor>& dlast, double rate, bool time_major, bool bf16,
-                                       bool need_dh0);
+std::tuple<at::Tensor, at::Tensor> gated_scan(const at::Tensor& p, const at::Tensor& decay,
+                                              const c10::optional<at::Tensor>& h0,
+                                              const c10::optional<at::Tensor>& mask,
+                                              const c10::optional<at::Tensor>& offsets, double rate, bool keep8);
 at::Tensor gated_scan_step(const at::Tensor& p, const at::Tensor& decay, at::Tensor& state,
                            const c10::optional<at::Tensor>& rows, double rate);
-std::vector<at::Tensor> norm_residual_fwd(const at::Tensor& x, const c10::optional<at::Tensor>& u,
-                                          const c10::optional<at::Tensor>& gate,
-                                          const c10::optional<at::Tensor>& w_post,
-                                          const c10::optional<at::Tensor>& w_pre,
-                                          const c10::optional<at::Tensor>& scale, double eps, bool keep8);
-std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const c10::optional<at::Tensor>& u,
-                                          const c10::optional<at::Tensor>& gate,
-                                          const c10::optional<at::Tensor>& scales,
-                                          const c10::optional<at::Tensor>& w_post,
-                                          const c10::optional<at::Tensor>& w_pre,
-                                          const c10::optional<at::Tensor>& scale, double eps,
-                                          const c10::optional<at::Tensor>& dy, const c10::optional<at::Tensor>& dn,
-                                          bool bf16);
+std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>> norm_residual(
+    const at::Tensor& x, const c10::optional<at::Tensor>& u, const c10::optional<at::Tensor>& gate,
+    const c10::optional<at::Tensor>& w_post, const c10::optional<at::Tensor>& w_pre,
+    const c10::optional<at::Tensor>& scale, double eps, bool keep8);
 std::vector<at::Tensor> quantize8(const at::Tensor& x);
 at::Tensor dequantize8(const at::Tensor& codes, const at::Tensor& scales, bool bf16);
 
@@ -273,11 +257,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("halo"), py::arg("n_rows"), py::arg("plan") = py::none());
   m.def("lstm_fwd", &lstm_fwd);
   m.def("lstm_bwd", &lstm_bwd);
-  m.def("gated_scan_fwd", &gated_scan_fwd);
-  m.def("gated_scan_bwd", &gated_scan_bwd);
+  m.def("gated_scan", &gated_scan);
   m.def("gated_scan_step", &gated_scan_step);
-  m.def("norm_residual_fwd", &norm_residual_fwd);
-  m.def("norm_residual_bwd", &norm_residual_bwd);
+  m.def("norm_residual", &norm_residual);
   m.def("quantize8", &quantize8);
   m.def("dequantize8", &dequantize8);
 }

@@ -127,7 +127,7 @@ int64_t groups_of(int64_t width) { return (width + kGroup8 - 1) / kGroup8; }
 
 // -> h, last state, kept states, codes, scales (those three undefined where not kept), marks of
 // packed sequences
-std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& decay, const OptTensor& h0,
+static std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& decay, const OptTensor& h0,
                                        const OptTensor& mask, const OptTensor& offsets, double rate, bool time_major,
                                        bool keep_states, bool keep8) {
   SU_CHECK_CUDA(p);
@@ -173,7 +173,7 @@ std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Tensor& de
 
 // `like`: p, or its 8-bit codes with `scales` (then the gradients have the type of h, `bf16`)
 // -> dp, ddecay, dh0
-std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptTensor& scales, const at::Tensor& states,
+static std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptTensor& scales, const at::Tensor& states,
                                        const at::Tensor& decay, const OptTensor& h0, const OptTensor& mask,
                                        const OptTensor& offsets, const OptTensor& marks, const OptTensor& dh,
                                        const OptTensor& dlast, double rate, bool time_major, bool bf16, bool need_dh0) {
@@ -235,9 +235,79 @@ std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptTensor& 
   return {dp, ddecay, dh0};
 }
 
-at::Tensor gated_scan_step(const at::Tensor& p, const at::Tensor& decay, at::Tensor& state, const OptTensor& rows,
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// A tensor that saved-tensor hooks leave alone: its bits as int32 (hooks that compress
+// activations take floating tensors).
+at::Tensor hidden(const at::Tensor& t) { return t.defined() ? t.view(at::kInt) : t; }
+at::Tensor shown(const at::Tensor& t) { return t.defined() ? t.view(at::kFloat) : t; }
+OptTensor maybe(const at::Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
+at::Tensor value(const OptTensor& t) { return given(t) ? *t : at::Tensor(); }
+
+void check_once(const char* name) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), name, ": its gradient cannot be differentiated again (create_graph)");
+}
+
+struct GatedScan : public torch::autograd::Function<GatedScan> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& p, const at::Tensor& decay,
+                               const OptTensor& h0, const OptTensor& mask, const OptTensor& offsets, double rate,
+                               bool time_major, bool keep8) {
+    auto out = gated_scan_fwd(p, decay, h0, mask, offsets, rate, time_major, true, keep8);
+    ctx->save_for_backward({keep8 ? out[3] : p, hidden(out[4]), hidden(out[2]), decay, hidden(value(h0)), value(mask),
+                            value(offsets), out[5]});
+    ctx->saved_data["rate"] = rate;
+    ctx->saved_data["time_major"] = time_major;
+    ctx->saved_data["bf16"] = p.scalar_type() == at::kBFloat16;
+    ctx->set_materialize_grads(false);
+    return {out[0], out[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once("gated_scan");
+    const auto v = ctx->get_saved_variables();
+    at::Tensor dh = grads[0], dlast = grads[1];
+    if (dh.defined() && !unit_last(dh)) dh = dh.contiguous();
+    if (dlast.defined()) dlast = dlast.contiguous();
+    auto g = gated_scan_bwd(v[0], maybe(shown(v[1])), shown(v[2]), v[3], maybe(shown(v[4])), maybe(v[5]), maybe(v[6]),
+                            maybe(v[7]), maybe(dh), maybe(dlast), ctx->saved_data["rate"].toDouble(),
+                            ctx->saved_data["time_major"].toBool(), ctx->saved_data["bf16"].toBool(),
+                            v[4].defined() && ctx->needs_input_grad(2));  // p, decay, h0: the tensors given
+    return {g[0], g[1], g[2], {}, {}, {}, {}, {}};
+  }
+};
+
+bool wants_grad(std::initializer_list<at::Tensor> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const auto& t : ts)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+
+}  // namespace
+
+// The op as the Python package calls it: layout of the dense rows, autograd.
+std::tuple<at::Tensor, at::Tensor> gated_scan(const at::Tensor& p_in, const at::Tensor& decay_in,
+                                              const OptTensor& h0_in, const OptTensor& mask, const OptTensor& offsets,
+                                              double rate, bool keep8) {
+  scan_sizes(p_in.sizes(), offsets, 3);
+  const at::Tensor p = unit_last(p_in) ? p_in : p_in.contiguous();
+  const at::Tensor decay = decay_in.contiguous();
+  const at::Tensor h0 = given(h0_in) ? h0_in->to(at::kFloat).contiguous() : at::Tensor();
+  const bool time_major = !given(offsets) && p.stride(1) > p.stride(0);
+  if (wants_grad({p, decay, h0})) {
+    auto out = GatedScan::apply(p, decay, maybe(h0), mask, offsets, rate, time_major, keep8);
+    return {out[0], out[1]};
+  }
+  auto out = gated_scan_fwd(p, decay, maybe(h0), mask, offsets, rate, time_major, false, false);
+  return {out[0], out[1]};
+}
+
+at::Tensor gated_scan_step(const at::Tensor& p_in, const at::Tensor& decay, at::Tensor& state, const OptTensor& rows,
                            double rate) {
-  SU_CHECK_CUDA(p);
+  SU_CHECK_CUDA(p_in);
+  const at::Tensor p = unit_last(p_in) ? p_in : p_in.detach().contiguous();
   TORCH_CHECK(is_float_type(p), "gated_scan_step: p must be float32 or bfloat16");
   TORCH_CHECK(p.dim() == 2 && p.size(1) > 0 && p.size(1) % 3 == 0 && unit_last(p),
               "gated_scan_step: p must be [rows, 3H] with unit stride along its last dimension");
@@ -303,7 +373,7 @@ NormArgs norm_args(const at::Tensor& x, int64_t width, const OptTensor& w_post, 
 }  // namespace
 
 // x, u, gate [rows, H] -> y (undefined without u), n (undefined without w_pre), codes, scales
-std::vector<at::Tensor> norm_residual_fwd(const at::Tensor& x, const OptTensor& u, const OptTensor& gate,
+static std::vector<at::Tensor> norm_residual_fwd(const at::Tensor& x, const OptTensor& u, const OptTensor& gate,
                                           const OptTensor& w_post, const OptTensor& w_pre, const OptTensor& scale,
                                           double eps, bool keep8) {
   SU_CHECK_CUDA(x);
@@ -361,7 +431,7 @@ std::vector<at::Tensor> norm_residual_fwd(const at::Tensor& x, const OptTensor& 
 
 // x, u, gate: the forward's rows, or (keep8) undefined u and gate with x = codes and `scales`
 // -> dx, du, dgate, dw_post, dw_pre, dscale (undefined where there is nothing to differentiate)
-std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const OptTensor& u, const OptTensor& gate,
+static std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const OptTensor& u, const OptTensor& gate,
                                           const OptTensor& scales, const OptTensor& w_post, const OptTensor& w_pre,
                                           const OptTensor& scale, double eps, const OptTensor& dy, const OptTensor& dn,
                                           bool bf16) {
@@ -445,6 +515,86 @@ std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const OptTensor& 
     SU_LAUNCH_CHECK();
   }
   return {dx, du, dgate, dw_post, dw_pre, dscale};
+}
+
+namespace {
+
+// [rows, H] of any shape, unit last stride (a copy where the rows cannot be one dimension)
+at::Tensor as_rows(const at::Tensor& t, int64_t width) {
+  if (!t.defined()) return t;
+  at::Tensor r = t.dim() == 2 ? t : t.reshape({-1, width});
+  return unit_last(r) ? r : r.contiguous();
+}
+at::Tensor like_shape(const at::Tensor& t, at::IntArrayRef shape) {
+  return !t.defined() || t.sizes() == shape ? t : t.view(shape);
+}
+
+struct NormResidual : public torch::autograd::Function<NormResidual> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& u, const OptTensor& gate,
+                               const OptTensor& w_post, const OptTensor& w_pre, const OptTensor& scale, double eps,
+                               bool keep8) {
+    const int64_t H = x.size(-1);
+    auto out = norm_residual_fwd(as_rows(x, H), maybe(as_rows(value(u), H)), maybe(as_rows(value(gate), H)), w_post,
+                                 w_pre, scale, eps, keep8);
+    if (keep8)
+      ctx->save_for_backward({out[2], {}, {}, hidden(out[3]), value(w_post), value(w_pre), value(scale)});
+    else
+      ctx->save_for_backward({x, value(u), value(gate), {}, value(w_post), value(w_pre), value(scale)});
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["bf16"] = x.scalar_type() == at::kBFloat16;
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["has_y"] = out[0].defined();
+    ctx->set_materialize_grads(false);
+    variable_list both;
+    for (int k = 0; k < 2; ++k)
+      if (out[k].defined()) both.push_back(like_shape(out[k], x.sizes()));
+    return both;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    check_once("norm_residual");
+    const auto v = ctx->get_saved_variables();
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const int64_t H = shape.back();
+    const bool keep8 = v[3].defined();
+    const bool has_y = ctx->saved_data["has_y"].toBool();
+    const at::Tensor dy = has_y ? grads[0] : at::Tensor();
+    const at::Tensor dn = has_y ? (grads.size() > 1 ? grads[1] : at::Tensor()) : grads[0];
+    auto g = norm_residual_bwd(keep8 ? v[0] : as_rows(v[0], H), maybe(as_rows(v[1], H)), maybe(as_rows(v[2], H)),
+                               maybe(shown(v[3])), maybe(v[4]), maybe(v[5]), maybe(v[6]),
+                               ctx->saved_data["eps"].toDouble(), maybe(as_rows(dy, H)), maybe(as_rows(dn, H)),
+                               ctx->saved_data["bf16"].toBool());
+    return {like_shape(g[0], shape), like_shape(g[1], shape), like_shape(g[2], shape), g[3], g[4], g[5], {}, {}};
+  }
+};
+
+}  // namespace
+
+// The op as the Python package calls it: any shape [.., H], autograd. -> y (None without u), n (None
+// without w_pre)
+std::tuple<OptTensor, OptTensor> norm_residual(const at::Tensor& x, const OptTensor& u_in, const OptTensor& gate_in,
+                                               const OptTensor& post_in, const OptTensor& pre_in,
+                                               const OptTensor& scale_in, double eps, bool keep8) {
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "norm_residual: x needs a last dimension of at least one value");
+  const at::Tensor u = value(u_in), gate = value(gate_in);
+  const auto vec = [](const OptTensor& t) { return given(t) ? t->contiguous() : at::Tensor(); };
+  const at::Tensor w_post = vec(post_in), w_pre = vec(pre_in), scale = vec(scale_in);
+  for (const auto& t : {u, gate})
+    TORCH_CHECK(!t.defined() || (t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device()),
+                "norm_residual: u and gate must have x's shape, type and device");
+  at::Tensor y, n;
+  if (wants_grad({x, u, gate, w_post, w_pre, scale})) {
+    auto out = NormResidual::apply(x, maybe(u), maybe(gate), maybe(w_post), maybe(w_pre), maybe(scale), eps, keep8);
+    size_t k = 0;
+    if (u.defined()) y = out[k++];
+    if (w_pre.defined()) n = out[k];
+  } else {
+    const int64_t H = x.size(-1);
+    auto out = norm_residual_fwd(as_rows(x, H), maybe(as_rows(u, H)), maybe(as_rows(gate, H)), maybe(w_post),
+                                 maybe(w_pre), maybe(scale), eps, false);
+    y = like_shape(out[0], x.sizes());
+    n = like_shape(out[1], x.sizes());
+  }
+  return {maybe(y), maybe(n)};
 }
 
 // x [rows, H] -> codes [rows, H], scales [rows, ceil(H / 32)]

@@ -10,8 +10,8 @@ so that a broken activation shows in the gradients.
 * ``quantize8(x)`` -> ``Packed8``; ``Packed8.dequantize(dtype=None)`` back to x's type.
 * ``with saved8(): loss = model(...)``: every activation that an autograd node of the
   block saves is kept in 8 bits (the framework's own ops and torch's alike) and restored
-  when its backward pass asks for it. Parameters, integer tensors, small tensors and
-  what an op marks as exact stay as they are. A saved ReLU output below half its group's
+  when its backward pass asks for it. Parameters, integer tensors and small tensors stay
+  as they are. A saved ReLU output below half its group's
   scale reads back as zero and passes no gradient.
 * ``gated_scan`` and ``norm_residual`` take ``checkpoint="int8"``: their own kernels write
   the codes while they read the inputs and read the codes in the backward pass, with no
@@ -94,22 +94,16 @@ def quantize8(x: torch.Tensor) -> Packed8:
     return Packed8(codes, scales, x.shape, x.dtype)
 
 
-def exact(t: torch.Tensor | None) -> torch.Tensor | None:
-    """Marks a tensor that an op saves for its backward pass as not to be kept in 8 bits."""
-    if t is not None:
-        t._su_exact = True
-    return t
-
-
 @contextmanager
 def saved8(min_numel: int = 1 << 16):
     """Keep the activations that autograd saves inside the block in 8 bits: float32 and
     bfloat16 tensors of at least two dimensions and `min_numel` values that are neither
-    parameters (leaves that require a gradient) nor marked by ``exact``."""
+    parameters (leaves that require a gradient). The recurrence's kept states and the scales of
+    codes stay exact."""
 
     def pack(t: torch.Tensor):
         if (t.dtype not in (torch.float32, torch.bfloat16) or t.dim() < 2 or t.numel() < max(1, min_numel)
-                or (t.is_leaf and t.requires_grad) or getattr(t, "_su_exact", False)):
+                or (t.is_leaf and t.requires_grad)):
             return t
         return quantize8(t)
 

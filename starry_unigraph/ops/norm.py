@@ -15,36 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from starry_unigraph.ops import cuda_ext
-from starry_unigraph.ops.checkpoint8 import check_checkpoint, exact, quantize8
-
-
-def _rows(t: torch.Tensor | None, width: int) -> torch.Tensor | None:
-    if t is None:
-        return None
-    t = t.reshape(-1, width)
-    return t if t.stride(1) == 1 or width == 1 else t.contiguous()
-
-
-class _NormResidual(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, u, gate, w_post, w_pre, scale, eps, keep8):
-        y, n, codes, scales = cuda_ext().norm_residual_fwd(x, u, gate, w_post, w_pre, scale, eps, keep8)
-        if keep8:
-            ctx.save_for_backward(exact(codes), None, None, exact(scales), w_post, w_pre, scale)
-        else:
-            ctx.save_for_backward(x, u, gate, None, w_post, w_pre, scale)
-        ctx.meta = (eps, x.dtype == torch.bfloat16)
-        ctx.set_materialize_grads(False)
-        return y, n
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dn):
-        x, u, gate, scales, w_post, w_pre, scale = ctx.saved_tensors
-        eps, bf16 = ctx.meta
-        dy, dn = (g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (dy, dn))
-        grads = cuda_ext().norm_residual_bwd(x, u, gate, scales, w_post, w_pre, scale, eps, dy, dn, bf16)
-        return (*grads, None, None)
+from starry_unigraph.ops.checkpoint8 import check_checkpoint, quantize8
 
 
 def _norm_torch(x, u, gate, w_post, w_pre, scale, eps):
@@ -115,6 +86,8 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, *, eps: float = 1e-6, checkpoint:
 
 def _call(x, u, gate, w_post, w_pre, scale, eps, checkpoint):
     keep8 = check_checkpoint(checkpoint)
+    if x.is_cuda:
+        return cuda_ext().norm_residual(x, u, gate, w_post, w_pre, scale, eps, keep8)
     H = x.size(-1) if x.dim() else 0
     if H == 0:
         raise ValueError("norm_residual: x needs a last dimension of at least one value")
@@ -128,15 +101,6 @@ def _call(x, u, gate, w_post, w_pre, scale, eps, checkpoint):
         if t is not None and tuple(t.shape) != (H,):
             raise ValueError(f"norm_residual: {name} must have shape ({H},), got {tuple(t.shape)}")
     args = (x, u, gate, w_post, w_pre, scale)
-    track = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args)
-    if not x.is_cuda:
-        if keep8 and track:
-            return _NormCodes.apply(*args, eps)
-        return _norm_torch(*args, eps)
-    rows = [_rows(t, H) for t in (x, u, gate)]
-    vecs = [None if t is None else t.contiguous() for t in (w_post, w_pre, scale)]
-    if track:
-        y, n = _NormResidual.apply(*rows, *vecs, float(eps), keep8)
-    else:
-        y, n, _, _ = cuda_ext().norm_residual_fwd(*rows, *vecs, float(eps), False)
-    return (None if y is None else y.view(x.shape)), (None if n is None else n.view(x.shape))
+    if keep8 and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        return _NormCodes.apply(*args, eps)
+    return _norm_torch(*args, eps)

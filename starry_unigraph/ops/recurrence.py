@@ -24,34 +24,9 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from starry_unigraph.ops import cuda_ext
-from starry_unigraph.ops.checkpoint8 import _dequantize_torch, _quantize_torch, check_checkpoint, exact
+from starry_unigraph.ops.checkpoint8 import _dequantize_torch, _quantize_torch, check_checkpoint
 
 STATE_EVERY = 16  # checkpoint="int8": steps between the fp32 states kept for the backward pass
-
-
-class _GatedScan(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, p, decay, h0, mask, offsets, rate, time_major, keep8):
-        h, last, states, codes, scales, marks = cuda_ext().gated_scan_fwd(p, decay, h0, mask, offsets, rate, time_major,
-                                                                          True, keep8)
-        ctx.save_for_backward(exact(codes) if keep8 else p, exact(scales), exact(states), decay,
-                              None if h0 is None else exact(h0.detach()), mask, offsets, marks)
-        ctx.meta = (rate, time_major, p.dtype == torch.bfloat16)
-        ctx.set_materialize_grads(False)
-        return h, last
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dh, dlast):
-        like, scales, states, decay, h0, mask, offsets, marks = ctx.saved_tensors
-        rate, time_major, bf16 = ctx.meta
-        if dh is not None and dh.stride(-1) != 1:
-            dh = dh.contiguous()
-        if dlast is not None:
-            dlast = dlast.contiguous()
-        dp, ddecay, dh0 = cuda_ext().gated_scan_bwd(like, scales, states, decay, h0, mask, offsets, marks, dh, dlast,
-                                                    rate, time_major, bf16, ctx.needs_input_grad[2])
-        return dp, ddecay, dh0, None, None, None, None, None
 
 
 def _scan_torch(p, decay, h0, mask, offsets, rate):
@@ -161,6 +136,8 @@ def gated_scan(p: torch.Tensor, decay: torch.Tensor, h0: torch.Tensor | None = N
     values of the codes, the states between fp32 ones that are kept every 16 steps (packed: rows of
     the packed axis) recomputed from them."""
     keep8 = check_checkpoint(checkpoint)
+    if p.is_cuda:
+        return cuda_ext().gated_scan(p, decay, h0, mask, offsets, rate, keep8)
     if p.dim() != (3 if offsets is None else 2) or p.size(-1) == 0 or p.size(-1) % 3:
         raise ValueError("gated_scan: p must be [batch, steps, 3H], or [rows, 3H] with offsets")
     if not rate > 0:
@@ -173,19 +150,9 @@ def gated_scan(p: torch.Tensor, decay: torch.Tensor, h0: torch.Tensor | None = N
         raise ValueError(f"gated_scan: h0 must have shape ({batch}, {H}), got {tuple(h0.shape)}")
     if mask is not None and (mask.dtype != torch.bool or mask.shape != p.shape[:-1]):
         raise ValueError(f"gated_scan: mask must be bool of shape {tuple(p.shape[:-1])}")
-    if not p.is_cuda:
-        if keep8:
-            return _ThroughCodes.apply(p, decay, h0, mask, offsets, float(rate))
-        return _scan_torch(p, decay, h0, mask, offsets, float(rate))
-    if p.stride(-1) != 1:
-        p = p.contiguous()
-    decay = decay.contiguous()
-    if h0 is not None:
-        h0 = h0.float().contiguous()
-    time_major = offsets is None and p.stride(1) > p.stride(0)
-    if torch.is_grad_enabled() and (p.requires_grad or decay.requires_grad or (h0 is not None and h0.requires_grad)):
-        return _GatedScan.apply(p, decay, h0, mask, offsets, float(rate), time_major, keep8)
-    return tuple(cuda_ext().gated_scan_fwd(p, decay, h0, mask, offsets, float(rate), time_major, False, False)[:2])
+    if keep8:
+        return _ThroughCodes.apply(p, decay, h0, mask, offsets, float(rate))
+    return _scan_torch(p, decay, h0, mask, offsets, float(rate))
 
 
 def gated_scan_step(p: torch.Tensor, decay: torch.Tensor, state: torch.Tensor, rows: torch.Tensor | None = None, *,
@@ -197,8 +164,7 @@ def gated_scan_step(p: torch.Tensor, decay: torch.Tensor, state: torch.Tensor, r
     ``check_status()``; its row of h is zero and nothing is written. No gradient flows
     through a step."""
     if p.is_cuda:
-        with torch.no_grad():
-            return cuda_ext().gated_scan_step(p if p.stride(-1) == 1 else p.contiguous(), decay, state, rows, rate)
+        return cuda_ext().gated_scan_step(p, decay, state, rows, rate)
     if p.dim() != 2 or p.size(1) == 0 or p.size(1) % 3:
         raise ValueError("gated_scan_step: p must be [rows, 3H]")
     if not rate > 0:
