@@ -13,41 +13,83 @@ struct Unit {
   int steps, tc;        // of the segment; the chunk's first step inside it
 };
 
-// A chunk's x, r, i and dh on their way to registers. In flight they are copies into slots of
-// shared memory that belong to the thread, so the next chunk's loads are under way while
-// this one is worked on and no barrier is needed.
-template <class T, int V, int CH>
+// A chunk's x, r, i (or their codes and scales), dh and marks on their way to registers. In
+// flight they are copies into slots of shared memory that belong to the thread, so the
+// next chunk's loads are under way while this one is worked on and no barrier is needed.
+template <class T, int V, int CH, bool CODES, bool MARKS>
 struct Slots {
-  static constexpr int kBytes = sizeof(T) * V;
-  using Raw = typename RawOf<kBytes>::type;
-  Raw* at;  // [2][CH][4][threads], at this thread's place
-  int ld;   // threads
+  using Raw = typename RawOf<sizeof(T) * V>::type;
+  static constexpr int kRows = CODES ? 1 : 4;                      // of Raw: dh, and without codes x, r, i
+  static constexpr int kWords = (CODES ? 6 : 0) + (MARKS ? 1 : 0);  // codes, scales, marks
+  static constexpr int kBytes = 2 * CH * (kRows * static_cast<int>(sizeof(Raw)) + kWords * 4);  // of a thread
+  Raw* rows;        // [2][CH][kRows][threads], at this thread's place
+  uint32_t* words;  // [2][CH][kWords][threads]
+  int ld;           // threads
 
-  __device__ __forceinline__ Raw* slot(int buf, int j, int w) const { return at + ((buf * CH + j) * 4 + w) * ld; }
+  __device__ __forceinline__ void init(void* smem) {
+    ld = blockDim.x;
+    rows = static_cast<Raw*>(smem) + threadIdx.x;
+    words = reinterpret_cast<uint32_t*>(static_cast<Raw*>(smem) + 2 * CH * kRows * ld) + threadIdx.x;
+  }
+  __device__ __forceinline__ Raw* row(int buf, int j, int w) const { return rows + ((buf * CH + j) * kRows + w) * ld; }
+  __device__ __forceinline__ uint32_t* word(int buf, int j, int w) const {
+    return words + ((buf * CH + j) * kWords + w) * ld;
+  }
   __device__ __forceinline__ void fetch(const ScanArgs& A, const Unit& u, int c, int buf) const {
+    const int64_t H = A.width, G = (A.width + kGroup8 - 1) / kGroup8;
     const int64_t t0 = u.begin + u.tc;
-    const T* in = static_cast<const T*>(A.p) + u.b * A.p_sb + t0 * A.p_st + c;
+    const int64_t at = u.b * A.row_sb + t0 * A.row_st;
+    const T* in = CODES ? nullptr : static_cast<const T*>(A.p) + u.b * A.p_sb + t0 * A.p_st + c;
+    // the aligned word that holds this lane's codes (rows of codes are multiples of 4)
+    const int8_t* code = CODES ? A.codes + at * 3 * H + (c & ~3) : nullptr;
+    const float* scale = CODES ? A.scales + at * 3 * G + c / kGroup8 : nullptr;
     const T* dh = static_cast<const T*>(A.dh) + (A.dh != nullptr ? u.b * A.dh_sb + t0 * A.dh_st + c : 0);
 #pragma unroll
     for (int j = 0; j < CH; ++j) {
       if (u.tc + j < u.steps) {
-        copy_async<kBytes>(slot(buf, j, 0), in);
-        copy_async<kBytes>(slot(buf, j, 1), in + A.width);
-        copy_async<kBytes>(slot(buf, j, 2), in + 2 * static_cast<int64_t>(A.width));
-        if (A.dh != nullptr) copy_async<kBytes>(slot(buf, j, 3), dh);
+        if constexpr (CODES) {
+#pragma unroll
+          for (int w = 0; w < 3; ++w) {
+            copy_async<4>(word(buf, j, w), code + w * H);
+            copy_async<4>(word(buf, j, 3 + w), scale + w * G);
+          }
+        } else {
+#pragma unroll
+          for (int w = 0; w < 3; ++w) copy_async<sizeof(Raw)>(row(buf, j, 1 + w), in + w * H);
+        }
+        if (A.dh != nullptr) copy_async<sizeof(Raw)>(row(buf, j, 0), dh);
+        if constexpr (MARKS) copy_async<4>(word(buf, j, kWords - 1), A.marks + t0 + j);
       }
-      in += A.p_st;
+      if (CODES) {
+        code += A.row_st * 3 * H;
+        scale += A.row_st * 3 * G;
+      } else {
+        in += A.p_st;
+      }
       dh += A.dh_st;
     }
   }
-  __device__ __forceinline__ void get(int buf, int j, int w, float (&f)[V]) const {
+  __device__ __forceinline__ void get(int buf, int j, int w, int c, float (&f)[V]) const {
+    if constexpr (CODES) {
+      Codes<V> q;
+      q.raw = static_cast<typename RawOf<V>::type>(*word(buf, j, w) >> (V == 4 ? 0 : 8 * (c & 3)));
+      q.get(__uint_as_float(*word(buf, j, 3 + w)), f);
+    } else {
+      Pack<T, V> p;
+      p.raw = *row(buf, j, 1 + w);
+      p.get(f);
+    }
+  }
+  __device__ __forceinline__ void get_dh(int buf, int j, float (&f)[V]) const {
     Pack<T, V> p;
-    p.raw = *slot(buf, j, w);
+    p.raw = *row(buf, j, 0);
     p.get(f);
   }
+  __device__ __forceinline__ int mark(int buf, int j) const { return static_cast<int>(*word(buf, j, kWords - 1)); }
 };
 
-// The same values in registers: narrow rows (single bf16 values) and 8-bit codes.
+// The same values in registers, where a lane's are less than the 4 bytes that a copy has: single
+// bf16 values, and single codes (whose 16 steps of words would take too much shared memory).
 template <class T, int V, int CH, bool CODES>
 struct Held {
   Pack<T, V> v[CODES ? 1 : CH][3], d[CH];
@@ -104,7 +146,7 @@ struct Held {
 constexpr int kBwdThreads = 128;
 template <class T, int V, int CH, bool CODES, int KIND>
 __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {
-  constexpr bool kAsync = !CODES && sizeof(T) * V >= 4;
+  constexpr bool kAsync = CODES ? V > 1 : sizeof(T) * V >= 4;
   extern __shared__ uint4 smem[];
   const int y = threadIdx.x / L.count;
   const int lane_c = threadIdx.x % L.count;
@@ -135,10 +177,9 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
   int64_t rr = static_cast<int64_t>(blockIdx.x) * L.rows + y;
   Unit u;
   bool more = place(rr, u);
-  Slots<T, V, CH> slots;
+  Slots<T, V, CH, CODES, KIND == kPacked> slots;
   if constexpr (kAsync) {
-    slots.at = reinterpret_cast<typename Slots<T, V, CH>::Raw*>(smem) + threadIdx.x;
-    slots.ld = blockDim.x;
+    slots.init(smem);
     if (more) slots.fetch(A, u, c, 0);
     commit_copies();
   }
@@ -172,6 +213,11 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
                                : (KIND != kPacked && A.h0 != nullptr ? A.h0 + u.b * H + c : nullptr);
 #pragma unroll
     for (int v = 0; v < V; ++v) h[v] = from != nullptr ? from[v] : 0.f;
+    if constexpr (kAsync) {
+      if (more_next) slots.fetch(A, next, c, buf ^ 1);
+      commit_copies();
+      wait_copies<1>();
+    }
     unsigned on = 0, firsts = 0, lasts = 0;
     if (KIND == kPlain) {
       const int n = u.steps - u.tc;
@@ -182,8 +228,12 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
       for (int j = 0; j < CH; ++j) {
         if (u.tc + j >= u.steps) continue;
         if (valid == nullptr || valid[j * A.m_st] != 0) on |= 1u << j;
-        if (KIND == kPacked) {
-          const int mk = A.marks[t0 + j];
+        if constexpr (KIND == kPacked) {
+          int mk;
+          if constexpr (kAsync)
+            mk = slots.mark(buf, j);
+          else
+            mk = A.marks[t0 + j];
           if (mk >= 0) {
             firsts |= static_cast<unsigned>(mk & kMarkFirst) << j;
             lasts |= static_cast<unsigned>((mk & kMarkLast) >> 1) << j;
@@ -192,13 +242,7 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
       }
     }
     Held<T, V, CH, CODES> held;
-    if constexpr (kAsync) {
-      if (more_next) slots.fetch(A, next, c, buf ^ 1);
-      commit_copies();
-      wait_copies<1>();
-    } else {
-      held.fetch(A, u, c, on);
-    }
+    if constexpr (!kAsync) held.fetch(A, u, c, on);
     // WHOLE: every step of the chunk is inside the sequence and counts
     auto work = [&](auto whole) {
       constexpr bool WHOLE = decltype(whole)::value;
@@ -212,9 +256,9 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
         }
         float fx[V], fr[V], fi[V];
         if constexpr (kAsync) {
-          slots.get(buf, j, 0, fx);
-          slots.get(buf, j, 1, fr);
-          slots.get(buf, j, 2, fi);
+          slots.get(buf, j, 0, c, fx);
+          slots.get(buf, j, 1, c, fr);
+          slots.get(buf, j, 2, c, fi);
         } else {
           held.get(j, 0, fx);
           held.get(j, 1, fr);
@@ -241,7 +285,7 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
         }
         float dy[V], dx[V], dr[V], di[V];
         if constexpr (kAsync) {
-          slots.get(buf, j, 3, dy);
+          slots.get_dh(buf, j, dy);
           if (A.dh == nullptr) {
 #pragma unroll
             for (int v = 0; v < V; ++v) dy[v] = 0.f;
@@ -419,8 +463,8 @@ void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
   const Lanes l = bwd_lanes(a);
   const dim3 grid(scan_bwd_blocks(a, p, sms), l.blocks);
   const int threads = l.count * l.rows;
-  const bool async = !CODES && sizeof(T) * V >= 4;
-  const size_t smem = async ? static_cast<size_t>(threads) * 2 * CH * 4 * sizeof(T) * V : 0;
+  const bool async = CODES ? V > 1 : sizeof(T) * V >= 4;
+  const size_t smem = async ? static_cast<size_t>(threads) * Slots<T, V, CH, CODES, KIND == kPacked>::kBytes : 0;
   auto kernel = scan_bwd_kernel<T, V, CH, CODES, KIND>;
   if (smem > 40 * 1024)
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));

@@ -5,34 +5,24 @@
 namespace su {
 namespace {
 
-template <class T, int V>
-struct Inputs {
-  Pack<T, V> x, r, i;
-  __device__ __forceinline__ void zero() {
-    x.zero();
-    r.zero();
-    i.zero();
-  }
-  template <bool KEEP>
-  __device__ __forceinline__ void load(const T* p, int H) {
-    if (KEEP) {
-      x.load_keep(p);
-      r.load_keep(p + H);
-      i.load_keep(p + 2 * H);
-    } else {
-      x.load(p);
-      r.load(p + H);
-      i.load(p + 2 * H);
-    }
-  }
+// U steps of one segment: a unit of work.
+struct Unit {
+  int64_t q, b, begin;  // segment, sequence, the segment's first step
+  int steps, t;         // of the segment; the unit's first step inside it
 };
 
 // MAPS: composes the segment's steps into h -> A h + B and writes nothing else. Otherwise
 // walks the states from the one before the segment.
-// Steps are taken U at a time: their inputs are loaded together, U x 3 loads of V values
-// under way per thread.
+//
+// While a unit is worked on, the inputs of the next one (of the next segment behind the last)
+// are copied into slots of shared memory that belong to the thread, so loads are always
+// under way, no barrier is needed and the registers hold one step's inputs. Single bf16
+// values, below the 4 bytes that such a copy has, are loaded when they are needed.
 template <class T, int V, int U, bool MAPS, bool CODES, int KIND>
-__global__ void __launch_bounds__(256, 3) scan_fwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {
+__global__ void __launch_bounds__(256, CODES ? 3 : 4) scan_fwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {
+  constexpr bool kAsync = sizeof(T) * V >= 4;
+  using Raw = typename Pack<T, V>::Raw;
+  extern __shared__ uint4 smem[];
   const int y = threadIdx.x / L.count;
   const int c = (blockIdx.y * L.count + threadIdx.x % L.count) * V;
   const bool live = c < A.width;
@@ -41,139 +31,216 @@ __global__ void __launch_bounds__(256, 3) scan_fwd_kernel(const ScanArgs A, cons
   const int G = (H + kGroup8 - 1) / kGroup8;
   const int64_t batch = KIND == kPacked ? 1 : A.batch;
   const int64_t rows = batch * P.seg.n;
-  float k[V];
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * L.rows;
+  const bool masked = KIND == kMasked || (KIND == kPacked && A.mask != nullptr);
+  float k[V], h[V], m[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) k[v] = live ? decay_factor(param_at(A.decay, A.decay_bf16, c + v), A.rate) : 0.f;
-  for (int64_t rr = static_cast<int64_t>(blockIdx.x) * L.rows + y; rr < rows;
-       rr += static_cast<int64_t>(gridDim.x) * L.rows) {
+  for (int v = 0; v < V; ++v) {
+    k[v] = live ? decay_factor(param_at(A.decay, A.decay_bf16, c + v), A.rate) : 0.f;
+    h[v] = m[v] = 0.f;
+  }
+  auto place = [&](int64_t rr, Unit& u) {
+    if (rr >= rows) return false;
     // after the maps were made first to last, the last segments are the ones still in L2
     const SegRow s = seg_row(rr, batch, P.seg, !MAPS && P.seg.n > 1);
-    const int64_t begin = s.q * P.seg.len;
-    const int steps = static_cast<int>(min(P.seg.len, A.steps - begin));
-    const int64_t row = s.b * A.row_sb + begin * A.row_st;
-    const int64_t at = (s.q * batch + s.b) * H + c;
-    const T* in = static_cast<const T*>(A.p) + s.b * A.p_sb + begin * A.p_st + c;
-    const uint8_t* valid = A.mask != nullptr ? A.mask + s.b * A.m_sb + begin * A.m_st : nullptr;
-    const int* mark = KIND == kPacked ? A.marks + begin : nullptr;
-    T* out = MAPS ? nullptr : static_cast<T*>(A.h) + row * H + c;
-    int8_t* code = CODES ? A.codes + row * 3 * H + c : nullptr;
-    float* scale = CODES ? A.scales + row * 3 * G + c / kGroup8 : nullptr;
-    float h[V], m[V];
+    u.q = s.q;
+    u.b = s.b;
+    u.begin = s.q * P.seg.len;
+    u.steps = static_cast<int>(min(P.seg.len, A.steps - u.begin));
+    u.t = 0;
+    return true;
+  };
+  Raw* const slots = reinterpret_cast<Raw*>(smem) + threadIdx.x;
+  const int ld = blockDim.x;
+  auto slot = [&](int buf, int j, int w) { return slots + ((buf * U + j) * 3 + w) * ld; };
+  auto input = [&](const Unit& u, int j) {
+    return static_cast<const T*>(A.p) + u.b * A.p_sb + (u.begin + u.t + j) * A.p_st + c;
+  };
+  auto fetch = [&](const Unit& u, int buf) {
+    if constexpr (kAsync) {
+      const T* in = input(u, 0);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      m[v] = 1.f;
-      h[v] = 0.f;
-      if (!MAPS && live) {
-        if (P.seg.n > 1)
-          h[v] = P.carry[at + v];
-        else if (KIND != kPacked && A.h0 != nullptr)
-          h[v] = A.h0[s.b * H + c + v];
+      for (int j = 0; j < U; ++j, in += A.p_st) {
+        if (u.t + j < u.steps && live) {
+          copy_async<sizeof(Raw)>(slot(buf, j, 0), in);
+          copy_async<sizeof(Raw)>(slot(buf, j, 1), in + H);
+          copy_async<sizeof(Raw)>(slot(buf, j, 2), in + 2 * static_cast<int64_t>(H));
+        }
       }
     }
-    for (int t0 = 0; t0 < steps; t0 += U) {
-      Inputs<T, V> w[U];
-      int mk[U];
-      bool on[U];
+  };
+  // marks and mask of a unit, a unit ahead of their use
+  auto peek = [&](const Unit& u, int (&mk)[U], bool (&on)[U]) {
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const bool inside = t0 + j < steps;
-        on[j] = inside && live;
-        if (KIND == kMasked || (KIND == kPacked && valid != nullptr)) {
-          if (inside) on[j] = on[j] && *valid != 0;
-          valid += A.m_st;
-        }
-        mk[j] = -1;
-        if (KIND == kPacked) {
-          if (inside) mk[j] = mark[j];
-        }
-        w[j].zero();
-        if (on[j]) w[j].template load<MAPS>(in, H);
-        in += A.p_st;
+    for (int j = 0; j < U; ++j) {
+      const bool inside = u.t + j < u.steps;
+      mk[j] = -1;
+      on[j] = inside;
+      if (KIND == kPacked && inside) mk[j] = A.marks[u.begin + u.t + j];
+      if (masked && inside) on[j] = A.mask[u.b * A.m_sb + (u.begin + u.t + j) * A.m_st] != 0;
+    }
+  };
+  int64_t rr = static_cast<int64_t>(blockIdx.x) * L.rows + y;
+  Unit u;
+  bool more = place(rr, u);
+  int mk[U];
+  bool on[U];
+  if (more) {
+    fetch(u, 0);
+    peek(u, mk, on);
+  }
+  commit_copies();
+  T* out = nullptr;
+  int8_t* code = nullptr;
+  float* scale = nullptr;
+  int buf = 0;
+  while (more) {
+    Unit next = u;
+    bool more_next = true;
+    if (u.t + U < u.steps) {
+      next.t += U;
+    } else {
+      rr += stride;
+      more_next = place(rr, next);
+    }
+    int mk_next[U];
+    bool on_next[U];
+    if (more_next) {
+      fetch(next, buf ^ 1);
+      peek(next, mk_next, on_next);
+    }
+    commit_copies();
+    const int64_t at = (u.q * batch + u.b) * H + c;
+    if (u.t == 0) {
+      const int64_t row = u.b * A.row_sb + u.begin * A.row_st;
+      out = MAPS ? nullptr : static_cast<T*>(A.h) + row * H + c;
+      if (CODES) {
+        code = A.codes + row * 3 * H + c;
+        scale = A.scales + row * 3 * G + c / kGroup8;
       }
-      if (KIND == kPacked) mark += U;
-      if (!MAPS && A.states != nullptr && live && begin + t0 > 0 && t0 % A.state_every == 0) {  // U divides it
-        float* to = A.states + (s.b * A.n_states + (begin + t0) / A.state_every - 1) * H + c;
 #pragma unroll
-        for (int v = 0; v < V; ++v) to[v] = h[v];
+      for (int v = 0; v < V; ++v) {
+        m[v] = 1.f;
+        h[v] = 0.f;
+        if (!MAPS && live) {
+          if (P.seg.n > 1)
+            h[v] = P.carry[at + v];
+          else if (KIND != kPacked && A.h0 != nullptr)
+            h[v] = A.h0[u.b * H + c + v];
+        }
       }
+    }
+    if (!MAPS && A.states != nullptr && live && u.begin + u.t > 0 && u.t % A.state_every == 0 && u.steps > 0) {
+      // U divides state_every
+      float* to = A.states + (u.b * A.n_states + (u.begin + u.t) / A.state_every - 1) * H + c;
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        if (t0 + j >= steps) break;
-        float fx[V], fr[V], fi[V];
-        w[j].x.get(fx);
-        w[j].r.get(fr);
-        w[j].i.get(fi);
-        if constexpr (CODES) {
-          Codes<V> q[3];
-          const float s0 = encode8(fx, q[0]), s1 = encode8(fr, q[1]), s2 = encode8(fi, q[2]);
-          if (live) {
-            q[0].store(code);
-            q[1].store(code + H);
-            q[2].store(code + 2 * H);
-            if (c % kGroup8 == 0) {
-              scale[0] = s0;
-              scale[G] = s1;
-              scale[2 * G] = s2;
-            }
+      for (int v = 0; v < V; ++v) to[v] = h[v];
+    }
+    wait_copies<1>();
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (u.t + j >= u.steps) break;
+      Pack<T, V> w[3];
+#pragma unroll
+      for (int s = 0; s < 3; ++s) {
+        w[s].zero();
+        if (live && (KIND == kPlain || on[j])) {
+          if constexpr (kAsync)
+            w[s].raw = *slot(buf, j, s);
+          else
+            w[s].load(input(u, j) + s * static_cast<int64_t>(H));
+        }
+      }
+      float fx[V], fr[V], fi[V];
+      w[0].get(fx);
+      w[1].get(fr);
+      w[2].get(fi);
+      if constexpr (CODES) {
+        Codes<V> q[3];
+        const float s0 = encode8(fx, q[0]), s1 = encode8(fr, q[1]), s2 = encode8(fi, q[2]);
+        if (live) {
+          q[0].store(code);
+          q[1].store(code + H);
+          q[2].store(code + 2 * static_cast<int64_t>(H));
+          if (c % kGroup8 == 0) {
+            scale[0] = s0;
+            scale[G] = s1;
+            scale[2 * static_cast<int64_t>(G)] = s2;
           }
-          code += A.row_st * 3 * H;
-          scale += A.row_st * 3 * G;
         }
-        if (KIND == kPacked && mk[j] >= 0 && (mk[j] & kMarkFirst) && live) {
-          const float* from = A.h0 != nullptr ? A.h0 + static_cast<int64_t>(mk[j] >> 2) * H + c : nullptr;
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            h[v] = from != nullptr ? from[v] : 0.f;
-            m[v] = 0.f;
-          }
-        }
-        if (KIND != kPlain && !on[j]) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) shut(fx[v], fr[v], fi[v]);
-        }
-        Step g[V];
-        steps_of(fx, fr, fi, k, g);
+        code += A.row_st * 3 * H;
+        scale += A.row_st * 3 * G;
+      }
+      if (KIND == kPacked && mk[j] >= 0 && (mk[j] & kMarkFirst) && live) {
+        const float* from = A.h0 != nullptr ? A.h0 + static_cast<int64_t>(mk[j] >> 2) * H + c : nullptr;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          h[v] = fmaf(g[v].a, h[v], g[v].add);
-          if (MAPS) m[v] *= g[v].a;
+          h[v] = from != nullptr ? from[v] : 0.f;
+          m[v] = 0.f;
         }
-        if (!MAPS) {
-          if (live) {
-            Pack<T, V> o;
-            o.set(h);
-            o.store(out);
-          }
-          out += A.row_st * H;
-          if (KIND == kPacked && mk[j] >= 0 && (mk[j] & kMarkLast) && live) {
-            float* to = A.last + static_cast<int64_t>(mk[j] >> 2) * H + c;
+      }
+      if (KIND != kPlain && !on[j]) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) to[v] = h[v];
-          }
+        for (int v = 0; v < V; ++v) shut(fx[v], fr[v], fi[v]);
+      }
+      Step g[V];
+      steps_of(fx, fr, fi, k, g);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        h[v] = fmaf(g[v].a, h[v], g[v].add);
+        if (MAPS) m[v] *= g[v].a;
+      }
+      if (!MAPS) {
+        if (live) {
+          Pack<T, V> o;
+          o.set(h);
+          o.store(out);
+        }
+        out += A.row_st * H;
+        if (KIND == kPacked && mk[j] >= 0 && (mk[j] & kMarkLast) && live) {
+          float* to = A.last + static_cast<int64_t>(mk[j] >> 2) * H + c;
+#pragma unroll
+          for (int v = 0; v < V; ++v) to[v] = h[v];
         }
       }
     }
-    if (!live) continue;
-    if (MAPS) {
+    if (u.t + U >= u.steps && live) {
+      if (MAPS) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) P.maps[at + v] = make_float2(m[v], h[v]);
-    } else if (KIND != kPacked && s.q == P.seg.n - 1) {
+        for (int v = 0; v < V; ++v) P.maps[at + v] = make_float2(m[v], h[v]);
+      } else if (KIND != kPacked && u.q == P.seg.n - 1) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) A.last[s.b * H + c + v] = h[v];
+        for (int v = 0; v < V; ++v) A.last[u.b * H + c + v] = h[v];
+      }
+    }
+    u = next;
+    more = more_next;
+    buf ^= 1;
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      mk[j] = mk_next[j];
+      on[j] = on_next[j];
     }
   }
 }
 
-template <class T, bool MAPS, bool CODES, int KIND>
+template <class T, int V, int U, bool MAPS, bool CODES, int KIND>
 void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
-  const Lanes l = lanes_of(a.width, a.vec ? 4 : 1, CODES, 256);
+  const Lanes l = lanes_of(a.width, V, CODES, 256);
   const int64_t rows = (a.offsets != nullptr ? 1 : a.batch) * p.seg.n;
   const dim3 grid(row_blocks(rows, l, sms), l.blocks);
   const int threads = l.count * l.rows;
-  if (a.vec)
-    scan_fwd_kernel<T, 4, 4, MAPS, CODES, KIND><<<grid, threads, 0, st>>>(a, p, l);
-  else
-    scan_fwd_kernel<T, 1, 8, MAPS, CODES, KIND><<<grid, threads, 0, st>>>(a, p, l);
+  const size_t smem = sizeof(T) * V >= 4 ? static_cast<size_t>(threads) * 2 * U * 3 * sizeof(T) * V : 0;
+  auto kernel = scan_fwd_kernel<T, V, U, MAPS, CODES, KIND>;
+  if (smem > 40 * 1024)
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  kernel<<<grid, threads, smem, st>>>(a, p, l);
+}
+
+// 192 bytes of slots a thread with 4 channels, four blocks an SM
+template <class T, bool MAPS, bool CODES, int KIND>
+void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
+  a.vec ? run<T, 4, 8 / static_cast<int>(sizeof(T)), MAPS, CODES, KIND>(a, p, sms, st) : run<T, 1, 4, MAPS, CODES, KIND>(a, p, sms, st);
 }
 
 template <class T, bool MAPS, bool CODES>

@@ -16,26 +16,42 @@
 namespace su {
 namespace {
 
-// Marks of the packed sequences' first and last rows; reports offsets that do not rise from
-// 0 to `rows`. `marks` holds -1 before.
-__global__ void scan_marks_kernel(const int64_t* __restrict__ offsets, int64_t batch, int64_t rows, int* marks,
-                                  int* status) {
-  for (int64_t s = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; s < batch;
-       s += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+// A warp per packed sequence: marks its first and last rows (marks != nullptr, -1 before), reports
+// offsets that do not rise from 0 to `rows`, and copies what an empty sequence returns, its
+// first state or the gradient of its last (`from`, nullptr: zeros).
+__global__ void __launch_bounds__(256) scan_sequences_kernel(const int64_t* __restrict__ offsets, int64_t batch,
+                                                             int64_t rows, int H, int* marks,
+                                                             const float* __restrict__ from, float* __restrict__ to,
+                                                             int* status) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t s = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32; s < batch;
+       s += static_cast<int64_t>(gridDim.x) * 8) {
     const int64_t lo = offsets[s], hi = offsets[s + 1];
     if (lo < 0 || hi < lo || hi > rows || (s == 0 && lo != 0) || (s == batch - 1 && hi != rows)) {
-      record_status(status, kBadIndex);
+      if (lane == 0) record_status(status, kBadIndex);
       continue;
     }
-    if (hi == lo) continue;
-    const int id = static_cast<int>(s) * 4;
-    if (hi - lo == 1) {
-      marks[lo] = id + kMarkFirst + kMarkLast;
-    } else {
-      marks[lo] = id + kMarkFirst;
-      marks[hi - 1] = id + kMarkLast;
+    if (hi == lo) {
+      if (to != nullptr)
+        for (int c = lane; c < H; c += 32) to[s * H + c] = from != nullptr ? from[s * H + c] : 0.f;
+    } else if (marks != nullptr && lane == 0) {
+      const int id = static_cast<int>(s) * 4;
+      if (hi - lo == 1) {
+        marks[lo] = id + kMarkFirst + kMarkLast;
+      } else {
+        marks[lo] = id + kMarkFirst;
+        marks[hi - 1] = id + kMarkLast;
+      }
     }
   }
+}
+
+void launch_sequences(const ScanArgs& a, int* marks, const float* from, float* to, cudaStream_t st) {
+  if (marks == nullptr && to == nullptr) return;
+  count_launch();
+  const int64_t blocks = (a.batch + 7) / 8;
+  scan_sequences_kernel<<<static_cast<unsigned>(blocks < 8192 ? blocks : 8192), 256, 0, st>>>(
+      a.offsets, a.batch, a.steps, a.width, marks, from, to, a.status);
 }
 
 // carry[q] = the state before segment q (backwards: the gradient after it), from `start` through
@@ -141,27 +157,17 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanStepArgs A) {
 
 constexpr int64_t kSumRows = 64;  // above 8 times it the partial sums are added up in two launches
 
-// what an empty packed sequence returns: its first state, or the gradient of its last
-void fill_packed(const ScanArgs& a, float* to, const float* from, cudaStream_t st) {
-  if (to == nullptr) return;
-  const size_t bytes = static_cast<size_t>(a.batch) * a.width * sizeof(float);
-  if (from != nullptr)
-    cudaMemcpyAsync(to, from, bytes, cudaMemcpyDeviceToDevice, st);
-  else
-    cudaMemsetAsync(to, 0, bytes, st);
-}
-
 }  // namespace
 
-// Segments: as many as fill the SMs once with the forward kernels' 768 threads each (lanes of 4
-// channels where rows are aligned; the backward kernel takes that in four whole rounds), none
+// Segments: as many as fill the SMs once with the forward kernels' 1024 threads each (lanes of 4
+// channels where rows are aligned), none
 // shorter than 2 kStateEvery; at most 4096, whose states the carry kernel walks in a few
 // microseconds. Sequences that fill half of that by themselves are left whole: the second
 // read would cost more than the idle threads.
 ScanPlan scan_plan(const ScanArgs& a, int sms, void* workspace) {
   const int64_t batch = a.offsets != nullptr ? 1 : a.batch;
   const int64_t lanes = batch * ((a.width + (a.vec ? 3 : 0)) / (a.vec ? 4 : 1));
-  const int64_t want = static_cast<int64_t>(sms) * 768;
+  const int64_t want = static_cast<int64_t>(sms) * 1024;
   ScanPlan p;
   p.seg = {1, (a.steps + kStateEvery - 1) / kStateEvery * kStateEvery};
   if (lanes * 2 < want && a.steps > 4 * kStateEvery) {
@@ -191,12 +197,8 @@ int64_t scan_partials(const ScanArgs& a, int sms) {
 void launch_scan_fwd(const ScanArgs& a, int sms, void* workspace, cudaStream_t st) {
   const ScanPlan p = scan_plan(a, sms, workspace);
   if (a.offsets != nullptr) {
-    cudaMemsetAsync(a.marks, 0xff, static_cast<size_t>(a.steps) * sizeof(int), st);
-    count_launch();
-    const int64_t blocks = (a.batch + 255) / 256;
-    scan_marks_kernel<<<static_cast<unsigned>(blocks < 4096 ? blocks : 4096), 256, 0, st>>>(a.offsets, a.batch, a.steps,
-                                                                                           a.marks, a.status);
-    fill_packed(a, a.last, a.h0, st);
+    if (a.steps > 0) cudaMemsetAsync(a.marks, 0xff, static_cast<size_t>(a.steps) * sizeof(int), st);
+    launch_sequences(a, a.marks, a.h0, a.last, st);
   }
   if (a.steps == 0 && a.offsets != nullptr) return;
   if (p.seg.n > 1) {
@@ -208,7 +210,7 @@ void launch_scan_fwd(const ScanArgs& a, int sms, void* workspace, cudaStream_t s
 
 void launch_scan_bwd(const ScanArgs& a, int sms, void* workspace, void* ddecay, cudaStream_t st) {
   const ScanPlan p = scan_plan(a, sms, workspace);
-  if (a.offsets != nullptr) fill_packed(a, a.dh0, a.dlast, st);
+  if (a.offsets != nullptr) launch_sequences(a, nullptr, a.dlast, a.dh0, st);
   if (p.seg.n > 1) {
     scan_bwd_maps(a, p, sms, st);
     launch_carry(a, p, true, st);

@@ -59,7 +59,7 @@ inline ScanKind kind_of(const ScanArgs& a) {
 // blocks over `rows` rows of threads: every SM filled a few times, so that per-block sums stay few
 inline int row_blocks(int64_t rows, const Lanes& l, int sms) {
   const int64_t want = (rows + l.rows - 1) / l.rows;
-  const int64_t most = (static_cast<int64_t>(sms) * 12 + l.blocks - 1) / l.blocks;
+  const int64_t most = (static_cast<int64_t>(sms) * 16 + l.blocks - 1) / l.blocks;
   return static_cast<int>(want < most ? want : most);
 }
 
