@@ -14,13 +14,16 @@ struct Unit {
 // MAPS: composes the segment's steps into h -> A h + B and writes nothing else. Otherwise
 // walks the states from the one before the segment.
 //
-// While a unit is worked on, the inputs of the next one (of the next segment behind the last)
-// are copied into slots of shared memory that belong to the thread, so loads are always
-// under way, no barrier is needed and the registers hold one step's inputs. Single bf16
-// values, below the 4 bytes that such a copy has, are loaded when they are needed.
+// With 16 bytes a thread and input (four fp32 channels), while a unit is worked on the inputs of
+// the next one (of the next segment behind the last) are copied into slots of shared memory
+// that belong to the thread, so loads are always under way, no barrier is needed and the
+// registers hold one step's inputs. Where a thread has less, bf16 and odd widths, the copies'
+// instructions cost more than they hide (2 x 65,537 x 256 bf16: 73 us with, 68 without): the
+// unit's inputs are loaded together into registers.
 template <class T, int V, int U, bool MAPS, bool CODES, int KIND>
-__global__ void __launch_bounds__(256, CODES ? 3 : 4) scan_fwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {
-  constexpr bool kAsync = sizeof(T) * V >= 4;
+__global__ void __launch_bounds__(256, CODES || sizeof(T) * V < 16 ? 3 : 4)
+    scan_fwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {
+  constexpr bool kAsync = sizeof(T) * V >= 16;
   using Raw = typename Pack<T, V>::Raw;
   extern __shared__ uint4 smem[];
   const int y = threadIdx.x / L.count;
@@ -136,25 +139,38 @@ __global__ void __launch_bounds__(256, CODES ? 3 : 4) scan_fwd_kernel(const Scan
 #pragma unroll
       for (int v = 0; v < V; ++v) to[v] = h[v];
     }
-    wait_copies<1>();
+    if constexpr (kAsync) wait_copies<1>();
+    Pack<T, V> w[kAsync ? 1 : U][3];
+    if constexpr (!kAsync) {
+      const T* in = input(u, 0);
+#pragma unroll
+      for (int j = 0; j < U; ++j, in += A.p_st)
+#pragma unroll
+        for (int s = 0; s < 3; ++s) {
+          w[j][s].zero();
+          if (on[j] && live) {
+            if (MAPS)
+              w[j][s].load_keep(in + s * static_cast<int64_t>(H));
+            else
+              w[j][s].load(in + s * static_cast<int64_t>(H));
+          }
+        }
+    }
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       if (u.t + j >= u.steps) break;
-      Pack<T, V> w[3];
+      constexpr int kAt = kAsync ? 0 : 1;
+      if constexpr (kAsync) {
 #pragma unroll
-      for (int s = 0; s < 3; ++s) {
-        w[s].zero();
-        if (live && (KIND == kPlain || on[j])) {
-          if constexpr (kAsync)
-            w[s].raw = *slot(buf, j, s);
-          else
-            w[s].load(input(u, j) + s * static_cast<int64_t>(H));
+        for (int s = 0; s < 3; ++s) {
+          w[0][s].zero();
+          if (live && (KIND == kPlain || on[j])) w[0][s].raw = *slot(buf, j, s);
         }
       }
       float fx[V], fr[V], fi[V];
-      w[0].get(fx);
-      w[1].get(fr);
-      w[2].get(fi);
+      w[kAt * j][0].get(fx);
+      w[kAt * j][1].get(fr);
+      w[kAt * j][2].get(fi);
       if constexpr (CODES) {
         Codes<V> q[3];
         const float s0 = encode8(fx, q[0]), s1 = encode8(fr, q[1]), s2 = encode8(fi, q[2]);
@@ -230,17 +246,17 @@ void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
   const int64_t rows = (a.offsets != nullptr ? 1 : a.batch) * p.seg.n;
   const dim3 grid(row_blocks(rows, l, sms), l.blocks);
   const int threads = l.count * l.rows;
-  const size_t smem = sizeof(T) * V >= 4 ? static_cast<size_t>(threads) * 2 * U * 3 * sizeof(T) * V : 0;
+  const size_t smem = sizeof(T) * V >= 16 ? static_cast<size_t>(threads) * 2 * U * 3 * sizeof(T) * V : 0;
   auto kernel = scan_fwd_kernel<T, V, U, MAPS, CODES, KIND>;
   if (smem > 40 * 1024)
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   kernel<<<grid, threads, smem, st>>>(a, p, l);
 }
 
-// 192 bytes of slots a thread with 4 channels, four blocks an SM
+// fp32: 192 bytes of slots a thread, four blocks an SM
 template <class T, bool MAPS, bool CODES, int KIND>
 void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
-  a.vec ? run<T, 4, 8 / static_cast<int>(sizeof(T)), MAPS, CODES, KIND>(a, p, sms, st) : run<T, 1, 4, MAPS, CODES, KIND>(a, p, sms, st);
+  a.vec ? run<T, 4, 8 / static_cast<int>(sizeof(T)), MAPS, CODES, KIND>(a, p, sms, st) : run<T, 1, 8, MAPS, CODES, KIND>(a, p, sms, st);
 }
 
 template <class T, bool MAPS, bool CODES>

@@ -159,15 +159,15 @@ constexpr int64_t kSumRows = 64;  // above 8 times it the partial sums are added
 
 }  // namespace
 
-// Segments: as many as fill the SMs once with the forward kernels' 1024 threads each (lanes of 4
-// channels where rows are aligned), none
-// shorter than 2 kStateEvery; at most 4096, whose states the carry kernel walks in a few
-// microseconds. Sequences that fill half of that by themselves are left whole: the second
-// read would cost more than the idle threads.
+// Segments: as many as fill the SMs once with the forward kernels' threads (1024 an SM with the
+// slots of fp32 channels by four, else 768; a partly filled second round costs as much as a whole
+// one: 2 x 65,537 x 256 bf16 129 us with 768, 152 with 1024), none shorter than 2 kStateEvery; at
+// most 4096, whose states the carry kernel walks in a few microseconds. Sequences that fill half
+// of that by themselves are left whole: the second read would cost more than the idle threads.
 ScanPlan scan_plan(const ScanArgs& a, int sms, void* workspace) {
   const int64_t batch = a.offsets != nullptr ? 1 : a.batch;
   const int64_t lanes = batch * ((a.width + (a.vec ? 3 : 0)) / (a.vec ? 4 : 1));
-  const int64_t want = static_cast<int64_t>(sms) * 1024;
+  const int64_t want = static_cast<int64_t>(sms) * (a.vec && !a.bf16 ? 1024 : 768);
   ScanPlan p;
   p.seg = {1, (a.steps + kStateEvery - 1) / kStateEvery * kStateEvery};
   if (lanes * 2 < want && a.steps > 4 * kStateEvery) {
