@@ -30,7 +30,8 @@ struct Team {
 };
 
 // Sums of N values over the team, the same on every thread, in a fixed order. For
-// whole-block teams `box` alternates between two halves, so one barrier per call does.
+// whole-block teams `box` (zero where no warp writes) alternates between two halves, so one
+// barrier per call does.
 template <int N>
 __device__ __forceinline__ void team_sum(const Team& T, float (&v)[N], float (*box)[N][32], int& turn) {
   const int width = min(T.size, 32);
@@ -50,9 +51,17 @@ __device__ __forceinline__ void team_sum(const Team& T, float (&v)[N], float (*b
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     float s = 0.f;
-    for (int w = 0; w < warps; ++w) s += b[i][w];
+    for (int w = 0; w < warps; w += 4) {
+      const float4 q = *reinterpret_cast<const float4*>(&b[i][w]);
+      s += (q.x + q.y) + (q.z + q.w);
+    }
     v[i] = s;
   }
+}
+
+template <int N>
+__device__ __forceinline__ void clear_box(float (*box)[N][32]) {
+  for (int i = threadIdx.x; i < 2 * N * 32; i += blockDim.x) (&box[0][0][0])[i] = 0.f;
 }
 
 // One thread's vectors of a row on their way to registers: two rows' slots of W streams. Vector j
@@ -66,10 +75,11 @@ struct Slots {
 };
 
 template <class T, int V, int NV, int MAXT, bool CODES, bool AHEAD>
-__global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const NormArgs A, const Team M) {
+__global__ void __launch_bounds__(MAXT, MAXT > 256 ? 1 : NV * V <= 8 && !CODES ? 4 : 2)
+    norm_fwd_kernel(const NormArgs A, const Team M) {
   constexpr bool kAsync = AHEAD;
   extern __shared__ uint4 smem[];
-  __shared__ float box[2][1][32];
+  __shared__ __align__(16) float box[2][1][32];
   int turn = 0;
   const int team = threadIdx.x / M.size, lane = threadIdx.x % M.size, teams = M.block / M.size;
   const int H = A.width;
@@ -89,17 +99,28 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const NormArgs A, const 
   const int64_t ld[3] = {A.x_ld, A.u_ld, A.gate_ld};
   using Raw = typename Pack<T, V>::Raw;
   Slots<Raw, 3, NV> slots{reinterpret_cast<Raw*>(smem) + threadIdx.x, static_cast<int>(blockDim.x)};
+  // this thread's vectors inside the row: the first n of them
+  const int c0 = lane * V, step = M.size * V;
+  const int n_live = c0 < H ? min(NV, (H - c0 + step - 1) / step) : 0;
+  clear_box(box);
+  if constexpr (kAsync) {  // what no copy writes reads as zero
+#pragma unroll
+    for (int w = 0; w < 3; ++w)
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (j >= n_live || src[w] == nullptr) *slots.slot(0, w, j) = *slots.slot(1, w, j) = Raw{};
+  }
+  __syncthreads();
   auto fetch = [&](int64_t row, int buf) {
     if constexpr (kAsync) {
       if (row < A.rows) {
 #pragma unroll
         for (int w = 0; w < 3; ++w) {
           if (src[w] == nullptr) continue;
+          const T* from = src[w] + row * ld[w] + c0;
 #pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            const int c = (j * M.size + lane) * V;
-            if (c < H) copy_async<sizeof(Raw)>(slots.slot(buf, w, j), src[w] + row * ld[w] + c);
-          }
+          for (int j = 0; j < NV; ++j, from += step)
+            if (j < n_live) copy_async<sizeof(Raw)>(slots.slot(buf, w, j), from);
         }
       }
       commit_copies();
@@ -111,25 +132,25 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const NormArgs A, const 
   fetch(static_cast<int64_t>(blockIdx.x) * teams + team, 0);
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * teams; r0 < A.rows; r0 += stride, buf ^= 1) {
     const int64_t row = r0 + team;
-    const bool in = row < A.rows;
+    const int n = row < A.rows ? n_live : 0;  // vectors to read and write
     fetch(row + stride, buf ^ 1);
     if constexpr (kAsync) wait_copies<1>();
     float f[3][NV][V];
 #pragma unroll
-    for (int w = 0; w < 3; ++w)
+    for (int w = 0; w < 3; ++w) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int c = (j * M.size + lane) * V;
         Pack<T, V> a;
-        a.zero();
-        if (in && c < H && src[w] != nullptr) {
-          if constexpr (kAsync)
-            a.raw = *slots.slot(buf, w, j);
-          else
-            a.load(src[w] + row * ld[w] + c);
+        if constexpr (kAsync) {
+          a.raw = *slots.slot(buf, w, j);  // of an earlier row behind the last: nothing of it is written
+        } else {
+          const int c = (j * M.size + lane) * V;
+          a.zero();
+          if (row < A.rows && c < H && src[w] != nullptr) a.load(src[w] + row * ld[w] + c);
         }
         a.get(f[w][j]);
       }
+    }
     float(&x)[NV][V] = f[0];
     float(&u)[NV][V] = f[1];
     float(&g)[NV][V] = f[2];
@@ -137,14 +158,15 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const NormArgs A, const 
 #pragma unroll
       for (int w = 0; w < 3; ++w) {
         if (src[w] == nullptr) continue;
+        int8_t* code = A.codes + (w * A.rows + row) * H + c0;
+        float* scale = A.scales + (w * A.rows + row) * G + c0 / kGroup8;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int c = (j * M.size + lane) * V;
+        for (int j = 0; j < NV; ++j, code += step, scale += step / kGroup8) {
           Codes<V> q;
           const float s = encode8(f[w][j], q);
-          if (in && c < H) {
-            q.store(A.codes + (w * A.rows + row) * H + c);
-            if (c % kGroup8 == 0) A.scales[(w * A.rows + row) * G + c / kGroup8] = s;
+          if (j < n) {
+            q.store(code);
+            if (c0 % kGroup8 == 0) *scale = s;  // a team is whole groups wide
           }
         }
       }
@@ -162,16 +184,15 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const NormArgs A, const 
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int c = (j * M.size + lane) * V;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float t = sc[j][v] * (A.gate != nullptr ? sigmoid_f(g[j][v]) : 1.f);
           x[j][v] = fmaf(t, u[j][v] * ru * wp[j][v], x[j][v]);
         }
-        if (in && c < H) {
+        if (j < n) {
           Pack<T, V> o;
           o.set(x[j]);
-          o.store(static_cast<T*>(A.y) + row * H + c);
+          o.store(static_cast<T*>(A.y) + row * H + c0 + j * step);
         }
       }
     }
@@ -185,14 +206,13 @@ __global__ void __launch_bounds__(MAXT) norm_fwd_kernel(const NormArgs A, const 
       const float ry = rsqrtf(q[0] * over + A.eps);
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int c = (j * M.size + lane) * V;
-        if (in && c < H) {
-          float n[V];
+        if (j < n) {
+          float t[V];
 #pragma unroll
-          for (int v = 0; v < V; ++v) n[v] = x[j][v] * ry * wn[j][v];
+          for (int v = 0; v < V; ++v) t[v] = x[j][v] * ry * wn[j][v];
           Pack<T, V> o;
-          o.set(n);
-          o.store(static_cast<T*>(A.n) + row * H + c);
+          o.set(t);
+          o.store(static_cast<T*>(A.n) + row * H + c0 + j * step);
         }
       }
     }
@@ -206,8 +226,8 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const 
   // streams: dy, dn, and without codes x, u, gate; with them three words of codes and three scales
   constexpr int W = CODES ? 2 : 5;
   constexpr int kWords = CODES ? 6 : 0;
-  __shared__ float box1[2][1][32];
-  __shared__ float box2[2][2][32];
+  __shared__ __align__(16) float box1[2][1][32];
+  __shared__ __align__(16) float box2[2][2][32];
   extern __shared__ uint4 smem[];
   int turn1 = 0, turn2 = 0;
   const int team = threadIdx.x / M.size, lane = threadIdx.x % M.size, teams = M.block / M.size;
@@ -232,22 +252,45 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const 
   Slots<uint32_t, kWords, NV> words{
       reinterpret_cast<uint32_t*>(reinterpret_cast<Raw*>(smem) + 2 * W * NV * blockDim.x) + threadIdx.x,
       static_cast<int>(blockDim.x)};
+  const int c0 = lane * V, step = M.size * V;
+  const int n_live = c0 < H ? min(NV, (H - c0 + step - 1) / step) : 0;
+  clear_box(box1);
+  clear_box(box2);
+  if constexpr (kAsync) {  // what no copy writes reads as zero
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int w = 0; w < W; ++w)
+        if (j >= n_live || src[w] == nullptr) *slots.slot(0, w, j) = *slots.slot(1, w, j) = Raw{};
+#pragma unroll
+      for (int w = 0; w < kWords; ++w)
+        if (j >= n_live || src[2 + w % 3] == nullptr) *words.slot(0, w, j) = *words.slot(1, w, j) = 0;
+    }
+  }
+  __syncthreads();
   auto fetch = [&](int64_t row, int buf) {
     if constexpr (kAsync) {
       if (row < A.rows) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int c = (j * M.size + lane) * V;
-          if (c >= H) continue;
+        for (int w = 0; w < W; ++w) {
+          if (src[w] == nullptr) continue;
+          const T* from = src[w] + row * ld[w] + c0;
 #pragma unroll
-          for (int w = 0; w < W; ++w)
-            if (src[w] != nullptr) copy_async<sizeof(Raw)>(slots.slot(buf, w, j), src[w] + row * ld[w] + c);
-          if constexpr (CODES) {
+          for (int j = 0; j < NV; ++j, from += step)
+            if (j < n_live) copy_async<sizeof(Raw)>(slots.slot(buf, w, j), from);
+        }
+        if constexpr (CODES) {
 #pragma unroll
-            for (int w = 0; w < 3; ++w) {
-              if (src[2 + w] == nullptr) continue;
-              copy_async<4>(words.slot(buf, w, j), A.codes + (w * A.rows + row) * H + c);
-              copy_async<4>(words.slot(buf, 3 + w, j), A.scales + (w * A.rows + row) * G + c / kGroup8);
+          for (int w = 0; w < 3; ++w) {
+            if (src[2 + w] == nullptr) continue;
+            const int8_t* code = A.codes + (w * A.rows + row) * H + c0;
+            const float* scale = A.scales + (w * A.rows + row) * G + c0 / kGroup8;
+#pragma unroll
+            for (int j = 0; j < NV; ++j, code += step, scale += step / kGroup8) {
+              if (j < n_live) {
+                copy_async<4>(words.slot(buf, w, j), code);
+                copy_async<4>(words.slot(buf, 3 + w, j), scale);
+              }
             }
           }
         }
@@ -260,40 +303,51 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const 
   fetch(static_cast<int64_t>(blockIdx.x) * teams + team, 0);
   for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * teams; r0 < A.rows; r0 += stride, buf ^= 1) {
     const int64_t row = r0 + team;
-    const bool in = row < A.rows;
+    const int n = row < A.rows ? n_live : 0;  // vectors to read and write
     fetch(row + stride, buf ^ 1);
     if constexpr (kAsync) wait_copies<1>();
     float f[5][NV][V];
 #pragma unroll
-    for (int w = 0; w < 5; ++w)
+    for (int w = 0; w < 5; ++w) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int c = (j * M.size + lane) * V;
-#pragma unroll
-        for (int v = 0; v < V; ++v) f[w][j][v] = 0.f;
-        if (!in || c >= H || src[w] == nullptr) continue;
         if constexpr (CODES) {
           if (w >= 2) {
             Codes<V> q;
-            float s;
+            float s = 0.f;
             if constexpr (kAsync) {
               q.raw = static_cast<typename RawOf<V>::type>(*words.slot(buf, w - 2, j));
               s = __uint_as_float(*words.slot(buf, w + 1, j));
             } else {
-              q.load(A.codes + ((w - 2) * A.rows + row) * H + c);
-              s = A.scales[((w - 2) * A.rows + row) * G + c / kGroup8];
+              q.zero();
+              if (j < n && src[w] != nullptr) {
+                q.load(A.codes + ((w - 2) * A.rows + row) * H + c0 + j * step);
+                s = A.scales[((w - 2) * A.rows + row) * G + (c0 + j * step) / kGroup8];
+              }
             }
             q.get(s, f[w][j]);
             continue;
           }
         }
         Pack<T, V> a;
-        if constexpr (kAsync)
+        if constexpr (kAsync) {
           a.raw = *slots.slot(buf, w < W ? w : 0, j);
-        else
-          a.load(src[w] + row * ld[w] + c);
+        } else {
+          const int c = (j * M.size + lane) * V;
+          a.zero();
+          if (row < A.rows && c < H && src[w] != nullptr) a.load(src[w] + row * ld[w] + c);
+        }
         a.get(f[w][j]);
       }
+    }
+    if (kAsync && row >= A.rows) {  // an earlier row's values: nothing of them reaches the sums
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int v = 0; v < V; ++v) f[w][j][v] = 0.f;
+    }
     float(&dy)[NV][V] = f[0];
     float(&dn)[NV][V] = f[1];
     float(&x)[NV][V] = f[2];
@@ -343,18 +397,16 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const 
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * M.size + lane) * V;
-      if (in && c < H && A.dx != nullptr) {
+      if (j < n) {
         Pack<T, V> o;
         o.set(dy[j]);
-        o.store(static_cast<T*>(A.dx) + row * H + c);
+        o.store(static_cast<T*>(A.dx) + row * H + c0 + j * step);
       }
     }
     if (A.u == nullptr) continue;
     float q[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * M.size + lane) * V;
       float dg[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) {
@@ -367,10 +419,10 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const 
         dn[j][v] = dv * wp[j][v];
         q[0] = fmaf(dn[j][v], u[j][v], q[0]);
       }
-      if (in && c < H && A.dgate != nullptr) {
+      if (j < n && A.dgate != nullptr) {
         Pack<T, V> o;
         o.set(dg);
-        o.store(static_cast<T*>(A.dgate) + row * H + c);
+        o.store(static_cast<T*>(A.dgate) + row * H + c0 + j * step);
       }
     }
     float m = 0.f;
@@ -380,14 +432,13 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const 
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int c = (j * M.size + lane) * V;
-      if (in && c < H && A.du != nullptr) {
-        float f[V];
+      if (j < n) {
+        float t[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) f[v] = ru * fmaf(-u[j][v], m, dn[j][v]);
+        for (int v = 0; v < V; ++v) t[v] = ru * fmaf(-u[j][v], m, dn[j][v]);
         Pack<T, V> o;
-        o.set(f);
-        o.store(static_cast<T*>(A.du) + row * H + c);
+        o.set(t);
+        o.store(static_cast<T*>(A.du) + row * H + c0 + j * step);
       }
     }
   }

@@ -56,8 +56,9 @@ void launch_sequences(const ScanArgs& a, int* marks, const float* from, float* t
 
 // carry[q] = the state before segment q (backwards: the gradient after it), from `start` through
 // the maps of the segments before it (after it). A block has 8 channels of one sequence (64
-// bytes of maps, two sectors); each of its 128 rows composes a share of the segments, the shares
-// meet in order, and the row walks its share again from the state it gets.
+// bytes of maps, two sectors); each of its rows of threads (a quarter of the segments' number, up
+// to 128) composes a share of the segments, the shares meet in order, and the row walks its
+// share again from the state it gets.
 constexpr int kShares = 128, kShareCols = 8;
 __global__ void __launch_bounds__(kShareCols * kShares) scan_carry_kernel(const float2* __restrict__ maps, const float* start,
                                                                   int64_t n, int64_t batch, int H, bool bwd,
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(kShareCols * kShares) scan_carry_kernel(const 
   const int c = blockIdx.y * kShareCols + threadIdx.x;
   const int64_t b = blockIdx.x;
   const bool live = c < H;
-  const int64_t share = (n + kShares - 1) / kShares;
+  const int64_t share = (n + blockDim.y - 1) / blockDim.y;
   const int64_t lo = min(n, threadIdx.y * share), hi = min(n, lo + share);
   const int64_t step = (bwd ? -1 : 1) * batch * H;
   const int64_t at = ((bwd ? n - 1 - lo : lo) * batch + b) * H + c;
@@ -102,9 +103,11 @@ __global__ void __launch_bounds__(kShareCols * kShares) scan_carry_kernel(const 
 void launch_carry(const ScanArgs& a, const ScanPlan& p, bool bwd, cudaStream_t st) {
   const int64_t batch = a.offsets != nullptr ? 1 : a.batch;
   const float* start = a.offsets != nullptr ? nullptr : (bwd ? a.dlast : a.h0);
+  int shares = 4;
+  while (shares < kShares && shares * 4 < p.seg.n) shares *= 2;
   count_launch();
   scan_carry_kernel<<<dim3(static_cast<unsigned>(batch), (a.width + kShareCols - 1) / kShareCols),
-                      dim3(kShareCols, kShares), 0, st>>>(p.maps, start, p.seg.n, batch, a.width, bwd, p.carry);
+                      dim3(kShareCols, shares), 0, st>>>(p.maps, start, p.seg.n, batch, a.width, bwd, p.carry);
 }
 
 // Rows k, k + m, k + 2m, ... of partial [n, H] added up in order into row k of out [m, H]:

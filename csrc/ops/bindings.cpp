@@ -188,7 +188,7 @@ std::tuple<c10::optional<at::Tensor>, c10::optional<at::Tensor>> norm_residual(
     const at::Tensor& x, const c10::optional<at::Tensor>& u, const c10::optional<at::Tensor>& gate,
     const c10::optional<at::Tensor>& w_post, const c10::optional<at::Tensor>& w_pre,
     const c10::optional<at::Tensor>& scale, double eps, bool keep8);
-std::vector<at::Tensor> quantize8(const at::Tensor& x);
+std::tuple<at::Tensor, at::Tensor> quantize8(const at::Tensor& x);
 at::Tensor dequantize8(const at::Tensor& codes, const at::Tensor& scales, bool bf16);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

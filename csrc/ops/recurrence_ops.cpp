@@ -597,19 +597,22 @@ std::tuple<OptTensor, OptTensor> norm_residual(const at::Tensor& x, const OptTen
   return {maybe(y), maybe(n)};
 }
 
-// x [rows, H] -> codes [rows, H], scales [rows, ceil(H / 32)]
-std::vector<at::Tensor> quantize8(const at::Tensor& x) {
-  SU_CHECK_CUDA(x);
-  TORCH_CHECK(is_float_type(x) && x.dim() == 2 && x.size(1) > 0, "quantize8: x must be float32 or bfloat16 rows");
-  TORCH_CHECK(unit_last(x), "quantize8: x must have unit stride along its last dimension");
-  TORCH_CHECK(x.size(1) <= INT32_MAX, "quantize8: rows of at most 2^31 - 1 values");
-  c10::cuda::CUDAGuard guard(x.device());
+// x [.., H] -> codes [rows, H], scales [rows, ceil(H / 32)]
+std::tuple<at::Tensor, at::Tensor> quantize8(const at::Tensor& x_in) {
+  SU_CHECK_CUDA(x_in);
+  TORCH_CHECK(is_float_type(x_in) && x_in.dim() >= 1 && x_in.size(-1) > 0,
+              "quantize8: x must be float32 or bfloat16 with a last dimension of at least one value");
+  TORCH_CHECK(x_in.size(-1) <= INT32_MAX, "quantize8: rows of at most 2^31 - 1 values");
+  c10::cuda::CUDAGuard guard(x_in.device());
+  at::AutoDispatchBelowADInplaceOrView below;  // the codes have no gradient
+  const at::Tensor x = as_rows(x_in, x_in.size(-1));
   const int64_t rows = x.size(0), H = x.size(1);
   at::Tensor codes = at::empty({rows, H}, x.options().dtype(at::kChar));
   at::Tensor scales = at::empty({rows, groups_of(H)}, x.options().dtype(at::kFloat));
   if (rows == 0) return {codes, scales};
   launch_quantize8(x.data_ptr(), x.scalar_type() == at::kBFloat16, x.stride(0), rows, static_cast<int>(H),
-                   codes.data_ptr<int8_t>(), scales.data_ptr<float>(), rows_of_four(x), num_sms(x.get_device()), cur_stream());
+                   codes.data_ptr<int8_t>(), scales.data_ptr<float>(), rows_of_four(x), num_sms(x.get_device()),
+                   cur_stream());
   SU_LAUNCH_CHECK();
   return {codes, scales};
 }

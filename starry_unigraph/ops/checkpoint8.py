@@ -78,11 +78,14 @@ class Packed8:
             out = cuda_ext().dequantize8(self.codes, self.scales, dtype == torch.bfloat16)
         else:
             out = _dequantize_torch(self.codes, self.scales, dtype)
-        return out.view(self.shape)
+        return out if out.shape == self.shape else out.view(self.shape)
 
 
 def quantize8(x: torch.Tensor) -> Packed8:
     """8-bit codes of x along its last dimension (float32 or bfloat16; on CPU float64 too)."""
+    if x.is_cuda:
+        codes, scales = cuda_ext().quantize8(x)
+        return Packed8(codes, scales, x.shape, x.dtype)
     if x.dim() == 0 or x.size(-1) == 0:
         raise ValueError("quantize8: x needs a last dimension of at least one value")
     if not x.is_floating_point():
@@ -90,7 +93,7 @@ def quantize8(x: torch.Tensor) -> Packed8:
     rows = x.detach().reshape(-1, x.size(-1))
     if rows.size(1) > 1 and rows.stride(1) != 1:
         rows = rows.contiguous()
-    codes, scales = cuda_ext().quantize8(rows) if x.is_cuda else _quantize_torch(rows)
+    codes, scales = _quantize_torch(rows)
     return Packed8(codes, scales, x.shape, x.dtype)
 
 
