@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(MAXT, MAXT > 256 ? 1 : NV * V <= 8 && !CODES ?
 }
 
 template <class T, int V, int NV, int MAXT, bool CODES, bool AHEAD>
-__global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const Team M) {
+__global__ void __launch_bounds__(MAXT, MAXT > 256 || NV * V > 12 ? 1 : 2)
+    norm_bwd_kernel(const NormArgs A, const Team M) {
   constexpr bool kAsync = AHEAD;
   using Raw = typename Pack<T, V>::Raw;
   // streams: dy, dn, and without codes x, u, gate; with them three words of codes and three scales
@@ -234,23 +235,58 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const 
   const int H = A.width;
   const int G = (H + kGroup8 - 1) / kGroup8;
   const float over = 1.f / static_cast<float>(H);
-  float wp[NV][V], wn[NV][V], sc[NV][V], gp[NV][V], gn[NV][V], gs[NV][V];
+  float gp[NV][V], gn[NV][V], gs[NV][V];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int c = (j * M.size + lane) * V + v;
-      wp[j][v] = (c < H && A.w_post != nullptr) ? param_at(A.w_post, A.post_bf16, c) : 1.f;
-      wn[j][v] = (c < H && A.w_pre != nullptr) ? param_at(A.w_pre, A.pre_bf16, c) : 1.f;
-      sc[j][v] = (c < H && A.scale != nullptr) ? param_at(A.scale, A.scale_bf16, c) : 1.f;
-      gp[j][v] = gn[j][v] = gs[j][v] = 0.f;
+    for (int v = 0; v < V; ++v) gp[j][v] = gn[j][v] = gs[j][v] = 0.f;
+  // The three vectors in shared memory, one copy a block: registers go to the row and its sums
+  // (8-bit 400,000 x 172: 456 -> 409 us). Lanes of 8 columns would meet in the banks there and
+  // keep theirs in registers (16,384 x 2048 bf16: 181 -> 157 us).
+  constexpr bool kOwn = V == 8;
+  const int span = M.size * NV * V;
+  float* const vecs = reinterpret_cast<float*>(smem);
+  float own[3][kOwn ? NV : 1][kOwn ? V : 1];
+  auto param = [&](int w, int c) {
+    const void* p = w == 0 ? A.w_post : w == 1 ? A.w_pre : A.scale;
+    const int bf16 = w == 0 ? A.post_bf16 : w == 1 ? A.pre_bf16 : A.scale_bf16;
+    return c < H && p != nullptr ? param_at(p, bf16, c) : 1.f;
+  };
+#pragma unroll
+  for (int w = 0; w < 3; ++w) {
+    if constexpr (kOwn) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) own[w][j][v] = param(w, (j * M.size + lane) * V + v);
+    } else {
+      for (int c = threadIdx.x; c < span; c += blockDim.x) vecs[w * span + c] = param(w, c);
     }
+  }
+  auto vec = [&](int w, int j, float (&f)[V]) {
+    if constexpr (kOwn) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) f[v] = own[w][j][v];
+    } else {
+      const float* p = vecs + w * span + (j * M.size + lane) * V;
+      if constexpr (V == 1) {
+        f[0] = *p;
+      } else {
+        const float4 q = *reinterpret_cast<const float4*>(p);
+        f[0] = q.x;
+        f[1] = q.y;
+        f[2] = q.z;
+        f[3] = q.w;
+      }
+    }
+  };
+  uint4* const rest = kOwn ? smem : smem + (3 * span + 3) / 4;
   const T* src[5] = {static_cast<const T*>(A.dy), static_cast<const T*>(A.dn), static_cast<const T*>(A.x),
                      static_cast<const T*>(A.u), static_cast<const T*>(A.gate)};
   const int64_t ld[5] = {A.dy_ld, A.dn_ld, A.x_ld, A.u_ld, A.gate_ld};
-  Slots<Raw, W, NV> slots{reinterpret_cast<Raw*>(smem) + threadIdx.x, static_cast<int>(blockDim.x)};
+  Slots<Raw, W, NV> slots{reinterpret_cast<Raw*>(rest) + threadIdx.x, static_cast<int>(blockDim.x)};
   Slots<uint32_t, kWords, NV> words{
-      reinterpret_cast<uint32_t*>(reinterpret_cast<Raw*>(smem) + 2 * W * NV * blockDim.x) + threadIdx.x,
+      reinterpret_cast<uint32_t*>(reinterpret_cast<Raw*>(rest) + 2 * W * NV * blockDim.x) + threadIdx.x,
       static_cast<int>(blockDim.x)};
   const int c0 = lane * V, step = M.size * V;
   const int n_live = c0 < H ? min(NV, (H - c0 + step - 1) / step) : 0;
@@ -366,34 +402,44 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const 
         ru = rsqrtf(q[0] * over + A.eps);
       }
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
+        float wp[V], sc[V];
+        vec(0, j, wp);
+        vec(2, j, sc);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           g[j][v] = A.gate != nullptr ? sigmoid_f(g[j][v]) : 1.f;
           u[j][v] *= ru;
-          x[j][v] = fmaf(sc[j][v] * g[j][v], u[j][v] * wp[j][v], x[j][v]);
+          x[j][v] = fmaf(sc[v] * g[j][v], u[j][v] * wp[v], x[j][v]);
         }
+      }
     }
     if (A.dn != nullptr) {
       float q[2] = {0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
+        float wn[V];
+        vec(1, j, wn);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           q[0] = fmaf(x[j][v], x[j][v], q[0]);
-          q[1] = fmaf(dn[j][v] * wn[j][v], x[j][v], q[1]);
+          q[1] = fmaf(dn[j][v] * wn[v], x[j][v], q[1]);
         }
+      }
       team_sum(M, q, box2, turn2);
       const float ry = rsqrtf(q[0] * over + A.eps);
       const float m = q[1] * ry * over;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j) {
+        float wn[V];
+        vec(1, j, wn);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float yh = x[j][v] * ry;
           gn[j][v] = fmaf(dn[j][v], yh, gn[j][v]);
-          dy[j][v] = fmaf(ry, fmaf(-yh, m, dn[j][v] * wn[j][v]), dy[j][v]);
+          dy[j][v] = fmaf(ry, fmaf(-yh, m, dn[j][v] * wn[v]), dy[j][v]);
         }
+      }
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -407,16 +453,18 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const 
     float q[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      float dg[V];
+      float dg[V], wp[V], sc[V];
+      vec(0, j, wp);
+      vec(2, j, sc);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float vv = u[j][v] * wp[j][v];
+        const float vv = u[j][v] * wp[v];
         const float ds = dy[j][v] * g[j][v];
         gs[j][v] = fmaf(ds, vv, gs[j][v]);
-        dg[v] = ds * sc[j][v] * vv * (1.f - g[j][v]);
-        const float dv = ds * sc[j][v];
+        dg[v] = ds * sc[v] * vv * (1.f - g[j][v]);
+        const float dv = ds * sc[v];
         gp[j][v] = fmaf(dv, u[j][v], gp[j][v]);
-        dn[j][v] = dv * wp[j][v];
+        dn[j][v] = dv * wp[v];
         q[0] = fmaf(dn[j][v], u[j][v], q[0]);
       }
       if (j < n && A.dgate != nullptr) {
@@ -444,7 +492,6 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(const NormArgs A, const 
   }
   // the block's share of the three column sums, its teams added up in order
   float* sums = reinterpret_cast<float*>(smem);  // [teams][size * NV * V] of one vector at a time
-  const int span = M.size * NV * V;
 #pragma unroll
   for (int w = 0; w < 3; ++w) {
     __syncthreads();
@@ -560,7 +607,8 @@ void run_case(const NormArgs& a, const Shape& s, int sms, cudaStream_t st, int* 
   static int fits[33] = {};
   const size_t threads = s.team.block;
   if constexpr (BWD) {
-    size_t smem = AHEAD ? threads * 2 * NV * (CODES ? 2 * sizeof(T) * V + 24 : 5 * sizeof(T) * V) : 0;
+    const size_t vecs = V == 8 ? 0 : (3 * s.team.size * NV * V + 3) / 4 * 16;
+    size_t smem = vecs + (AHEAD ? threads * 2 * NV * (CODES ? 2 * sizeof(T) * V + 24 : 5 * sizeof(T) * V) : 0);
     const size_t sums = threads * NV * V * sizeof(float);
     smem = smem > sums ? smem : sums;
     run(norm_bwd_kernel<T, V, NV, MAXT, CODES, AHEAD>, fits, a, s, smem, sms, st, grid);
