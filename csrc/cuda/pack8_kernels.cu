@@ -14,11 +14,12 @@ __global__ void __launch_bounds__(256) quantize8_kernel(const T* __restrict__ x,
                                                         int8_t* __restrict__ codes, float* __restrict__ scales,
                                                         const Lanes L) {
   const int G = (H + kGroup8 - 1) / kGroup8;
-  const int c = (blockIdx.y * L.count + threadIdx.x % L.count) * V;
-  const bool live = c < H;
   const int64_t step = static_cast<int64_t>(gridDim.x) * L.rows;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * L.rows + threadIdx.x / L.count; r0 < rows;
+  for (int cb = blockIdx.y; cb < L.blocks; cb += gridDim.y)  // very long rows
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * L.rows + threadIdx.x / L.count; r0 < rows;
        r0 += kUnroll * step) {
+    const int c = (cb * L.count + threadIdx.x % L.count) * V;
+    const bool live = c < H;
     Pack<T, V> a[kUnroll];
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
@@ -46,11 +47,12 @@ __global__ void __launch_bounds__(256) dequantize8_kernel(const int8_t* __restri
                                                           const float* __restrict__ scales, int64_t rows, int H,
                                                           T* __restrict__ x, const Lanes L) {
   const int G = (H + kGroup8 - 1) / kGroup8;
-  const int c = (blockIdx.y * L.count + threadIdx.x % L.count) * V;
-  if (c >= H) return;
   const int64_t step = static_cast<int64_t>(gridDim.x) * L.rows;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * L.rows + threadIdx.x / L.count; r0 < rows;
+  for (int cb = blockIdx.y; cb < L.blocks; cb += gridDim.y)  // very long rows
+    for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * L.rows + threadIdx.x / L.count; r0 < rows;
        r0 += kUnroll * step) {
+    const int c = (cb * L.count + threadIdx.x % L.count) * V;
+    if (c >= H) break;
     Codes<V> q[kUnroll];
     float s[kUnroll];
 #pragma unroll
@@ -77,7 +79,7 @@ __global__ void __launch_bounds__(256) dequantize8_kernel(const int8_t* __restri
 dim3 grid_of(int64_t rows, const Lanes& l, int sms) {
   const int64_t want = (rows + l.rows * kUnroll - 1) / (l.rows * kUnroll);
   const int64_t most = (static_cast<int64_t>(sms) * 32 + l.blocks - 1) / l.blocks;
-  return dim3(static_cast<unsigned>(want < most ? want : most), l.blocks);
+  return dim3(static_cast<unsigned>(want < most ? want : most), l.blocks < 65535 ? l.blocks : 65535);
 }
 
 template <class T, int V>

@@ -60,7 +60,7 @@ ScanSizes scan_sizes(at::IntArrayRef shape, const OptTensor& offsets, int64_t pe
               "gated_scan: p must be [batch, steps, 3H], or [rows, 3H] with offsets");
   TORCH_CHECK(shape.back() > 0 && shape.back() % per_row == 0, "gated_scan: the last dimension of p must be 3H, H > 0");
   s.width = shape.back() / per_row;
-  TORCH_CHECK(s.width <= (1 << 24), "gated_scan: H above 2^24");
+  TORCH_CHECK(s.width <= (1 << 18), "gated_scan: H above 2^18");
   s.steps = s.packed ? shape[0] : shape[1];
   s.batch = s.packed ? offsets->size(0) - 1 : shape[0];
   return s;
@@ -312,7 +312,7 @@ at::Tensor gated_scan_step(const at::Tensor& p_in, const at::Tensor& decay, at::
   TORCH_CHECK(p.dim() == 2 && p.size(1) > 0 && p.size(1) % 3 == 0 && unit_last(p),
               "gated_scan_step: p must be [rows, 3H] with unit stride along its last dimension");
   const int64_t n = p.size(0), H = p.size(1) / 3;
-  TORCH_CHECK(H <= (1 << 24), "gated_scan_step: H above 2^24");
+  TORCH_CHECK(H <= (1 << 18), "gated_scan_step: H above 2^18");
   TORCH_CHECK(rate > 0 && std::isfinite(rate), "gated_scan_step: rate must be positive and finite");
   c10::cuda::CUDAGuard guard(p.device());
   check_param(decay, "gated_scan_step: decay", H, p.device());

@@ -544,3 +544,111 @@ def test_example_on_cuda(tmp_path, monkeypatch):
                              "--checkpoint", keep, "--artifact-root", str(tmp_path / keep)])
         assert res[keep]["train"][-1] < res[keep]["train"][0]
     assert abs(res["int8"]["train"][-1] - res["none"]["train"][-1]) < 0.02 * res["none"]["train"][-1]
+
+
+def test_more_refusals_on_cuda():
+    """Shapes, devices and types that the calls refuse, each before anything is launched."""
+    from starry_unigraph.ops.checkpoint8 import quantize8
+    from starry_unigraph.ops.norm import norm_residual, rms_norm
+    from starry_unigraph.ops.recurrence import gated_scan, gated_scan_step
+
+    p, d = torch.randn(2, 3, 12, device="cuda"), torch.randn(4, device="cuda")
+    m = torch.ones(2, 3, dtype=torch.bool, device="cuda")
+    off = torch.tensor([0, 1, 3], device="cuda")
+    x, w = torch.randn(3, 8, device="cuda"), torch.randn(8, device="cuda")
+    t = torch.zeros(5, 4, device="cuda")
+    for bad in (lambda: gated_scan(p[..., :11], d), lambda: gated_scan(p, d[:3]), lambda: gated_scan(p, torch.stack([d, d])),
+                lambda: gated_scan(p, d, torch.zeros(3, 4, device="cuda")), lambda: gated_scan(p, d, mask=m.t()),
+                lambda: gated_scan(p, d, mask=m.float()), lambda: gated_scan(p, d, mask=m.cpu()),
+                lambda: gated_scan(p, d, offsets=off), lambda: gated_scan(p[0], d), lambda: gated_scan(p, d, rate=-1.0),
+                lambda: gated_scan(p, d, rate=float("inf")), lambda: gated_scan(p, d, checkpoint="int4"),
+                lambda: gated_scan(p[0], d, torch.zeros(3, 4, device="cuda"), offsets=off),
+                lambda: gated_scan(torch.randn(1, 1, 3 << 19, device="cuda"), torch.randn(1 << 19, device="cuda")),
+                lambda: gated_scan_step(p[0, :, :11], d, t), lambda: gated_scan_step(p[0].half(), d, t[:3]),
+                lambda: gated_scan_step(p[0], d, t[:3], rate=0.0), lambda: gated_scan_step(p[0], d, t.t()[:3]),
+                lambda: norm_residual(x, x[:2], w), lambda: norm_residual(x, x, w[:7]), lambda: norm_residual(x, x.bfloat16(), w),
+                lambda: norm_residual(x, x, w, eps=0.0), lambda: norm_residual(x, x, w, gate=x[:, :4]),
+                lambda: norm_residual(x, x, w, scale=torch.ones(8)), lambda: rms_norm(x[:, :0], w[:0]),
+                lambda: norm_residual(x, x, w, checkpoint="fp8"), lambda: quantize8(x.half()), lambda: quantize8(x[:, :0]),
+                lambda: quantize8(torch.tensor(1.0, device="cuda")), lambda: quantize8(x).dequantize(torch.float16)):
+        with pytest.raises((RuntimeError, ValueError)):
+            bad()
+    status_clear()
+
+
+def test_gradients_are_not_differentiated_again():
+    from starry_unigraph.ops.norm import norm_residual
+    from starry_unigraph.ops.recurrence import gated_scan
+
+    p, d = torch.randn(2, 3, 12, device="cuda", requires_grad=True), torch.randn(4, device="cuda")
+    x, w = torch.randn(3, 8, device="cuda", requires_grad=True), torch.randn(8, device="cuda")
+    for out, leaf in ((gated_scan(p, d)[0], p), (norm_residual(x, x, w)[0], x)):
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(out.sum(), leaf, create_graph=True)
+    out = gated_scan(p, d)[0]
+    a, = torch.autograd.grad(out.sum(), p, retain_graph=True)
+    b, = torch.autograd.grad(out.sum(), p)  # the same graph again
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_scan_gradient_against_differences_on_cuda(checkpoint):
+    """Directional derivatives of the forward kernel alone: central differences with a step of 2^-6,
+    whose error is h^2 / 6 of the third derivative (below 2e-4 of the gradient here) plus the
+    rounding of fp32 sums over the step (1e-4); with 8-bit inputs the gradient is that at values up
+    to half a scale off (amax / 254, near 1 %)."""
+    from starry_unigraph.ops.recurrence import gated_scan
+
+    torch.manual_seed(11)
+    B, T, H = 3, 40, 64
+    p, d, h0 = (torch.randn(*s, device="cuda") for s in ((B, T, 3 * H), (H,), (B, H)))
+    gh, gl = torch.randn(B, T, H, device="cuda"), torch.randn(B, H, device="cuda")
+    leaves = [t.clone().requires_grad_() for t in (p, d, h0)]
+    h, last = gated_scan(*leaves, checkpoint=checkpoint)
+    grads = torch.autograd.grad((h, last), leaves, (gh, gl))
+
+    def f(*a):
+        h, last = gated_scan(*a)
+        return float((h.double() * gh).sum() + (last.double() * gl).sum())
+
+    for k in range(3):
+        u = [torch.zeros_like(t) for t in (p, d, h0)]
+        # along the gradient: the derivative is its norm, nothing cancels
+        u[k] = grads[k] / grads[k].norm()
+        e = 2.0 ** -6
+        got = (f(*[t + e * v for t, v in zip((p, d, h0), u)]) - f(*[t - e * v for t, v in zip((p, d, h0), u)])) / (2 * e)
+        want = float(grads[k].double().norm())
+        assert abs(got - want) < (2e-3 if checkpoint is None else 2e-2) * want
+
+
+@pytest.mark.parametrize("steps", [9, 31, 65, 200])
+@pytest.mark.parametrize("batch,H", [(1, 64), (1, 2048), (40, 300), (700, 129)])
+def test_scan_split_and_whole_agree(batch, H, steps):
+    """Few sequences are cut into segments, many are walked whole: the first of many equal the few
+    up to rounding, as 1, `batch` and many times `batch` sequences."""
+    from starry_unigraph.ops.recurrence import gated_scan
+
+    g = torch.Generator(device="cuda").manual_seed(steps)
+    many = batch * max(1, 200_000 // (batch * H))
+    p = torch.randn(many, steps, 3 * H, device="cuda", generator=g)
+    d, gh = torch.randn(H, device="cuda", generator=g) - 3, torch.randn(many, steps, H, device="cuda", generator=g)
+
+    def run(n):
+        q = p[:n].clone().requires_grad_()
+        h, last = gated_scan(q, d)
+        return h, last, torch.autograd.grad((h, last), q, (gh[:n], gh[:n, 0]))[0]
+
+    whole = run(many)
+    for n in (1, batch):
+        for a, b in zip(run(n), whole):
+            assert rel(a, b[:n]) < 2 * F32  # two fp32 results
+
+
+def test_codes_of_very_long_rows():
+    from starry_unigraph.ops.checkpoint8 import quantize8
+
+    x = torch.randn((1 << 25) + 35, device="cuda")
+    q = quantize8(x)
+    whole = quantize8(x[: 1 << 25].view(-1, 4096))
+    assert torch.equal(q.codes[0, : 1 << 25], whole.codes.view(-1))
+    assert torch.equal(q.dequantize()[-35:], quantize8(x[-35:]).dequantize())
