@@ -48,7 +48,7 @@ struct ScanArgs {
   const float* dlast = nullptr;  // [batch, H] or nullptr
   void* dp = nullptr;           // dense rows of 3H
   float* dh0 = nullptr;         // [batch, H] or nullptr
-  float* partial = nullptr;     // [n_partial, H] per-block sums of dz sigmoid(r)
+  float* partial = nullptr;     // [n_partial, H] per-block sums of -dz sigmoid(r)
   int vec = 1;                  // every row of p, dh, h, dp starts on a multiple of 4 values, H % 4 == 0
 };
 

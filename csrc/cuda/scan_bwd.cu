@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
   const int64_t batch = KIND == kPacked ? 1 : A.batch;
   const int64_t rows = live ? batch * P.seg.n : 0;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * L.rows;
-  float k[V], dl[V], E[V];
+  Vf<V> k, dl, E;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     k[v] = live ? decay_factor(param_at(A.decay, A.decay_bf16, c + v), A.rate) : 0.f;
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
           E[v] = A.dlast[u.b * H + c + v];
       }
     }
-    float h[V];
+    Vf<V> h;
     const float* from = t0 > 0 ? A.states + (u.b * A.n_states + t0 / A.state_every - 1) * H + c
                                : (KIND != kPacked && A.h0 != nullptr ? A.h0 + u.b * H + c : nullptr);
 #pragma unroll
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
     // WHOLE: every step of the chunk is inside the sequence and counts
     auto work = [&](auto whole) {
       constexpr bool WHOLE = decltype(whole)::value;
-      Slope f[CH][V];
+      Slope<V> f[CH];
 #pragma unroll
       for (int j = 0; j < CH; ++j) {
         if (KIND == kPacked && (firsts >> j & 1)) {
@@ -254,24 +254,18 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
 #pragma unroll
           for (int v = 0; v < V; ++v) h[v] = A.h0 != nullptr ? A.h0[q * H + c + v] : 0.f;
         }
-        float fx[V], fr[V], fi[V];
+        Vf<V> fx, fr, fi;
         if constexpr (kAsync) {
-          slots.get(buf, j, 0, c, fx);
-          slots.get(buf, j, 1, c, fr);
-          slots.get(buf, j, 2, c, fi);
+          slots.get(buf, j, 0, c, fx.v);
+          slots.get(buf, j, 1, c, fr.v);
+          slots.get(buf, j, 2, c, fi.v);
         } else {
-          held.get(j, 0, fx);
-          held.get(j, 1, fr);
-          held.get(j, 2, fi);
+          held.get(j, 0, fx.v);
+          held.get(j, 1, fr.v);
+          held.get(j, 2, fi.v);
         }
-        if (!WHOLE && !(on >> j & 1)) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) shut(fx[v], fr[v], fi[v]);
-        }
-        Gate g[V];
-        gates_of(fx, fr, fi, k, g);
-#pragma unroll
-        for (int v = 0; v < V; ++v) f[j][v] = slope_of(g[v], h[v]);
+        if (!WHOLE && !(on >> j & 1)) shut(fx, fr, fi);
+        f[j] = slope_of(gate_of(fx, fr, fi, k), h);
       }
       T* out = static_cast<T*>(A.dp) + (row + CH * A.row_st) * 3 * H + c;
 #pragma unroll
@@ -283,31 +277,26 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
 #pragma unroll
           for (int v = 0; v < V; ++v) E[v] = A.dlast != nullptr ? A.dlast[q * H + c + v] : 0.f;
         }
-        float dy[V], dx[V], dr[V], di[V];
+        Vf<V> dy;
         if constexpr (kAsync) {
-          slots.get_dh(buf, j, dy);
+          slots.get_dh(buf, j, dy.v);
           if (A.dh == nullptr) {
 #pragma unroll
             for (int v = 0; v < V; ++v) dy[v] = 0.f;
           }
         } else {
-          held.d[j].get(dy);
+          held.d[j].get(dy.v);
         }
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float g = dy[v] + E[v];
-          dx[v] = g * f[j][v].x;
-          dr[v] = g * f[j][v].r;
-          di[v] = g * f[j][v].i;
-          dl[v] = fmaf(g, f[j][v].l, dl[v]);
-          E[v] = g * f[j][v].a;
-        }
+        const Vf<V> g = dy + E;
+        const Vf<V> dx = g * f[j].x, dr = g * f[j].r, di = g * f[j].i;
+        dl = fma(g, f[j].l, dl);
+        E = g * f[j].a;
         Pack<T, V> o;
-        o.set(dx);
+        o.set(dx.v);
         o.store(out);
-        o.set(dr);
+        o.set(dr.v);
         o.store(out + H);
-        o.set(di);
+        o.set(di.v);
         o.store(out + 2 * H);
         if (KIND == kPacked && (firsts >> j & 1) && A.dh0 != nullptr) {
           const int64_t q = A.marks[t0 + j] >> 2;
@@ -329,7 +318,7 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
     more = more_next;
     buf ^= 1;
   }
-  // the block's share of sum dz sigmoid(r), added up over its rows in order
+  // the block's share of -sum dz sigmoid(r), added up over its rows in order
   __shared__ float sum[kBwdThreads * V];
 #pragma unroll
   for (int v = 0; v < V; ++v) sum[threadIdx.x * V + v] = dl[v];
@@ -354,7 +343,7 @@ __global__ void __launch_bounds__(256) scan_bwd_maps_kernel(const ScanArgs A, co
   const int G = (H + kGroup8 - 1) / kGroup8;
   const int64_t batch = KIND == kPacked ? 1 : A.batch;
   const int64_t rows = batch * P.seg.n;
-  float k[V];
+  Vf<V> k;
 #pragma unroll
   for (int v = 0; v < V; ++v) k[v] = decay_factor(param_at(A.decay, A.decay_bf16, c + v), A.rate);
   for (int64_t rr = static_cast<int64_t>(blockIdx.x) * L.rows + y; rr < rows;
@@ -363,7 +352,7 @@ __global__ void __launch_bounds__(256) scan_bwd_maps_kernel(const ScanArgs A, co
     const SegRow s = seg_row(rr, batch, P.seg, true);
     const int64_t begin = s.q * P.seg.len;
     const int steps = static_cast<int>(min(P.seg.len, A.steps - begin));
-    float m[V], E[V];
+    Vf<V> m, E;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       m[v] = 1.f;
@@ -423,23 +412,16 @@ __global__ void __launch_bounds__(256) scan_bwd_maps_kernel(const ScanArgs A, co
             m[v] = 0.f;
           }
         }
-        float fr[V], fd[V];
-        d[j].get(fd);
+        Vf<V> fr, fd;
+        d[j].get(fd.v);
         if constexpr (CODES)
-          q[j].get(scale[j], fr);
+          q[j].get(scale[j], fr.v);
         else
-          r[j].get(fr);
-        float a[V];
-        if (!on[j]) {
-#pragma unroll
-          for (int v = 0; v < V; ++v) fr[v] = -1e30f;  // a = 1; dh is 0 beyond the last step
-        }
-        decays_of(fr, k, a);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          E[v] = a[v] * (E[v] + fd[v]);
-          m[v] *= a[v];
-        }
+          r[j].get(fr.v);
+        if (!on[j]) fr = splat<V>(-1e30f);  // a = 1; dh is 0 beyond the last step
+        const Vf<V> a = decay_of(fr, k);
+        E = a * (E + fd);
+        m = m * a;
       }
     }
 #pragma unroll

@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(256, CODES || sizeof(T) * V < 16 ? 3 : 4)
   const int64_t rows = batch * P.seg.n;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * L.rows;
   const bool masked = KIND == kMasked || (KIND == kPacked && A.mask != nullptr);
-  float k[V], h[V], m[V];
+  Vf<V> k, h, m;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     k[v] = live ? decay_factor(param_at(A.decay, A.decay_bf16, c + v), A.rate) : 0.f;
@@ -167,13 +167,13 @@ __global__ void __launch_bounds__(256, CODES || sizeof(T) * V < 16 ? 3 : 4)
           if (live && (KIND == kPlain || on[j])) w[0][s].raw = *slot(buf, j, s);
         }
       }
-      float fx[V], fr[V], fi[V];
-      w[kAt * j][0].get(fx);
-      w[kAt * j][1].get(fr);
-      w[kAt * j][2].get(fi);
+      Vf<V> fx, fr, fi;
+      w[kAt * j][0].get(fx.v);
+      w[kAt * j][1].get(fr.v);
+      w[kAt * j][2].get(fi.v);
       if constexpr (CODES) {
         Codes<V> q[3];
-        const float s0 = encode8(fx, q[0]), s1 = encode8(fr, q[1]), s2 = encode8(fi, q[2]);
+        const float s0 = encode8(fx.v, q[0]), s1 = encode8(fr.v, q[1]), s2 = encode8(fi.v, q[2]);
         if (live) {
           q[0].store(code);
           q[1].store(code + H);
@@ -195,21 +195,14 @@ __global__ void __launch_bounds__(256, CODES || sizeof(T) * V < 16 ? 3 : 4)
           m[v] = 0.f;
         }
       }
-      if (KIND != kPlain && !on[j]) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) shut(fx[v], fr[v], fi[v]);
-      }
-      Step g[V];
-      steps_of(fx, fr, fi, k, g);
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        h[v] = fmaf(g[v].a, h[v], g[v].add);
-        if (MAPS) m[v] *= g[v].a;
-      }
+      if (KIND != kPlain && !on[j]) shut(fx, fr, fi);
+      const Step<V> g = step_of(fx, fr, fi, k);
+      h = fma(g.a, h, g.add);
+      if (MAPS) m = m * g.a;
       if (!MAPS) {
         if (live) {
           Pack<T, V> o;
-          o.set(h);
+          o.set(h.v);
           o.store(out);
         }
         out += A.row_st * H;

@@ -111,7 +111,8 @@ void launch_carry(const ScanArgs& a, const ScanPlan& p, bool bwd, cudaStream_t s
 }
 
 // Rows k, k + m, k + 2m, ... of partial [n, H] added up in order into row k of out [m, H]:
-// 32 channels x 32 shares per block. `last`: out is ddecay, -c sigmoid(decay) times the sum.
+// 32 channels x 32 shares per block. `last`: out is ddecay, c sigmoid(decay) times the
+// sum (of -dz sigmoid(r)).
 __global__ void scan_decay_grad_kernel(const float* __restrict__ partial, int64_t n, int H, bool last, const void* decay,
                                        int decay_bf16, float rate, void* out) {
   __shared__ float sum[32][33];
@@ -127,7 +128,7 @@ __global__ void scan_decay_grad_kernel(const float* __restrict__ partial, int64_
   if (threadIdx.y == 0 && c < H) {
     for (int w = 1; w < 32; ++w) t += sum[w][threadIdx.x];
     if (last)
-      param_store(out, decay_bf16, c, -rate * sigmoid_f(param_at(decay, decay_bf16, c)) * t);
+      param_store(out, decay_bf16, c, rate * sigmoid_f(param_at(decay, decay_bf16, c)) * t);
     else
       static_cast<float*>(out)[static_cast<int64_t>(blockIdx.y) * H + c] = t;
   }
@@ -142,17 +143,16 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const ScanStepArgs A) {
   const int64_t row = e / A.width;
   const int c = static_cast<int>(e - row * A.width);
   const T* p = static_cast<const T*>(A.p) + row * A.p_sb + c;
-  const float x[1] = {to_f32(p[0])}, r[1] = {to_f32(p[A.width])}, i[1] = {to_f32(p[2 * static_cast<int64_t>(A.width)])};
-  const float k[1] = {decay_factor(param_at(A.decay, A.decay_bf16, c), A.rate)};
+  const Vf<1> x{{to_f32(p[0])}}, r{{to_f32(p[A.width])}}, i{{to_f32(p[2 * static_cast<int64_t>(A.width)])}};
+  const Vf<1> k{{decay_factor(param_at(A.decay, A.decay_bf16, c), A.rate)}};
   const int64_t at = A.index != nullptr ? A.index[row] : row;
   float h = 0.f;
   if (at < 0 || at >= A.table_rows) {
     record_status(A.status, kBadIndex);  // the row is left out
   } else {
     float* to = A.state + at * A.state_sb + c;
-    Step g[1];
-    steps_of(x, r, i, k, g);
-    h = fmaf(g[0].a, *to, g[0].add);
+    const Step<1> g = step_of(x, r, i, k);
+    h = fmaf(g.a[0], *to, g.add[0]);
     *to = h;
   }
   static_cast<T*>(A.h)[e] = from_f32<T>(h);

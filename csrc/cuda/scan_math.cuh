@@ -21,108 +21,189 @@
 
 namespace su {
 
-// 1 - exp(z) for V values z <= 0. Taylor's series up to z^6 where |z| <= 0.25 (remainder below
+// V channels of a thread. Pairs of them go through the packed fp32 instructions (one issue
+// slot for two products or sums, each rounded as its scalar form): the kernels of bf16 inputs
+// are bound by issue slots and the special-function unit, not by bytes.
+template <int V>
+struct Vf {
+  float v[V];
+  __device__ __forceinline__ float& operator[](int i) { return v[i]; }
+  __device__ __forceinline__ float operator[](int i) const { return v[i]; }
+};
+
+__device__ __forceinline__ void pair_fma(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0,
+                                         float c1) {
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void pair_mul(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void pair_add(float& d0, float& d1, float a0, float a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+
+template <int V>
+__device__ __forceinline__ Vf<V> splat(float x) {
+  Vf<V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = x;
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vf<V> fma(const Vf<V>& a, const Vf<V>& b, const Vf<V>& c) {
+  Vf<V> r;
+  if constexpr (V == 1) {
+    r.v[0] = fmaf(a.v[0], b.v[0], c.v[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2)
+      pair_fma(r.v[i], r.v[i + 1], a.v[i], a.v[i + 1], b.v[i], b.v[i + 1], c.v[i], c.v[i + 1]);
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vf<V> operator*(const Vf<V>& a, const Vf<V>& b) {
+  Vf<V> r;
+  if constexpr (V == 1) {
+    r.v[0] = __fmul_rn(a.v[0], b.v[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) pair_mul(r.v[i], r.v[i + 1], a.v[i], a.v[i + 1], b.v[i], b.v[i + 1]);
+  }
+  return r;
+}
+template <int V>
+__device__ __forceinline__ Vf<V> operator+(const Vf<V>& a, const Vf<V>& b) {
+  Vf<V> r;
+  if constexpr (V == 1) {
+    r.v[0] = __fadd_rn(a.v[0], b.v[0]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) pair_add(r.v[i], r.v[i + 1], a.v[i], a.v[i + 1], b.v[i], b.v[i + 1]);
+  }
+  return r;
+}
+// 1 - a
+template <int V>
+__device__ __forceinline__ Vf<V> rest_of(const Vf<V>& a) {
+  return fma(a, splat<V>(-1.f), splat<V>(1.f));
+}
+template <int V>
+__device__ __forceinline__ Vf<V> sigmoid(const Vf<V>& a) {
+  Vf<V> e = a * splat<V>(-kLog2e);
+#pragma unroll
+  for (int i = 0; i < V; ++i) e.v[i] = ex2_f(e.v[i]);
+  e = e + splat<V>(1.f);
+#pragma unroll
+  for (int i = 0; i < V; ++i) e.v[i] = rcp_f(e.v[i]);
+  return e;
+}
+
+
+// 1 - exp(-y) for V values y >= 0. Taylor's series up to y^6 where y <= 0.25 (remainder below
 // 0.25^6 / 7! = 5e-8 of the result), else the difference, which cancels at most two bits. A
 // thread whose V values are all small, the rule for a memory of many steps, branches past
 // the exponentials: the special-function unit is what bounds bf16 inputs.
 template <int V>
-__device__ __forceinline__ void one_minus_exp(const float (&z)[V], float (&em)[V]) {
-  float least = z[0];
+__device__ __forceinline__ Vf<V> one_minus_exp(const Vf<V>& y) {
+  Vf<V> t = fma(y, splat<V>(-1.f / 720.f), splat<V>(1.f / 120.f));
+  t = fma(y, t, splat<V>(-1.f / 24.f));
+  t = fma(y, t, splat<V>(1.f / 6.f));
+  t = fma(y, t, splat<V>(-0.5f));
+  t = fma(y, t, splat<V>(1.f));
+  Vf<V> em = y * t;
+  float most = y.v[0];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    float t = fmaf(z[v], 1.f / 720.f, 1.f / 120.f);
-    t = fmaf(z[v], t, 1.f / 24.f);
-    t = fmaf(z[v], t, 1.f / 6.f);
-    t = fmaf(z[v], t, 0.5f);
-    t = fmaf(z[v], t, 1.f);
-    em[v] = -z[v] * t;
-    least = fminf(least, z[v]);
-  }
-  if (least < -0.25f) {
+  for (int i = 1; i < V; ++i) most = fmaxf(most, y.v[i]);
+  if (most > 0.25f) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const float e = 1.f - ex2_f(kLog2e * z[v]);
-      em[v] = z[v] < -0.25f ? e : em[v];
+    for (int i = 0; i < V; ++i) {
+      const float e = 1.f - ex2_f(-kLog2e * y.v[i]);
+      em.v[i] = y.v[i] > 0.25f ? e : em.v[i];
     }
   }
+  return em;
 }
 
-// -c softplus(decay)
+// c softplus(decay), so that z = -k sigmoid(r)
 __device__ __forceinline__ float decay_factor(float decay, float rate) {
-  return -rate * (fmaxf(decay, 0.f) + log1pf(expf(-fabsf(decay))));
+  return rate * (fmaxf(decay, 0.f) + log1pf(expf(-fabsf(decay))));
 }
 
 // What a step maps the state with: h -> a h + add.
+template <int V>
 struct Step {
-  float a, add;
+  Vf<V> a, add;
 };
 template <int V>
-__device__ __forceinline__ void steps_of(const float (&x)[V], const float (&r)[V], const float (&i)[V],
-                                         const float (&k)[V], Step (&g)[V]) {
-  float z[V], em[V];
+__device__ __forceinline__ Step<V> step_of(const Vf<V>& x, const Vf<V>& r, const Vf<V>& i, const Vf<V>& k) {
+  const Vf<V> em = one_minus_exp(k * sigmoid(r));
+  Step<V> g;
+  g.a = rest_of(em);
+  Vf<V> s = fma(em, g.a, em);
 #pragma unroll
-  for (int v = 0; v < V; ++v) z[v] = k[v] * sigmoid_f(r[v]);
-  one_minus_exp(z, em);
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    g[v].a = 1.f - em[v];
-    g[v].add = sqrt_f(em[v] * (1.f + g[v].a)) * sigmoid_f(i[v]) * x[v];
-  }
+  for (int v = 0; v < V; ++v) s.v[v] = sqrt_f(s.v[v]);
+  g.add = s * sigmoid(i) * x;
+  return g;
 }
 template <int V>
-__device__ __forceinline__ void decays_of(const float (&r)[V], const float (&k)[V], float (&a)[V]) {
-  float z[V], em[V];
-#pragma unroll
-  for (int v = 0; v < V; ++v) z[v] = k[v] * sigmoid_f(r[v]);
-  one_minus_exp(z, em);
-#pragma unroll
-  for (int v = 0; v < V; ++v) a[v] = 1.f - em[v];
+__device__ __forceinline__ Vf<V> decay_of(const Vf<V>& r, const Vf<V>& k) {
+  return rest_of(one_minus_exp(k * sigmoid(r)));
 }
 
 // One step's gradients are products with g, the gradient at h_t: dx = g x, dr = g r,
-// di = g i, the share of ddecay's sum is g l and a g goes on to h_{t-1}. `Gate` is what the
+// di = g i, the share of ddecay's sum is -g l and a g goes on to h_{t-1}. `Gate` is what the
 // inputs alone give; the state before the step turns it into `Slope`. Each is evaluated once.
+template <int V>
 struct Gate {
-  float a, x, i, add, q, z, sr;
+  Vf<V> a, x, i, add, q, y, sr;
 };
 template <int V>
-__device__ __forceinline__ void gates_of(const float (&x)[V], const float (&r)[V], const float (&i)[V],
-                                         const float (&k)[V], Gate (&g)[V]) {
-  float z[V], em[V];
+__device__ __forceinline__ Gate<V> gate_of(const Vf<V>& x, const Vf<V>& r, const Vf<V>& i, const Vf<V>& k) {
+  Gate<V> g;
+  g.sr = sigmoid(r);
+  const Vf<V> si = sigmoid(i);
+  const Vf<V> y = k * g.sr;  // -z
+  const Vf<V> em = one_minus_exp(y);
+  g.a = rest_of(em);
+  const Vf<V> ss = fma(em, g.a, em);
+  Vf<V> rs;
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    g[v].sr = sigmoid_f(r[v]);
-    z[v] = k[v] * g[v].sr;
-  }
-  one_minus_exp(z, em);
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const float si = sigmoid_f(i[v]);
-    g[v].a = 1.f - em[v];
-    const float ss = em[v] * (1.f + g[v].a);
-    const float rs = rsqrt_f(fmaxf(ss, 1.2e-38f));  // finite where the gate is closed; s and z are 0 there
-    g[v].x = ss * rs * si;
-    g[v].add = g[v].x * x[v];
-    g[v].i = fmaf(-g[v].add, si, g[v].add);
-    g[v].q = g[v].a * rs * (si * x[v]);
-    g[v].z = fmaf(-z[v], g[v].sr, z[v]);
-  }
+  for (int v = 0; v < V; ++v) rs.v[v] = rsqrt_f(fmaxf(ss.v[v], 1.2e-38f));  // finite where the gate is closed: s, z 0
+  g.x = ss * rs * si;
+  g.add = g.x * x;
+  g.i = g.add * rest_of(si);
+  g.q = g.a * rs * (si * x);
+  g.y = y * rest_of(g.sr);
+  return g;
 }
 // Inputs of a step that leaves the state as it is: sigmoid(r) = 0, so a = 1 and s = 0.
-__device__ __forceinline__ void shut(float& x, float& r, float& i) {
-  x = 0.f;
-  r = -1e30f;
-  i = 0.f;
+template <int V>
+__device__ __forceinline__ void shut(Vf<V>& x, Vf<V>& r, Vf<V>& i) {
+  x = splat<V>(0.f);
+  r = splat<V>(-1e30f);
+  i = splat<V>(0.f);
 }
 
+template <int V>
 struct Slope {
-  float a, x, r, i, l;
+  Vf<V> a, x, r, i, l;
 };
 // at the state before the step, which moves on to h_t
-__device__ __forceinline__ Slope slope_of(const Gate& g, float& h) {
-  const float f = g.a * (h - g.q);
-  h = fmaf(g.a, h, g.add);
-  return Slope{g.a, g.x, f * g.z, g.i, f * g.sr};
+template <int V>
+__device__ __forceinline__ Slope<V> slope_of(const Gate<V>& g, Vf<V>& h) {
+  const Vf<V> f = g.a * fma(h, splat<V>(-1.f), g.q);  // -(a h - (a^2 / s) sigmoid(i) x)
+  h = fma(g.a, h, g.add);
+  return Slope<V>{g.a, g.x, f * g.y, g.i, f * g.sr};
 }
 
 }  // namespace su
