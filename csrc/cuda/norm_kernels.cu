@@ -583,11 +583,11 @@ int64_t round_count(const NormArgs& a, const Shape& s) {
 constexpr int kMostBlocks = 8;  // per SM
 // fits[block / 32]: blocks that an SM takes, asked once per kernel and block size
 template <class K>
-void run(K kernel, int (&fits)[33], const NormArgs& a, const Shape& s, size_t smem, int sms, cudaStream_t st,
+void run(K kernel, int (&fits)[33], uint64_t& allowed, const NormArgs& a, const Shape& s, size_t smem, int sms, cudaStream_t st,
          int* grid) {
+  allow_smem(kernel, smem, allowed);
   int& per_sm = fits[s.team.block / 32];
   if (per_sm == 0) {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
     int n = 1;
     cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, s.team.block, smem);
     per_sm = n < 1 ? 1 : (n > kMostBlocks ? kMostBlocks : n);
@@ -605,16 +605,17 @@ void run(K kernel, int (&fits)[33], const NormArgs& a, const Shape& s, size_t sm
 template <class T, int V, int NV, int MAXT, bool CODES, bool BWD, bool AHEAD>
 void run_case(const NormArgs& a, const Shape& s, int sms, cudaStream_t st, int* grid) {
   static int fits[33] = {};
+  static uint64_t allowed = 0;
   const size_t threads = s.team.block;
   if constexpr (BWD) {
     const size_t vecs = V == 8 ? 0 : (3 * s.team.size * NV * V + 3) / 4 * 16;
     size_t smem = vecs + (AHEAD ? threads * 2 * NV * (CODES ? 2 * sizeof(T) * V + 24 : 5 * sizeof(T) * V) : 0);
     const size_t sums = threads * NV * V * sizeof(float);
     smem = smem > sums ? smem : sums;
-    run(norm_bwd_kernel<T, V, NV, MAXT, CODES, AHEAD>, fits, a, s, smem, sms, st, grid);
+    run(norm_bwd_kernel<T, V, NV, MAXT, CODES, AHEAD>, fits, allowed, a, s, smem, sms, st, grid);
   } else {
     const size_t smem = AHEAD ? threads * 2 * NV * 3 * sizeof(T) * V : 0;
-    run(norm_fwd_kernel<T, V, NV, MAXT, CODES, AHEAD>, fits, a, s, smem, sms, st, grid);
+    run(norm_fwd_kernel<T, V, NV, MAXT, CODES, AHEAD>, fits, allowed, a, s, smem, sms, st, grid);
   }
 }
 template <class T, int V, int NV, int MAXT, bool CODES, bool BWD>

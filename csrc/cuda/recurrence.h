@@ -13,6 +13,19 @@ namespace su {
 constexpr int kStateEvery = 16;
 constexpr int kStateShort = 8;
 
+// Shared memory above the default limit, allowed once per kernel and device (`done` is the
+// launcher's own, a bit per device): the call costs as much as a small launch.
+template <class K>
+inline void allow_smem(K kernel, size_t bytes, uint64_t& done) {
+  if (bytes <= 40 * 1024) return;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done & bit) return;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024);
+  done |= bit;
+}
+
 constexpr int kGroup8 = 32;  // values of a row that share one scale in the 8-bit format
 
 // One call of the gated linear recurrence. Sequences lie in a [batch, steps] grid

@@ -448,8 +448,8 @@ void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
   const bool async = CODES ? V > 1 : sizeof(T) * V >= 4;
   const size_t smem = async ? static_cast<size_t>(threads) * Slots<T, V, CH, CODES, KIND == kPacked>::kBytes : 0;
   auto kernel = scan_bwd_kernel<T, V, CH, CODES, KIND>;
-  if (smem > 40 * 1024)
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static uint64_t allowed = 0;
+  allow_smem(kernel, smem, allowed);
   kernel<<<grid, threads, smem, st>>>(a, p, l);
 }
 

@@ -241,8 +241,8 @@ void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
   const int threads = l.count * l.rows;
   const size_t smem = sizeof(T) * V >= 16 ? static_cast<size_t>(threads) * 2 * U * 3 * sizeof(T) * V : 0;
   auto kernel = scan_fwd_kernel<T, V, U, MAPS, CODES, KIND>;
-  if (smem > 40 * 1024)
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static uint64_t allowed = 0;
+  allow_smem(kernel, smem, allowed);
   kernel<<<grid, threads, smem, st>>>(a, p, l);
 }
 
