@@ -23,7 +23,11 @@
 namespace su {
 namespace {
 
-// A team: `size` neighbouring threads (8, 16 or 32, or the whole block).
+// 8-bit codes to write: none, or of rows of at least one group of 32 or narrower ones, whose
+// group is the team
+enum { kNoCodes = 0, kWide = 1, kNarrow = 2 };
+
+// A team: `size` neighbouring threads (4 to 32, a power of two, or the whole block).
 struct Team {
   int size;
   int block;  // threads of a block
@@ -74,7 +78,7 @@ struct Slots {
   __device__ __forceinline__ Raw* slot(int buf, int w, int j) const { return at + ((buf * W + w) * NV + j) * ld; }
 };
 
-template <class T, int V, int NV, int MAXT, bool CODES, bool AHEAD>
+template <class T, int V, int NV, int MAXT, int CODES, bool AHEAD>
 __global__ void __launch_bounds__(MAXT, MAXT > 256 ? 1 : NV * V <= 8 && !CODES ? 4 : 2)
     norm_fwd_kernel(const NormArgs A, const Team M) {
   constexpr bool kAsync = AHEAD;
@@ -163,7 +167,7 @@ __global__ void __launch_bounds__(MAXT, MAXT > 256 ? 1 : NV * V <= 8 && !CODES ?
 #pragma unroll
         for (int j = 0; j < NV; ++j, code += step, scale += step / kGroup8) {
           Codes<V> q;
-          const float s = encode8(f[w][j], q);
+          const float s = encode8<CODES == kNarrow>(f[w][j], q, M.size);
           if (j < n) {
             q.store(code);
             if (c0 % kGroup8 == 0) *scale = s;  // a team is whole groups wide
@@ -376,9 +380,9 @@ __global__ void __launch_bounds__(MAXT, MAXT > 256 || NV * V > 12 ? 1 : 2)
         a.get(f[w][j]);
       }
     }
-    if (kAsync && row >= A.rows) {  // an earlier row's values: nothing of them reaches the sums
+    if (kAsync && row >= A.rows) {  // the slots hold an earlier row or nothing: the sums get zeros
 #pragma unroll
-      for (int w = 0; w < 2; ++w)
+      for (int w = 0; w < 5; ++w)
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -526,8 +530,8 @@ __global__ void norm_param_grad_kernel(const NormArgs A) {
   }
 }
 
-// How a width is laid out over threads. Teams of 8, 16 or 32 lanes (at least a whole 8-bit
-// group wide) with up to `most` vectors each where that holds the row, whichever leaves the fewest
+// How a width is laid out over threads. Teams of 4 to 32 lanes (at least a whole 8-bit group
+// wide) with up to `most` vectors each where that holds the row, whichever leaves the fewest
 // vectors idle; else the whole block, with the fewest vectors a thread that fit.
 struct Shape {
   Team team;
@@ -535,9 +539,9 @@ struct Shape {
 };
 int round_nv(int nv, int V) {  // the counts that are compiled
   if (V > 1) return nv;
-  int n = 1;
-  while (n < nv) n *= 2;
-  return n;
+  for (int n : {1, 2, 3, 4, 6, 8})
+    if (nv <= n) return n;
+  return 16;
 }
 Shape shape_of(const NormArgs& a, int V, int least, int most) {
   Shape s;
@@ -545,7 +549,10 @@ Shape shape_of(const NormArgs& a, int V, int least, int most) {
   const int vecs = (a.width + V - 1) / V;
   const bool few = a.rows < 4096;  // one short round: the fewest vectors a lane
   int best = 1 << 30;
-  for (int size = kGroup8 / V > 8 ? kGroup8 / V : 8; size <= 32; size *= 2) {
+  // with codes a lane's group is a team's, or the team whole groups wide
+  const int least_size = a.codes != nullptr ? group_lanes(a.width, V) : 1;
+  const int from = vecs > 4 ? 8 : 4;
+  for (int size = least_size > from ? least_size : from; size <= 32; size *= 2) {
     const int nv = round_nv((vecs + size - 1) / size, V);
     if (nv <= most && nv * size < best + few) {  // equal: fewer lanes, more loads each
       best = nv * size;
@@ -615,7 +622,14 @@ void run_case(const NormArgs& a, const Shape& s, int sms, cudaStream_t st, int* 
     run(norm_bwd_kernel<T, V, NV, MAXT, CODES, AHEAD>, fits, allowed, a, s, smem, sms, st, grid);
   } else {
     const size_t smem = AHEAD ? threads * 2 * NV * 3 * sizeof(T) * V : 0;
-    run(norm_fwd_kernel<T, V, NV, MAXT, CODES, AHEAD>, fits, allowed, a, s, smem, sms, st, grid);
+    constexpr int kCodes = !CODES ? kNoCodes : kWide;
+    if constexpr (CODES && NV == 1) {
+      if (a.width < kGroup8) {
+        static int narrow_fits[33] = {};
+        return run(norm_fwd_kernel<T, V, NV, MAXT, kNarrow, AHEAD>, narrow_fits, allowed, a, s, smem, sms, st, grid);
+      }
+    }
+    run(norm_fwd_kernel<T, V, NV, MAXT, kCodes, AHEAD>, fits, allowed, a, s, smem, sms, st, grid);
   }
 }
 template <class T, int V, int NV, int MAXT, bool CODES, bool BWD>
@@ -649,7 +663,9 @@ void run_norm(const NormArgs& a, int sms, cudaStream_t st, int* grid) {
   SU_NORM_CASE(4, 4, 1024)
   SU_NORM_CASE(1, 1, 256)
   SU_NORM_CASE(1, 2, 256)
+  SU_NORM_CASE(1, 3, 256)
   SU_NORM_CASE(1, 4, 256)
+  SU_NORM_CASE(1, 6, 256)
   SU_NORM_CASE(1, 8, 256)
   SU_NORM_CASE(1, 8, 1024)
   SU_NORM_CASE(1, 16, 1024)

@@ -9,11 +9,12 @@ namespace {
 constexpr int kUnroll = 4;  // rows whose loads are under way together
 
 // A group of 32 values per 32 / V lanes; every group of a row has lanes of its own.
-template <class T, int V>
+template <class T, int V, bool NARROW>
 __global__ void __launch_bounds__(256) quantize8_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int H,
                                                         int8_t* __restrict__ codes, float* __restrict__ scales,
                                                         const Lanes L) {
   const int G = (H + kGroup8 - 1) / kGroup8;
+  const int group = group_lanes(H, V);
   const int64_t step = static_cast<int64_t>(gridDim.x) * L.rows;
   for (int cb = blockIdx.y; cb < L.blocks; cb += gridDim.y)  // very long rows
     for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * L.rows + threadIdx.x / L.count; r0 < rows;
@@ -33,7 +34,7 @@ __global__ void __launch_bounds__(256) quantize8_kernel(const T* __restrict__ x,
       float f[V];
       a[j].get(f);
       Codes<V> q;
-      const float s = encode8(f, q);
+      const float s = encode8<NARROW>(f, q, group);
       if (live) {
         q.store(codes + row * H + c);
         if (c % kGroup8 == 0) scales[row * G + c / kGroup8] = s;
@@ -86,8 +87,8 @@ template <class T, int V>
 void run_quantize(const void* x, int64_t ld, int64_t rows, int width, int8_t* codes, float* scales, int sms,
                   cudaStream_t st) {
   const Lanes l = lanes_of(width, V, true, 256);
-  quantize8_kernel<T, V><<<grid_of(rows, l, sms), l.count * l.rows, 0, st>>>(static_cast<const T*>(x), ld, rows, width,
-                                                                             codes, scales, l);
+  auto kernel = width < kGroup8 ? quantize8_kernel<T, V, true> : quantize8_kernel<T, V, false>;
+  kernel<<<grid_of(rows, l, sms), l.count * l.rows, 0, st>>>(static_cast<const T*>(x), ld, rows, width, codes, scales, l);
 }
 template <class T, int V>
 void run_dequantize(const int8_t* codes, const float* scales, int64_t rows, int width, void* x, int sms,

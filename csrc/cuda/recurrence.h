@@ -62,7 +62,7 @@ struct ScanArgs {
   void* dp = nullptr;           // dense rows of 3H
   float* dh0 = nullptr;         // [batch, H] or nullptr
   float* partial = nullptr;     // [n_partial, H] per-block sums of -dz sigmoid(r)
-  int vec = 1;                  // every row of p, dh, h, dp starts on a multiple of 4 values, H % 4 == 0
+  int vec = 1;                  // 4 or 2: every row of p, dh, h, dp starts on a multiple of so many values; else 1
 };
 
 // Bytes of workspace that a call needs (16-byte aligned, no initial value).

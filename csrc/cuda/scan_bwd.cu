@@ -434,8 +434,9 @@ struct BwdShape {
 };
 // 16 steps' factors of one channel fit the registers, so do 8 of two and 4 of four
 BwdShape bwd_shape(const ScanArgs& a) {
-  if (a.offsets == nullptr && a.steps <= 4) return {a.vec ? 4 : 1, 4};
-  if (a.state_every == kStateShort || (a.offsets == nullptr && a.steps <= 8)) return {a.vec ? 2 : 1, 8};
+  const int vec = a.codes != nullptr && a.vec != 4 ? 1 : a.vec;  // codes go by words of four
+  if (a.offsets == nullptr && a.steps <= 4 && vec != 2) return {vec, 4};
+  if (a.state_every == kStateShort || (a.offsets == nullptr && a.steps <= 8)) return {vec > 1 ? 2 : 1, 8};
   return {1, kStateEvery};
 }
 Lanes bwd_lanes(const ScanArgs& a) { return lanes_of(a.width, bwd_shape(a).V, false, kBwdThreads); }
@@ -469,14 +470,21 @@ void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
 
 template <class T, bool CODES, int KIND>
 void run_maps(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
-  const Lanes l = lanes_of(a.width, a.vec ? 4 : 1, false, 256);
+  const Lanes l = lanes_of(a.width, a.codes != nullptr && a.vec != 4 ? 1 : a.vec, false, 256);
   const int64_t rows = (a.offsets != nullptr ? 1 : a.batch) * p.seg.n;
   const dim3 grid(row_blocks(rows, l, sms), l.blocks);
   const int threads = l.count * l.rows;
-  if (a.vec)
+  if (a.vec == 4) {
     scan_bwd_maps_kernel<T, 4, 4, CODES, KIND><<<grid, threads, 0, st>>>(a, p, l);
-  else
-    scan_bwd_maps_kernel<T, 1, 8, CODES, KIND><<<grid, threads, 0, st>>>(a, p, l);
+    return;
+  }
+  if constexpr (!CODES) {
+    if (a.vec == 2) {
+      scan_bwd_maps_kernel<T, 2, 8, CODES, KIND><<<grid, threads, 0, st>>>(a, p, l);
+      return;
+    }
+  }
+  scan_bwd_maps_kernel<T, 1, 8, CODES, KIND><<<grid, threads, 0, st>>>(a, p, l);
 }
 
 template <class T, bool CODES>

@@ -5,6 +5,9 @@
 namespace su {
 namespace {
 
+// 8-bit codes to write: none, or with rows of at least one group of 32 or narrower ones
+enum { kNoCodes = 0, kWide = 1, kNarrow = 2 };
+
 // U steps of one segment: a unit of work.
 struct Unit {
   int64_t q, b, begin;  // segment, sequence, the segment's first step
@@ -20,7 +23,7 @@ struct Unit {
 // registers hold one step's inputs. Where a thread has less, bf16 and odd widths, the copies'
 // instructions cost more than they hide (2 x 65,537 x 256 bf16: 73 us with, 68 without): the
 // unit's inputs are loaded together into registers.
-template <class T, int V, int U, bool MAPS, bool CODES, int KIND>
+template <class T, int V, int U, bool MAPS, int CODES, int KIND>
 __global__ void __launch_bounds__(256, CODES || sizeof(T) * V < 16 ? 3 : 4)
     scan_fwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {
   constexpr bool kAsync = sizeof(T) * V >= 16;
@@ -35,6 +38,7 @@ __global__ void __launch_bounds__(256, CODES || sizeof(T) * V < 16 ? 3 : 4)
   const int64_t batch = KIND == kPacked ? 1 : A.batch;
   const int64_t rows = batch * P.seg.n;
   const int64_t stride = static_cast<int64_t>(gridDim.x) * L.rows;
+  const int group = CODES ? group_lanes(H, V) : 1;
   const bool masked = KIND == kMasked || (KIND == kPacked && A.mask != nullptr);
   Vf<V> k, h, m;
 #pragma unroll
@@ -173,7 +177,8 @@ __global__ void __launch_bounds__(256, CODES || sizeof(T) * V < 16 ? 3 : 4)
       w[kAt * j][2].get(fi.v);
       if constexpr (CODES) {
         Codes<V> q[3];
-        const float s0 = encode8(fx.v, q[0]), s1 = encode8(fr.v, q[1]), s2 = encode8(fi.v, q[2]);
+        const float s0 = encode8<CODES == kNarrow>(fx.v, q[0], group), s1 = encode8<CODES == kNarrow>(fr.v, q[1], group),
+                    s2 = encode8<CODES == kNarrow>(fi.v, q[2], group);
         if (live) {
           q[0].store(code);
           q[1].store(code + H);
@@ -233,7 +238,7 @@ __global__ void __launch_bounds__(256, CODES || sizeof(T) * V < 16 ? 3 : 4)
   }
 }
 
-template <class T, int V, int U, bool MAPS, bool CODES, int KIND>
+template <class T, int V, int U, bool MAPS, int CODES, int KIND>
 void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
   const Lanes l = lanes_of(a.width, V, CODES, 256);
   const int64_t rows = (a.offsets != nullptr ? 1 : a.batch) * p.seg.n;
@@ -247,12 +252,13 @@ void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
 }
 
 // fp32: 192 bytes of slots a thread, four blocks an SM
-template <class T, bool MAPS, bool CODES, int KIND>
+template <class T, bool MAPS, int CODES, int KIND>
 void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
-  a.vec ? run<T, 4, 8 / static_cast<int>(sizeof(T)), MAPS, CODES, KIND>(a, p, sms, st) : run<T, 1, 8, MAPS, CODES, KIND>(a, p, sms, st);
+  if (a.vec == 2) return run<T, 2, 4, MAPS, CODES, KIND>(a, p, sms, st);
+  a.vec == 4 ? run<T, 4, 8 / static_cast<int>(sizeof(T)), MAPS, CODES, KIND>(a, p, sms, st) : run<T, 1, 8, MAPS, CODES, KIND>(a, p, sms, st);
 }
 
-template <class T, bool MAPS, bool CODES>
+template <class T, bool MAPS, int CODES>
 void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
   count_launch();
   switch (kind_of(a)) {
@@ -268,14 +274,16 @@ void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
 }  // namespace
 
 void scan_fwd_maps(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
-  a.bf16 ? run<__nv_bfloat16, true, false>(a, p, sms, st) : run<float, true, false>(a, p, sms, st);
+  a.bf16 ? run<__nv_bfloat16, true, kNoCodes>(a, p, sms, st) : run<float, true, kNoCodes>(a, p, sms, st);
 }
 
 void scan_fwd_rows(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
-  if (a.codes != nullptr)
-    a.bf16 ? run<__nv_bfloat16, false, true>(a, p, sms, st) : run<float, false, true>(a, p, sms, st);
+  if (a.codes == nullptr)
+    a.bf16 ? run<__nv_bfloat16, false, kNoCodes>(a, p, sms, st) : run<float, false, kNoCodes>(a, p, sms, st);
+  else if (a.width >= kGroup8)
+    a.bf16 ? run<__nv_bfloat16, false, kWide>(a, p, sms, st) : run<float, false, kWide>(a, p, sms, st);
   else
-    a.bf16 ? run<__nv_bfloat16, false, false>(a, p, sms, st) : run<float, false, false>(a, p, sms, st);
+    a.bf16 ? run<__nv_bfloat16, false, kNarrow>(a, p, sms, st) : run<float, false, kNarrow>(a, p, sms, st);
 }
 
 }  // namespace su

@@ -169,8 +169,8 @@ constexpr int64_t kSumRows = 64;  // above 8 times it the partial sums are added
 // of that by themselves are left whole: the second read would cost more than the idle threads.
 ScanPlan scan_plan(const ScanArgs& a, int sms, void* workspace) {
   const int64_t batch = a.offsets != nullptr ? 1 : a.batch;
-  const int64_t lanes = batch * ((a.width + (a.vec ? 3 : 0)) / (a.vec ? 4 : 1));
-  const int64_t want = static_cast<int64_t>(sms) * (a.vec && !a.bf16 ? 1024 : 768);
+  const int64_t lanes = batch * ((a.width + a.vec - 1) / a.vec);
+  const int64_t want = static_cast<int64_t>(sms) * (a.vec == 4 && !a.bf16 ? 1024 : 768);
   ScanPlan p;
   p.seg = {1, (a.steps + kStateEvery - 1) / kStateEvery * kStateEvery};
   if (lanes * 2 < want && a.steps > 4 * kStateEvery) {

@@ -17,7 +17,7 @@ struct Lanes {
 // Lanes of H channels at V per lane in blocks of up to `threads` threads; with 8-bit codes
 // every group of 32 channels gets its own aligned lanes, the last one's beyond H included.
 inline Lanes lanes_of(int width, int V, bool codes, int threads) {
-  const int unit = codes ? kGroup8 / V : 1;
+  const int unit = codes ? group_lanes(width, V) : 1;
   const int all = codes ? (width + kGroup8 - 1) / kGroup8 * unit : (width + V - 1) / V;
   Lanes l;
   l.blocks = (all + threads - 1) / threads;

@@ -143,15 +143,27 @@ __device__ __forceinline__ Scale8 scale8(float amax) {
   return s;
 }
 
-// The largest magnitude of a group that LANES neighbouring lanes hold (LANES a power of
-// two, aligned inside the warp; every lane of the group calls).
-template <int LANES>
-__device__ __forceinline__ float group_top(float top) {
+// The largest magnitude of a group that FULL neighbouring lanes hold, or with NARROW `lanes` of
+// them (powers of two, aligned inside the warp; every lane of the group calls).
+template <int FULL, bool NARROW>
+__device__ __forceinline__ float group_top(float top, int lanes) {
   const unsigned lane = threadIdx.x & 31;
-  const unsigned mask = LANES == 32 ? 0xffffffffu : (((1u << LANES) - 1u) << (lane & ~(LANES - 1u)));
+  if constexpr (!NARROW) {
+    const unsigned mask = FULL == 32 ? 0xffffffffu : (((1u << FULL) - 1u) << (lane & ~(FULL - 1u)));
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(mask, top, o));
+    for (int o = FULL / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(mask, top, o));
+  } else {
+    const unsigned mask = ((1u << lanes) - 1u) << (lane & ~(lanes - 1u));
+    for (int o = lanes / 2; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(mask, top, o));
+  }
   return top;
+}
+// Lanes that a group takes at V values each: fewer than 32 / V where the row is less than a group
+// (NARROW kernels; the others unroll their five, four or three exchanges).
+__host__ __device__ inline int group_lanes(int width, int V) {
+  int lanes = 1;
+  while (lanes < kGroup8 / V && lanes * V < width) lanes *= 2;
+  return lanes;
 }
 
 // V codes side by side, lowest address first
@@ -172,13 +184,13 @@ struct Codes {
   }
 };
 
-// codes of V values per lane; returns the group's scale
-template <int V>
-__device__ __forceinline__ float encode8(const float (&f)[V], Codes<V>& code) {
+// codes of V values per lane, `lanes` lanes a group where NARROW; returns the group's scale
+template <bool NARROW, int V>
+__device__ __forceinline__ float encode8(const float (&f)[V], Codes<V>& code, int lanes) {
   float top = fabsf(f[0]);
 #pragma unroll
   for (int i = 1; i < V; ++i) top = max_nan(top, fabsf(f[i]));
-  const Scale8 s = scale8(group_top<kGroup8 / V>(top));
+  const Scale8 s = scale8(group_top<kGroup8 / V, NARROW>(top, lanes));
   uint32_t n[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) n[i] = __float_as_uint(__fadd_rn(__fmul_rn(f[i], s.inv), 12582912.f));

@@ -34,6 +34,12 @@ bool rows_of(int n, const at::Tensor& t) {
   return t.size(-1) % n == 0;
 }
 bool rows_of_four(const at::Tensor& t) { return rows_of(4, t); }
+// 4, 2 or 1: values that rows of t, and of vectors `width` wide, start on multiples of
+int row_unit(const at::Tensor& t, int64_t width) {
+  for (int n : {4, 2})
+    if (width % n == 0 && rows_of(n, t)) return n;
+  return 1;
+}
 
 void check_param(const at::Tensor& t, const char* name, int64_t width, const at::Device& dev) {
   TORCH_CHECK(t.device() == dev, name, " must be on ", dev);
@@ -140,7 +146,7 @@ static std::vector<at::Tensor> gated_scan_fwd(const at::Tensor& p, const at::Ten
   a.p = p.data_ptr();
   a.p_sb = z.packed ? 0 : p.stride(0);
   a.p_st = p.stride(z.packed ? 0 : 1);
-  a.vec = rows_of_four(p) && z.width % 4 == 0;
+  a.vec = row_unit(p, z.width);
   const auto f32 = p.options().dtype(at::kFloat);
   at::Tensor h = dense_rows(z, z.width, time_major, p.options());
   at::Tensor last = at::empty({z.batch, z.width}, f32);
@@ -185,7 +191,7 @@ static std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptT
   const auto f32 = like.options().dtype(at::kFloat);
   const auto type = bf16 ? at::kBFloat16 : at::kFloat;
   a.bf16 = bf16;
-  a.vec = z.width % 4 == 0;
+  a.vec = z.width % 4 == 0 ? 4 : z.width % 2 == 0 ? 2 : 1;
   if (given(scales)) {
     TORCH_CHECK(like.scalar_type() == at::kChar, "gated_scan: 8-bit codes must be int8");
     a.codes = like.data_ptr<int8_t>();
@@ -195,7 +201,7 @@ static std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptT
     a.p = like.data_ptr();
     a.p_sb = z.packed ? 0 : like.stride(0);
     a.p_st = like.stride(z.packed ? 0 : 1);
-    a.vec = a.vec && rows_of_four(like);
+    a.vec = std::min(a.vec, row_unit(like, z.width));
   }
   TORCH_CHECK(states.numel() == (z.packed ? 1 : z.batch) * a.n_states * z.width, "gated_scan: kept states do not fit");
   a.states = const_cast<float*>(states.data_ptr<float>());
@@ -210,7 +216,7 @@ static std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptT
     a.dh = dh->data_ptr();
     a.dh_sb = z.packed ? 0 : dh->stride(0);
     a.dh_st = dh->stride(z.packed ? 0 : 1);
-    a.vec = a.vec && rows_of_four(*dh);
+    a.vec = std::min(a.vec, row_unit(*dh, z.width));
   }
   if (given(dlast)) {
     TORCH_CHECK(dlast->scalar_type() == at::kFloat && dlast->is_contiguous() && dlast->numel() == z.batch * z.width,

@@ -652,3 +652,24 @@ def test_codes_of_very_long_rows():
     whole = quantize8(x[: 1 << 25].view(-1, 4096))
     assert torch.equal(q.codes[0, : 1 << 25], whole.codes.view(-1))
     assert torch.equal(q.dequantize()[-35:], quantize8(x[-35:]).dequantize())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H", [1, 2, 3, 5, 6, 8, 10, 12, 17, 20, 26, 30, 34, 38])
+def test_narrow_and_even_widths(H, dtype):
+    """Rows narrower than a group of codes, and widths that are even but no multiple of four."""
+    for B, T, lens in ((3, 3, None), (4, 7, None), (2, 90, None), (3, 0, [50, 0, 41])):
+        for masked in (False, True):
+            x = scan_inputs(B, T, H, dtype, "batch", B + T + H, masked, lens)
+            got, want = run_scan(*x, "batch", "cuda"), run_scan(*x, "batch", "cpu", torch.float64)
+            for k, (a, b) in enumerate(zip(got, want)):
+                assert rel(a, b) < bound(a) * (4 if k == 3 else 1)  # ddecay: one sum a channel, whose terms may cancel
+            got = run_scan(*x, "batch", "cuda", checkpoint="int8")
+            for k, (a, b) in enumerate(zip(got, run_scan(*x, "batch", "cpu", checkpoint="int8"))):
+                assert rel(a, b) < 2 * bound(a) * (4 if k == 3 else 1)
+    for rows in (5, 5000):
+        inp = norm_inputs(rows, H, dtype, rows + H)
+        for a, b in zip(run_norm(inp, "cuda"), run_norm(inp, "cpu", torch.float64)):
+            assert rel(a, b) < bound(a)
+        for a, b in zip(run_norm(inp, "cuda", checkpoint="int8"), run_norm(inp, "cpu", checkpoint="int8")):
+            assert rel(a, b) < 2 * bound(a)
