@@ -17,16 +17,24 @@ struct Unit {
 // MAPS: composes the segment's steps into h -> A h + B and writes nothing else. Otherwise
 // walks the states from the one before the segment.
 //
-// With 16 bytes a thread and input (four fp32 channels), while a unit is worked on the inputs of
-// the next one (of the next segment behind the last) are copied into slots of shared memory
-// that belong to the thread, so loads are always under way, no barrier is needed and the
-// registers hold one step's inputs. Where a thread has less, bf16 and odd widths, the copies'
-// instructions cost more than they hide (2 x 65,537 x 256 bf16: 73 us with, 68 without): the
-// unit's inputs are loaded together into registers.
+// ASYNC, threads of four channels: while a unit is worked on the inputs of the next one (of the
+// next segment behind the last) are copied into slots of shared memory that belong to the
+// thread, so loads are always under way, no barrier is needed and the registers hold one step's
+// inputs. Otherwise the unit's inputs are loaded together into registers: threads of fewer
+// channels, and bf16 with marks or a mask, where the copies' instructions cost more than they
+// hide. Copies against registers: 200,000 x 8 x 64 bf16 166 and 180 us, 200,000 x 4 x 128 bf16
+// to 8-bit codes 370 and 451; packed 404,952 x 100 bf16 113 and 103, masked 68 x 9,528 x 30
+// fp32 (two channels) 68 and 63.
+//
+// Bound by bytes at fp32: 200,000 x 8 x 64 takes 262 us, 6.3 TB/s. With codes the encoding's
+// instructions bound it (400,000 x 4 x 128 fp32: 698 us), in bf16 the gates' as well.
+template <class T, int V, int KIND>
+constexpr bool kAsyncOf = V == 4 && (sizeof(T) == 4 || KIND == kPlain);
+
 template <class T, int V, int U, bool MAPS, int CODES, int KIND>
-__global__ void __launch_bounds__(256, CODES || sizeof(T) * V < 16 ? 3 : 4)
+__global__ void __launch_bounds__(256, !CODES && kAsyncOf<T, V, KIND> ? 4 : 3)
     scan_fwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {
-  constexpr bool kAsync = sizeof(T) * V >= 16;
+  constexpr bool kAsync = kAsyncOf<T, V, KIND>;
   using Raw = typename Pack<T, V>::Raw;
   extern __shared__ uint4 smem[];
   const int y = threadIdx.x / L.count;
@@ -244,14 +252,14 @@ void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
   const int64_t rows = (a.offsets != nullptr ? 1 : a.batch) * p.seg.n;
   const dim3 grid(row_blocks(rows, l, sms), l.blocks);
   const int threads = l.count * l.rows;
-  const size_t smem = sizeof(T) * V >= 16 ? static_cast<size_t>(threads) * 2 * U * 3 * sizeof(T) * V : 0;
+  const size_t smem = kAsyncOf<T, V, KIND> ? static_cast<size_t>(threads) * 2 * U * 3 * sizeof(T) * V : 0;
   auto kernel = scan_fwd_kernel<T, V, U, MAPS, CODES, KIND>;
   static uint64_t allowed = 0;
   allow_smem(kernel, smem, allowed);
   kernel<<<grid, threads, smem, st>>>(a, p, l);
 }
 
-// fp32: 192 bytes of slots a thread, four blocks an SM
+// four channels: 192 bytes of slots a thread, four blocks an SM
 template <class T, bool MAPS, int CODES, int KIND>
 void run(const ScanArgs& a, const ScanPlan& p, int sms, cudaStream_t st) {
   if (a.vec == 2) return run<T, 2, 4, MAPS, CODES, KIND>(a, p, sms, st);
