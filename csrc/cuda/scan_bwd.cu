@@ -351,7 +351,8 @@ __global__ void __launch_bounds__(256) scan_bwd_maps_kernel(const ScanArgs A, co
     // the first segments last: the pass that follows begins with them
     const SegRow s = seg_row(rr, batch, P.seg, true);
     const int64_t begin = s.q * P.seg.len;
-    const int steps = static_cast<int>(min(P.seg.len, A.steps - begin));
+    int steps = static_cast<int>(min(P.seg.len, A.steps - begin));
+    if (KIND == kPacked) steps = min(steps, static_cast<int>(P.seg.len) - max(0, P.reach[s.q]));
     Vf<V> m, E;
 #pragma unroll
     for (int v = 0; v < V; ++v) {

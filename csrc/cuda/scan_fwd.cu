@@ -63,6 +63,7 @@ __global__ void __launch_bounds__(256, !CODES && kAsyncOf<T, V, KIND> ? 4 : 3)
     u.begin = s.q * P.seg.len;
     u.steps = static_cast<int>(min(P.seg.len, A.steps - u.begin));
     u.t = 0;
+    if (MAPS && KIND == kPacked) u.t = max(0, P.reach[u.q]);  // that step's mark starts h and m
     return true;
   };
   Raw* const slots = reinterpret_cast<Raw*>(smem) + threadIdx.x;

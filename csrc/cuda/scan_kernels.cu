@@ -18,11 +18,12 @@ namespace {
 
 // A warp per packed sequence: marks its first and last rows (marks != nullptr, -1 before), reports
 // offsets that do not rise from 0 to `rows`, and copies what an empty sequence returns, its
-// first state or the gradient of its last (`from`, nullptr: zeros).
+// first state or the gradient of its last (`from`, nullptr: zeros). reach (see ScanPlan, -1
+// before): maxima of integers, in whatever order they come.
 __global__ void __launch_bounds__(256) scan_sequences_kernel(const int64_t* __restrict__ offsets, int64_t batch,
                                                              int64_t rows, int H, int* marks,
                                                              const float* __restrict__ from, float* __restrict__ to,
-                                                             int* status) {
+                                                             int* reach, int64_t len, bool bwd, int* status) {
   const int lane = threadIdx.x & 31;
   for (int64_t s = static_cast<int64_t>(blockIdx.x) * 8 + threadIdx.x / 32; s < batch;
        s += static_cast<int64_t>(gridDim.x) * 8) {
@@ -34,7 +35,12 @@ __global__ void __launch_bounds__(256) scan_sequences_kernel(const int64_t* __re
     if (hi == lo) {
       if (to != nullptr)
         for (int c = lane; c < H; c += 32) to[s * H + c] = from != nullptr ? from[s * H + c] : 0.f;
-    } else if (marks != nullptr && lane == 0) {
+    } else if (lane == 0) {
+      if (reach != nullptr) {
+        const int64_t at = bwd ? hi - 1 : lo, q = at / len;
+        atomicMax(reach + q, static_cast<int>(bwd ? len - 1 - (at - q * len) : at - q * len));
+      }
+      if (marks == nullptr) continue;
       const int id = static_cast<int>(s) * 4;
       if (hi - lo == 1) {
         marks[lo] = id + kMarkFirst + kMarkLast;
@@ -46,12 +52,17 @@ __global__ void __launch_bounds__(256) scan_sequences_kernel(const int64_t* __re
   }
 }
 
-void launch_sequences(const ScanArgs& a, int* marks, const float* from, float* to, cudaStream_t st) {
-  if (marks == nullptr && to == nullptr) return;
+void launch_sequences(const ScanArgs& a, const ScanPlan& p, bool bwd, cudaStream_t st) {
+  int* const marks = bwd ? nullptr : a.marks;
+  float* const to = bwd ? a.dh0 : a.last;
+  int* const reach = p.seg.n > 1 ? p.reach : nullptr;
+  if (marks != nullptr && a.steps > 0) cudaMemsetAsync(marks, 0xff, static_cast<size_t>(a.steps) * sizeof(int), st);
+  if (reach != nullptr) cudaMemsetAsync(reach, 0xff, static_cast<size_t>(p.seg.n) * sizeof(int), st);
+  if (marks == nullptr && to == nullptr && reach == nullptr) return;
   count_launch();
   const int64_t blocks = (a.batch + 7) / 8;
   scan_sequences_kernel<<<static_cast<unsigned>(blocks < 8192 ? blocks : 8192), 256, 0, st>>>(
-      a.offsets, a.batch, a.steps, a.width, marks, from, to, a.status);
+      a.offsets, a.batch, a.steps, a.width, marks, bwd ? a.dlast : a.h0, to, reach, p.seg.len, bwd, a.status);
 }
 
 // carry[q] = the state before segment q (backwards: the gradient after it), from `start` through
@@ -183,13 +194,16 @@ ScanPlan scan_plan(const ScanArgs& a, int sms, void* workspace) {
   }
   p.maps = static_cast<float2*>(workspace);
   p.carry = reinterpret_cast<float*>(p.maps + p.seg.n * batch * a.width);
+  p.reach = reinterpret_cast<int*>(p.carry + p.seg.n * batch * a.width);
   return p;
 }
 
 size_t scan_workspace(const ScanArgs& a, int sms) {
   const ScanPlan p = scan_plan(a, sms, nullptr);
   const int64_t batch = a.offsets != nullptr ? 1 : a.batch;
-  return p.seg.n > 1 ? static_cast<size_t>(p.seg.n * batch * a.width) * (sizeof(float2) + sizeof(float)) : 0;
+  if (p.seg.n == 1) return 0;
+  return static_cast<size_t>(p.seg.n * batch * a.width) * (sizeof(float2) + sizeof(float)) +
+         (a.offsets != nullptr ? static_cast<size_t>(p.seg.n) * sizeof(int) : 0);
 }
 
 int64_t scan_partials(const ScanArgs& a, int sms) {
@@ -199,10 +213,7 @@ int64_t scan_partials(const ScanArgs& a, int sms) {
 
 void launch_scan_fwd(const ScanArgs& a, int sms, void* workspace, cudaStream_t st) {
   const ScanPlan p = scan_plan(a, sms, workspace);
-  if (a.offsets != nullptr) {
-    if (a.steps > 0) cudaMemsetAsync(a.marks, 0xff, static_cast<size_t>(a.steps) * sizeof(int), st);
-    launch_sequences(a, a.marks, a.h0, a.last, st);
-  }
+  if (a.offsets != nullptr) launch_sequences(a, p, false, st);
   if (a.steps == 0 && a.offsets != nullptr) return;
   if (p.seg.n > 1) {
     scan_fwd_maps(a, p, sms, st);
@@ -213,7 +224,7 @@ void launch_scan_fwd(const ScanArgs& a, int sms, void* workspace, cudaStream_t s
 
 void launch_scan_bwd(const ScanArgs& a, int sms, void* workspace, void* ddecay, cudaStream_t st) {
   const ScanPlan p = scan_plan(a, sms, workspace);
-  if (a.offsets != nullptr) launch_sequences(a, nullptr, a.dlast, a.dh0, st);
+  if (a.offsets != nullptr) launch_sequences(a, p, true, st);
   if (p.seg.n > 1) {
     scan_bwd_maps(a, p, sms, st);
     launch_carry(a, p, true, st);

@@ -70,6 +70,10 @@ struct ScanPlan {
   Segments seg;
   float2* maps;
   float* carry;
+  // Packed sequences: a segment's map needs the steps from its last first row on only (backwards:
+  // up to its first last row), since a state starts anew there. Per segment the step that
+  // the map begins with, or -1 (backwards: the steps of a segment behind the map's).
+  int* reach;
 };
 
 ScanPlan scan_plan(const ScanArgs& a, int sms, void* workspace);
