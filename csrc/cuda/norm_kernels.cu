@@ -16,6 +16,11 @@
 // The backward pass recomputes y and both statistics from x, u and gate (or from their
 // 8-bit codes) instead of reading y: the bytes are the same and nothing that was rounded
 // to bf16 enters the gradients.
+//
+// Bound by bytes where a row fits a team inside a warp: 1,600,000 x 64 fp32 331 us forward and
+// 495 backward, 6.2 and 6.6 TB/s. Wider rows pay the block's sums and the issue of three columns'
+// gradients: 16,384 x 2048 bf16 64 and 158 us, 5.2 and 3.4 TB/s; with codes the encoding and
+// decoding: 400,000 x 172 fp32 352 and 407 us.
 #include "kernels.h"
 #include "recurrence.h"
 #include "vec_io.cuh"
@@ -245,8 +250,8 @@ __global__ void __launch_bounds__(MAXT, MAXT > 256 || NV * V > 12 ? 1 : 2)
 #pragma unroll
     for (int v = 0; v < V; ++v) gp[j][v] = gn[j][v] = gs[j][v] = 0.f;
   // The three vectors in shared memory, one copy a block: registers go to the row and its sums
-  // (8-bit 400,000 x 172: 456 -> 409 us). Lanes of 8 columns would meet in the banks there and
-  // keep theirs in registers (16,384 x 2048 bf16: 181 -> 157 us).
+  // (8-bit 400,000 x 172: 456 -> 407 us). Lanes of 8 columns would meet in the banks there and
+  // keep theirs in registers (16,384 x 2048 bf16: 181 -> 158 us).
   constexpr bool kOwn = V == 8;
   const int span = M.size * NV * V;
   float* const vecs = reinterpret_cast<float*>(smem);
@@ -607,7 +612,7 @@ void run(K kernel, int (&fits)[33], uint64_t& allowed, const NormArgs& a, const 
 
 // The next row is fetched ahead where a block or a few warps with codes to decode would wait for
 // it; teams inside a warp have enough other rows under way (1,600,000 rows of 64 fp32,
-// backward: 491 us without, 588 us with it). Copies have 4 bytes at least, and two rows of
+// backward: 495 us without, 588 us with it). Copies have 4 bytes at least, and two rows of
 // blocks above 256 threads do not fit.
 template <class T, int V, int NV, int MAXT, bool CODES, bool BWD, bool AHEAD>
 void run_case(const NormArgs& a, const Shape& s, int sms, cudaStream_t st, int* grid) {

@@ -6,10 +6,12 @@
 // A h + B, and two runs compose to (A2 A1, A2 B1 + B2): one pass over the inputs makes the
 // segments' maps, a short kernel walks the states through them, and the second pass starts
 // every segment from its state. The inputs are read twice (backwards only r and dh are),
-// which costs 7/4 of the bytes forward and 9/7 backward; nothing waits for another block.
+// which costs 7/4 of the bytes forward and 9/7 backward (packed sequences less: the maps need
+// not go behind a sequence's start); nothing waits for another block.
 // Handing the states on inside one pass instead (each tile publishing its map and gathering
-// those before it) reads once, and was no faster at any size tried: 10 to 17 us a tile went
-// by in the exchange, 1.44 against 0.86 ms forward for 1,000,000 packed rows of 100 fp32.
+// those before it) reads once, and was slower at every size tried: 10 to 17 us a tile went
+// by in the exchange, 1.44 against 0.83 ms forward for 1,000,000 packed rows of 100 fp32 with the
+// same arithmetic in both (0.56 ms now).
 // Every sum and composition has a fixed order: results are the same every run.
 #include "scan_shape.cuh"
 
@@ -146,6 +148,7 @@ __global__ void scan_decay_grad_kernel(const float* __restrict__ partial, int64_
 }
 
 // One new token per row: thread per channel, states read and written in place.
+// 600 rows of 100 channels: 2.2 us, the launch itself.
 template <class T>
 __global__ void __launch_bounds__(256) scan_step_kernel(const ScanStepArgs A) {
   const int64_t n = A.rows * A.width;
@@ -175,8 +178,9 @@ constexpr int64_t kSumRows = 64;  // above 8 times it the partial sums are added
 
 // Segments: as many as fill the SMs once with the forward kernels' threads (1024 an SM with the
 // slots of fp32 channels by four, else 768; a partly filled second round costs as much as a whole
-// one: 2 x 65,537 x 256 bf16 129 us with 768, 152 with 1024), none shorter than 2 kStateEvery; at
-// most 4096, whose states the carry kernel walks in a few microseconds. Sequences that fill half
+// one: the four passes over 2 x 65,537 x 256 bf16 293 us with 768, 303 with 1024), none shorter than
+// 2 kStateEvery; at most 4096, whose states the carry kernel walks in under 20 us (8192 for packed
+// 1,000,000 x 100 fp32: the passes 15 us less in all, the two carries 11 us more). Sequences that fill half
 // of that by themselves are left whole: the second read would cost more than the idle threads.
 ScanPlan scan_plan(const ScanArgs& a, int sms, void* workspace) {
   const int64_t batch = a.offsets != nullptr ? 1 : a.batch;

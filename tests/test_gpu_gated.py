@@ -99,6 +99,19 @@ def test_scan_packed(lens, H, masked, dtype):
     status_clear()
 
 
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("H", [6, 33, 64])
+@pytest.mark.parametrize("lens", [[32] * 9, [31, 1, 64, 33, 0, 31, 96, 1, 31], [1, 200, 32, 1, 1, 30, 160, 31]], ids=str)
+def test_scan_packed_at_segment_edges(lens, H, masked):
+    """Sequences that start, end, start one row early and end one row late where segments of 32 steps do."""
+    x = scan_inputs(len(lens), None, H, torch.float32, "batch", sum(lens) + H, masked, lens)
+    got = run_scan(*x, "batch", "cuda")
+    want = run_scan(*x, "batch", "cpu", torch.float64)
+    for a, b in zip(got, want):
+        assert rel(a, b) < bound(a)
+    status_clear()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("masked", [False, True])
 @pytest.mark.parametrize("B,T,H", [(3, 1, 5), (40, 4, 64), (9, 8, 128), (2, 16, 33), (3, 50, 100), (2, 300, 64), (1, 400, 30)])
