@@ -77,6 +77,7 @@ void launch_scan_bwd(const ScanArgs& a, int sms, void* workspace, void* ddecay, 
 // index[i] (nullptr: i) is row i's place in the table.
 struct ScanStepArgs {
   int bf16 = 0;
+  int vec = 1;  // 4: width, rows of p and of the table are multiples of four values
   int64_t rows = 0, table_rows = 0;
   int width = 0;
   float rate = 0.f;

@@ -147,29 +147,44 @@ __global__ void scan_decay_grad_kernel(const float* __restrict__ partial, int64_
   }
 }
 
-// One new token per row: thread per channel, states read and written in place.
-// 600 rows of 100 channels: 2.2 us, the launch itself.
-template <class T>
+// One new token per row: a thread per V channels, states read and written in place. 600 rows of
+// 100 channels: 2.2 us, the launch itself; 70,915 rows of 260 bf16: 61 us, 4.8 TB/s over rows of
+// the table in any order.
+template <class T, int V>
 __global__ void __launch_bounds__(256) scan_step_kernel(const ScanStepArgs A) {
-  const int64_t n = A.rows * A.width;
+  const int lanes = A.width / V;
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (e >= n) return;
-  const int64_t row = e / A.width;
-  const int c = static_cast<int>(e - row * A.width);
+  if (e >= A.rows * lanes) return;
+  const int64_t row = e / lanes;
+  const int c = static_cast<int>(e - row * lanes) * V;
   const T* p = static_cast<const T*>(A.p) + row * A.p_sb + c;
-  const Vf<1> x{{to_f32(p[0])}}, r{{to_f32(p[A.width])}}, i{{to_f32(p[2 * static_cast<int64_t>(A.width)])}};
-  const Vf<1> k{{decay_factor(param_at(A.decay, A.decay_bf16, c), A.rate)}};
+  Pack<T, V> in[3], out;
+#pragma unroll
+  for (int w = 0; w < 3; ++w) in[w].load(p + w * static_cast<int64_t>(A.width));
+  Vf<V> x, r, i, k, h;
+  in[0].get(x.v);
+  in[1].get(r.v);
+  in[2].get(i.v);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    k[v] = decay_factor(param_at(A.decay, A.decay_bf16, c + v), A.rate);
+    h[v] = 0.f;
+  }
   const int64_t at = A.index != nullptr ? A.index[row] : row;
-  float h = 0.f;
   if (at < 0 || at >= A.table_rows) {
     record_status(A.status, kBadIndex);  // the row is left out
   } else {
-    float* to = A.state + at * A.state_sb + c;
-    const Step<1> g = step_of(x, r, i, k);
-    h = fmaf(g.a[0], *to, g.add[0]);
-    *to = h;
+    auto* to = reinterpret_cast<typename Pack<float, V>::Raw*>(A.state + at * A.state_sb + c);
+    Pack<float, V> s;
+    s.raw = *to;
+    s.get(h.v);
+    const Step<V> g = step_of(x, r, i, k);
+    h = fma(g.a, h, g.add);
+    s.set(h.v);
+    *to = s.raw;
   }
-  static_cast<T*>(A.h)[e] = from_f32<T>(h);
+  out.set(h.v);
+  out.store(static_cast<T*>(A.h) + row * A.width + c);
 }
 
 constexpr int64_t kSumRows = 64;  // above 8 times it the partial sums are added up in two launches
@@ -250,14 +265,18 @@ void launch_scan_bwd(const ScanArgs& a, int sms, void* workspace, void* ddecay, 
   scan_decay_grad_kernel<<<cols, threads, 0, st>>>(from, n, a.width, true, a.decay, a.decay_bf16, a.rate, ddecay);
 }
 
+template <class T, int V>
+static void run_step(const ScanStepArgs& a, cudaStream_t st) {
+  const int64_t n = a.rows * (a.width / V);
+  scan_step_kernel<T, V><<<static_cast<unsigned>((n + 255) / 256), 256, 0, st>>>(a);
+}
+
 void launch_scan_step(const ScanStepArgs& a, cudaStream_t st) {
   count_launch();
-  const int64_t n = a.rows * a.width;
-  const unsigned blocks = static_cast<unsigned>((n + 255) / 256);
   if (a.bf16)
-    scan_step_kernel<__nv_bfloat16><<<blocks, 256, 0, st>>>(a);
+    a.vec == 4 ? run_step<__nv_bfloat16, 4>(a, st) : run_step<__nv_bfloat16, 1>(a, st);
   else
-    scan_step_kernel<float><<<blocks, 256, 0, st>>>(a);
+    a.vec == 4 ? run_step<float, 4>(a, st) : run_step<float, 1>(a, st);
 }
 
 }  // namespace su

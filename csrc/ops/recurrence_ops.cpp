@@ -338,6 +338,10 @@ at::Tensor gated_scan_step(const at::Tensor& p_in, const at::Tensor& decay, at::
   at::Tensor h = at::empty({n, H}, p.options());
   if (n == 0) return h;
   a.bf16 = p.scalar_type() == at::kBFloat16;
+  // four channels a thread once single ones would fill the SMs: 70,915 x 260 bf16 61 us against
+  // 121, and 600 x 100 fp32 2.6 against 2.2, where one thread's four gates take longer
+  const bool many = n * H > static_cast<int64_t>(num_sms(p.get_device())) * 2048;
+  a.vec = many && H % 4 == 0 && rows_of_four(p) && rows_of_four(state) ? 4 : 1;
   a.rows = n;
   a.table_rows = state.size(0);
   a.width = static_cast<int>(H);

@@ -256,6 +256,30 @@ def test_step(n, H, dtype):
     assert torch.equal(tab[:, 0], keep[:, 0]) and torch.equal(tab[:, 1 + H:], keep[:, 1 + H:])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("H", [128, 130, 132])
+def test_step_of_many_rows(H, dtype):
+    """More rows than fill the device: groups of channels a thread where the table's and p's rows allow."""
+    from starry_unigraph.ops.recurrence import gated_scan_step
+
+    torch.manual_seed(H)
+    n = 5003
+    p, decay, table = torch.randn(n, 3 * H + 4).to(dtype), torch.randn(H), torch.randn(2 * n, H + 4)
+    rows = torch.randperm(2 * n)[:n]
+    rows[7] = 2 * n  # outside the table
+    for shift in (0, 1, 4):
+        q, ref = p[:, shift:shift + 3 * H], table[:, shift:shift + H].double()
+        keep = torch.arange(n) != 7
+        want = gated_scan_step(q.double()[keep], decay.double(), ref, rows[keep])
+        got = table.cuda()
+        h = gated_scan_step(p.cuda()[:, shift:shift + 3 * H], decay.cuda(), got[:, shift:shift + H], rows.cuda())
+        assert rel(h[keep.cuda()], want) < bound(h) and rel(got[:, shift:shift + H], ref) < F32
+        assert h[7].abs().max() == 0 and torch.equal(got[:, shift + H:].cpu(), table[:, shift + H:])
+        assert torch.equal(got[:, :shift].cpu(), table[:, :shift])
+        with pytest.raises(RuntimeError, match="index out of range"):
+            status_clear()
+
+
 def test_step_reports_places_outside_the_table():
     from starry_unigraph.ops import check_status
     from starry_unigraph.ops.recurrence import gated_scan_step
