@@ -14,7 +14,7 @@ template <class T, int V, bool NARROW>
 __global__ void __launch_bounds__(256) quantize8_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int H,
                                                         int8_t* __restrict__ codes, float* __restrict__ scales,
                                                         const Lanes L) {
-  const int G = (H + kGroup8 - 1) / kGroup8;
+  const int G = groups_in(H);
   const int group = group_lanes(H, V);
   const int64_t step = static_cast<int64_t>(gridDim.x) * L.rows;
   for (int cb = blockIdx.y; cb < L.blocks; cb += gridDim.y)  // very long rows
@@ -48,7 +48,7 @@ template <class T, int V>
 __global__ void __launch_bounds__(256) dequantize8_kernel(const int8_t* __restrict__ codes,
                                                           const float* __restrict__ scales, int64_t rows, int H,
                                                           T* __restrict__ x, const Lanes L) {
-  const int G = (H + kGroup8 - 1) / kGroup8;
+  const int G = groups_in(H);
   const int64_t step = static_cast<int64_t>(gridDim.x) * L.rows;
   for (int cb = blockIdx.y; cb < L.blocks; cb += gridDim.y)  // very long rows
     for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * L.rows + threadIdx.x / L.count; r0 < rows;

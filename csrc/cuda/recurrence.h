@@ -27,6 +27,11 @@ inline void allow_smem(K kernel, size_t bytes, uint64_t& done) {
 }
 
 constexpr int kGroup8 = 32;  // values of a row that share one scale in the 8-bit format
+// groups of a row of 1 to 2^31 - 1 values
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline int groups_in(int width) { return (width - 1) / kGroup8 + 1; }
 
 // One call of the gated linear recurrence. Sequences lie in a [batch, steps] grid
 // (offsets == nullptr) or one after another on one axis of `steps` rows (packed).

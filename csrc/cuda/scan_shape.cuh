@@ -18,10 +18,11 @@ struct Lanes {
 // every group of 32 channels gets its own aligned lanes, the last one's beyond H included.
 inline Lanes lanes_of(int width, int V, bool codes, int threads) {
   const int unit = codes ? group_lanes(width, V) : 1;
-  const int all = codes ? (width + kGroup8 - 1) / kGroup8 * unit : (width + V - 1) / V;
+  // (64 bits: the lanes of 2^31 - 1 columns in whole groups are 2^31)
+  const int64_t all = codes ? static_cast<int64_t>(groups_in(width)) * unit : (width - 1) / V + 1;
   Lanes l;
-  l.blocks = (all + threads - 1) / threads;
-  l.count = (all + l.blocks - 1) / l.blocks;
+  l.blocks = static_cast<int>((all + threads - 1) / threads);
+  l.count = static_cast<int>((all + l.blocks - 1) / l.blocks);
   l.count = (l.count + unit - 1) / unit * unit;
   l.rows = threads / l.count;
   return l;
