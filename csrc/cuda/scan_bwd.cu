@@ -413,10 +413,7 @@ __global__ void __launch_bounds__(256) scan_bwd_maps_kernel(const ScanArgs A, co
         if (KIND == kPacked && mk[j] >= 0 && (mk[j] & kMarkLast)) {
           const float* from = A.dlast != nullptr ? A.dlast + static_cast<int64_t>(mk[j] >> 2) * H + c : nullptr;
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            E[v] = from != nullptr ? from[v] : 0.f;
-            m[v] = 0.f;
-          }
+          for (int v = 0; v < V; ++v) E[v] = from != nullptr ? from[v] : 0.f;
         }
         Vf<V> fr, fd;
         d[j].get(fd.v);
@@ -430,8 +427,9 @@ __global__ void __launch_bounds__(256) scan_bwd_maps_kernel(const ScanArgs A, co
         m = m * a;
       }
     }
+    const bool anew = KIND == kPacked && P.reach[s.q] >= 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v) P.maps[(s.q * batch + s.b) * H + c + v] = make_float2(m[v], E[v]);
+    for (int v = 0; v < V; ++v) P.maps[(s.q * batch + s.b) * H + c + v] = make_float2(anew ? kAnew : m[v], E[v]);
   }
 }
 

@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(256, !CODES && kAsyncOf<T, V, KIND> ? 4 : 3)
     u.begin = s.q * P.seg.len;
     u.steps = static_cast<int>(min(P.seg.len, A.steps - u.begin));
     u.t = 0;
-    if (MAPS && KIND == kPacked) u.t = max(0, P.reach[u.q]);  // that step's mark starts h and m
+    if (MAPS && KIND == kPacked) u.t = max(0, P.reach[u.q]);  // that step's mark starts h
     return true;
   };
   Raw* const slots = reinterpret_cast<Raw*>(smem) + threadIdx.x;
@@ -204,10 +204,7 @@ __global__ void __launch_bounds__(256, !CODES && kAsyncOf<T, V, KIND> ? 4 : 3)
       if (KIND == kPacked && mk[j] >= 0 && (mk[j] & kMarkFirst) && live) {
         const float* from = A.h0 != nullptr ? A.h0 + static_cast<int64_t>(mk[j] >> 2) * H + c : nullptr;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          h[v] = from != nullptr ? from[v] : 0.f;
-          m[v] = 0.f;
-        }
+        for (int v = 0; v < V; ++v) h[v] = from != nullptr ? from[v] : 0.f;
       }
       if (KIND != kPlain && !on[j]) shut(fx, fr, fi);
       const Step<V> g = step_of(fx, fr, fi, k);
@@ -229,8 +226,9 @@ __global__ void __launch_bounds__(256, !CODES && kAsyncOf<T, V, KIND> ? 4 : 3)
     }
     if (u.t + U >= u.steps && live) {
       if (MAPS) {
+        const bool anew = KIND == kPacked && P.reach[u.q] >= 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) P.maps[at + v] = make_float2(m[v], h[v]);
+        for (int v = 0; v < V; ++v) P.maps[at + v] = make_float2(anew ? kAnew : m[v], h[v]);
       } else if (KIND != kPacked && u.q == P.seg.n - 1) {
 #pragma unroll
         for (int v = 0; v < V; ++v) A.last[u.b * H + c + v] = h[v];

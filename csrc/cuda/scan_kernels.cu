@@ -84,32 +84,24 @@ __global__ void __launch_bounds__(kShareCols * kShares) scan_carry_kernel(const 
   const int64_t lo = min(n, threadIdx.y * share), hi = min(n, lo + share);
   const int64_t step = (bwd ? -1 : 1) * batch * H;
   const int64_t at = ((bwd ? n - 1 - lo : lo) * batch + b) * H + c;
-  float A = 1.f, B = 0.f;
+  float2 all = make_float2(1.f, 0.f);
   if (live) {
     const float2* m = maps + at;
 #pragma unroll 8
-    for (int64_t q = lo; q < hi; ++q, m += step) {
-      const float2 t = *m;
-      A *= t.x;
-      B = fmaf(t.x, B, t.y);
-    }
+    for (int64_t q = lo; q < hi; ++q, m += step) all = compose(all, *m);
   }
-  part[threadIdx.y][threadIdx.x] = make_float2(A, B);
+  part[threadIdx.y][threadIdx.x] = all;
   __syncthreads();
   if (!live) return;
   float h = start != nullptr ? start[b * H + c] : 0.f;
 #pragma unroll 8
-  for (int k = 0; k < static_cast<int>(threadIdx.y); ++k) {
-    const float2 t = part[k][threadIdx.x];
-    h = fmaf(t.x, h, t.y);
-  }
+  for (int k = 0; k < static_cast<int>(threadIdx.y); ++k) h = through(part[k][threadIdx.x], h);
   const float2* m = maps + at;
   float* to = carry + at;
 #pragma unroll 8
   for (int64_t q = lo; q < hi; ++q, m += step, to += step) {
-    const float2 t = *m;
     *to = h;
-    h = fmaf(t.x, h, t.y);
+    h = through(*m, h);
   }
 }
 

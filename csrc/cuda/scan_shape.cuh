@@ -73,9 +73,22 @@ struct ScanPlan {
   float* carry;
   // Packed sequences: a segment's map needs the steps from its last first row on only (backwards:
   // up to its first last row), since a state starts anew there. Per segment the step that
-  // the map begins with, or -1 (backwards: the steps of a segment behind the map's).
+  // the map begins with, or -1 (backwards: the steps of a segment behind the map's). Where there
+  // is one, the map's A is kAnew.
   int* reach;
 };
+
+// A of a map that forgets the state before it. Not 0, which products of many factors reach: 0 times
+// a NaN or an infinity is NaN, right inside a sequence, but nothing of one sequence enters another.
+constexpr float kAnew = -1.f;
+__device__ __forceinline__ float through(const float2& map, float h) {
+  return map.x == kAnew ? map.y : fmaf(map.x, h, map.y);
+}
+// the map of `first`, then `second`
+__device__ __forceinline__ float2 compose(const float2& first, const float2& second) {
+  const float a = first.x == kAnew || second.x == kAnew ? kAnew : first.x * second.x;
+  return make_float2(a, through(second, first.y));
+}
 
 ScanPlan scan_plan(const ScanArgs& a, int sms, void* workspace);
 int scan_bwd_blocks(const ScanArgs& a, const ScanPlan& p, int sms);

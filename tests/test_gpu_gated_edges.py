@@ -29,3 +29,46 @@ def test_codes_of_the_longest_rows(H):
     del q
     both = two.dequantize()
     assert torch.equal(both[0, -n:], both[1, -n:]) and torch.equal(both[0, :n], both[1, :n])
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("H,dtype", [(5, torch.float32), (6, torch.float32), (100, torch.float32), (100, torch.bfloat16)])
+def test_a_broken_history_stays_alone(H, dtype, masked, checkpoint):
+    """A NaN or an infinity in one packed history, or in a gradient that enters it, leaves every bit of the
+    others' results: histories over several segments, of one row, from edge to edge and inside a segment."""
+    from starry_unigraph.ops.recurrence import gated_scan
+
+    lens = [100, 60, 1, 0, 31, 96, 200, 10]
+    off = torch.tensor([0] + lens, device="cuda").cumsum(0)
+    n = int(off[-1])
+    g = torch.Generator(device="cuda").manual_seed(H)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    p, dh, d = r(n, 3 * H).to(dtype), r(n, H).to(dtype), r(H) - 3
+    h0, dl = r(len(lens), H), r(len(lens), H)
+    mask = None
+    if masked:
+        mask = torch.rand(n, device="cuda", generator=g) < 0.7
+        mask[off[:-1].clamp_max(n - 1)] = True
+    first, last = off[:-1].tolist(), (off[1:] - 1).tolist()
+
+    def run(p, dh, h0, dl):
+        q, s = p.clone().requires_grad_(), h0.clone().requires_grad_()
+        h, end = gated_scan(q, d, s, offsets=off, mask=mask, checkpoint=checkpoint)
+        return [h.detach(), end.detach(), *torch.autograd.grad((h, end), (q, s), (dh, dl))]
+
+    clean = run(p, dh, h0, dl)
+    for who, size in enumerate(lens):
+        for bad in (float("nan"), float("inf")):
+            args = [t.clone() for t in (p, dh, h0, dl)]
+            if size:
+                args[0][first[who], :H] = bad
+                args[1][last[who]] = bad
+            args[2][who], args[3][who] = bad, bad
+            got = run(*args)
+            for a, b in zip(got, clean):
+                keep = torch.ones(len(a), dtype=torch.bool, device="cuda")
+                keep[slice(first[who], first[who] + size) if len(a) == n else who] = False
+                assert torch.equal(a[keep], b[keep]), (who, bad)
+            own = slice(first[who], first[who] + size)
+            assert not torch.isfinite(got[0][own]).any() and not torch.isfinite(got[2][own, :H][mask[own] if masked else ...]).any()
