@@ -354,6 +354,9 @@ at::Tensor gated_scan_step(const at::Tensor& p_in, const at::Tensor& decay, at::
   a.state_sb = state.stride(0);
   a.h = h.data_ptr();
   a.status = device_status_ptr(p.get_device());
+  // autograd refuses a backward pass over a table that it saved and this overwrites (tensors of
+  // inference mode are never saved, and have no version)
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
   launch_scan_step(a, cur_stream());
   SU_LAUNCH_CHECK();
   return h;

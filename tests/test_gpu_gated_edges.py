@@ -72,3 +72,26 @@ def test_a_broken_history_stays_alone(H, dtype, masked, checkpoint):
                 assert torch.equal(a[keep], b[keep]), (who, bad)
             own = slice(first[who], first[who] + size)
             assert not torch.isfinite(got[0][own]).any() and not torch.isfinite(got[2][own, :H][mask[own] if masked else ...]).any()
+
+
+def test_autograd_sees_the_step():
+    """A table that a node saved and a step overwrote before the backward pass is refused as after any
+    write in place, through a view too. Tables of inference mode advance outside it as well."""
+    from starry_unigraph.ops.recurrence import gated_scan, gated_scan_step
+
+    torch.manual_seed(0)
+    p, tok = torch.randn(3, 5, 12, device="cuda", requires_grad=True), torch.randn(3, 12, device="cuda")
+    d, w = torch.randn(4, device="cuda"), torch.randn(3, 4, device="cuda", requires_grad=True)
+    wide = torch.randn(3, 6, device="cuda")
+    for table, rows in ((torch.randn(3, 4, device="cuda"), None), (wide[:, 1:5], torch.arange(3, device="cuda"))):
+        outs = [w * table] + ([gated_scan(p, d, table)[0]] if table.is_contiguous() else [])
+        gated_scan_step(tok, d, table, rows)
+        for out in outs:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                out.sum().backward()
+    with torch.inference_mode():
+        table = torch.randn(3, 4, device="cuda")
+    want = table.cpu().clone()
+    gated_scan_step(tok, d, table)
+    gated_scan_step(tok.cpu(), d.cpu(), want)
+    assert float((table.cpu() - want).abs().max()) < 1e-5
