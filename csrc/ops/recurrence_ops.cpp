@@ -68,7 +68,11 @@ ScanSizes scan_sizes(at::IntArrayRef shape, const OptTensor& offsets, int64_t pe
   s.width = shape.back() / per_row;
   TORCH_CHECK(s.width <= (1 << 18), "gated_scan: H above 2^18");
   s.steps = s.packed ? shape[0] : shape[1];
+  if (s.packed) TORCH_CHECK(offsets->dim() == 1, "gated_scan: offsets must be a vector of sequences + 1");
   s.batch = s.packed ? offsets->size(0) - 1 : shape[0];
+  // (the offsets' values are checked on the device, in a kernel over the sequences)
+  TORCH_CHECK(!s.packed || s.batch != 0 || s.steps == 0, "gated_scan: offsets must rise from 0 to the number of rows, ",
+              "but there are rows and no sequence");
   return s;
 }
 

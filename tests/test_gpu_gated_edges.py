@@ -95,3 +95,19 @@ def test_autograd_sees_the_step():
     gated_scan_step(tok, d, table)
     gated_scan_step(tok.cpu(), d.cpu(), want)
     assert float((table.cpu() - want).abs().max()) < 1e-5
+
+
+def test_rows_without_a_sequence_are_refused():
+    from starry_unigraph.ops.recurrence import gated_scan
+
+    p, d = torch.randn(5, 12, device="cuda", requires_grad=True), torch.randn(4, device="cuda")
+    one = torch.zeros(1, dtype=torch.long, device="cuda")
+    for keep in (None, "int8"):
+        for q in (p, p.detach()):
+            with pytest.raises(RuntimeError, match="no sequence"):
+                gated_scan(q, d, offsets=one, checkpoint=keep)
+        h, last = gated_scan(p[:0], d, offsets=one, checkpoint=keep)
+        assert h.shape == (0, 4) and last.shape == (0, 4)
+    for off in (one[:0], one[0]):
+        with pytest.raises(RuntimeError, match="offsets must be"):
+            gated_scan(p, d, offsets=off)
