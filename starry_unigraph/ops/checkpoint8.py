@@ -99,15 +99,16 @@ def quantize8(x: torch.Tensor) -> Packed8:
 
 @contextmanager
 def saved8(min_numel: int = 1 << 16):
-    """Keep the activations that autograd saves inside the block in 8 bits: float32 and
-    bfloat16 tensors of at least two dimensions and `min_numel` values that are neither
+    """Keep the activations that autograd saves inside the block in 8 bits: dense float32
+    and bfloat16 tensors of at least two dimensions and `min_numel` values that are neither
     parameters (``nn.Parameter``, frozen or not, or another leaf that requires a gradient) nor
     views of one, as the transposed weight that torch's linear saves. The recurrence's kept
     states and the scales of codes stay exact. A tensor that several nodes save is packed for
     each of them."""
 
     def pack(t: torch.Tensor):
-        if t.dtype not in (torch.float32, torch.bfloat16) or t.dim() < 2 or t.numel() < max(1, min_numel):
+        if (t.layout != torch.strided or t.dtype not in (torch.float32, torch.bfloat16) or t.dim() < 2
+                or t.numel() < max(1, min_numel)):
             return t
         owner = t if t._base is None else t._base
         if isinstance(owner, torch.nn.Parameter) or (owner.is_leaf and owner.requires_grad):

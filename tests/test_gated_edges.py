@@ -24,3 +24,16 @@ def test_saved8_leaves_weights_alone():
     g = torch.randn_like(y)
     gw, = torch.autograd.grad(y, lin.weight, g)
     torch.testing.assert_close(gw, g.t() @ quantize8(x).dequantize())
+
+
+def test_saved8_leaves_sparse_tensors_alone():
+    """A sparse adjacency has no rows to pack; its product is differentiated as without saved8."""
+    torch.manual_seed(1)
+    dense = (torch.rand(300, 300) < 0.05) * torch.randn(300, 300)
+    x = torch.randn(300, 3)
+    for adj in (dense.to_sparse(), dense.to_sparse_csr()):
+        q = x.clone().requires_grad_()
+        with saved8():
+            y = torch.sparse.mm(adj, q)
+        got, = torch.autograd.grad(y.sin().sum(), q)
+        torch.testing.assert_close(got, dense.t() @ y.detach().cos())
