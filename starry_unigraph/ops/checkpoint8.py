@@ -57,6 +57,19 @@ def _dequantize_torch(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dt
     return (codes.to(wide.dtype) * wide).to(dtype)
 
 
+_BITS = {2: torch.int16, 4: torch.int32, 8: torch.int64}
+
+
+def _hidden(t: torch.Tensor | None) -> torch.Tensor | None:
+    """The bits of t as integers, which saved-tensor hooks leave alone (the values of codes and kept
+    states must not be packed again); back by ``view(dtype)``."""
+    return None if t is None else t.view(_BITS[t.element_size()])
+
+
+def _shown(t: torch.Tensor | None, dtype: torch.dtype) -> torch.Tensor | None:
+    return None if t is None else t.view(dtype)
+
+
 @dataclass
 class Packed8:
     """8-bit codes [rows, H] and scales [rows, ceil(H / 32)] of a tensor of `shape` and `dtype`."""

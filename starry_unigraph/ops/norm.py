@@ -15,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from starry_unigraph.ops import cuda_ext
-from starry_unigraph.ops.checkpoint8 import check_checkpoint, quantize8
+from starry_unigraph.ops.checkpoint8 import _hidden, _shown, check_checkpoint, quantize8
 
 
 def _norm_torch(x, u, gate, w_post, w_pre, scale, eps):
@@ -44,17 +44,19 @@ class _NormCodes(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, u, gate, w_post, w_pre, scale, eps):
         wide = torch.float64 if x.dtype == torch.float64 else torch.float32
-        held = [None if t is None else quantize8(t).dequantize(wide) for t in (x, u, gate)]
+        held = [None if t is None else _hidden(quantize8(t).dequantize(wide)) for t in (x, u, gate)]
         ctx.save_for_backward(*held, w_post, w_pre, scale)
-        ctx.meta = (eps, x.dtype)
+        ctx.meta = (eps, x.dtype, wide)
         ctx.set_materialize_grads(False)
         return _norm_torch(x, u, gate, w_post, w_pre, scale, eps)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dn):
-        eps, dtype = ctx.meta
-        leaves = [None if t is None else t.detach().requires_grad_() for t in ctx.saved_tensors]
+        eps, dtype, wide = ctx.meta
+        saved = ctx.saved_tensors
+        saved = (*(_shown(t, wide) for t in saved[:3]), *saved[3:])
+        leaves = [None if t is None else t.detach().requires_grad_() for t in saved]
         with torch.enable_grad():
             outs = _norm_torch(*leaves, eps)
             pairs = [(o, g.to(o.dtype)) for o, g in zip(outs, (dy, dn)) if o is not None and g is not None]

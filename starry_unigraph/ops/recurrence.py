@@ -24,7 +24,7 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from starry_unigraph.ops import cuda_ext
-from starry_unigraph.ops.checkpoint8 import _dequantize_torch, _quantize_torch, check_checkpoint
+from starry_unigraph.ops.checkpoint8 import _dequantize_torch, _hidden, _quantize_torch, _shown, check_checkpoint
 
 STATE_EVERY = 16  # checkpoint="int8": steps between the fp32 states kept for the backward pass
 
@@ -78,15 +78,16 @@ class _ThroughCodes(torch.autograd.Function):
         parts = wide.reshape(-1, p.size(-1) // 3)
         codes = _dequantize_torch(*_quantize_torch(parts), parts.dtype).view(wide.shape)
         full, _ = _scan_torch(wide, decay, h0, mask, offsets, rate)
-        ctx.save_for_backward(codes, full, decay, h0, mask, offsets)
-        ctx.meta = (rate, p.dtype)
+        ctx.save_for_backward(_hidden(codes), _hidden(full), decay, _hidden(h0), mask, offsets)
+        ctx.meta = (rate, p.dtype, codes.dtype, None if h0 is None else h0.dtype)
         return h, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, dlast):
         codes, full, decay, h0, mask, offsets = ctx.saved_tensors
-        rate, dtype = ctx.meta
+        rate, dtype, wide, first_dtype = ctx.meta
+        codes, full, h0 = _shown(codes, wide), _shown(full, wide), _shown(h0, first_dtype)
         E = dlast.to(codes.dtype)
         dp, ddecay = torch.zeros_like(codes), torch.zeros_like(decay, dtype=codes.dtype)
         dh0 = E.clone()

@@ -1,9 +1,13 @@
 """Edges of the gated recurrence, the norms around a block and 8-bit activations on CPU: what
 8-bit saved tensors leave alone, values that are not finite, arguments that are refused."""
+from contextlib import nullcontext
+
 import pytest
 import torch
 
 from starry_unigraph.ops.checkpoint8 import quantize8, saved8
+from starry_unigraph.ops.norm import norm_residual
+from starry_unigraph.ops.recurrence import gated_scan
 
 
 def test_saved8_leaves_weights_alone():
@@ -37,3 +41,28 @@ def test_saved8_leaves_sparse_tensors_alone():
             y = torch.sparse.mm(adj, q)
         got, = torch.autograd.grad(y.sin().sum(), q)
         torch.testing.assert_close(got, dense.t() @ y.detach().cos())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
+@pytest.mark.parametrize("layout", ["dense", "packed", "no h0"])
+def test_codes_and_states_are_not_packed_again(layout, dtype):
+    """checkpoint="int8" inside saved8 gives the gradients that it gives outside."""
+    torch.manual_seed(2)
+    p, d, h0 = torch.randn(3, 40, 96), torch.randn(32) - 3, torch.randn(3, 32)
+    p, h0 = p.to(dtype), h0.to(dtype)
+    off = None
+    if layout == "packed":
+        p, off = p.flatten(0, 1), torch.tensor([0, 50, 50, 120])
+    x, u, g = (torch.randn(30, 40).to(dtype) for _ in range(3))
+    w = torch.randn(40)
+
+    def grads(inside):
+        a = [t.clone().requires_grad_() for t in (p, d, h0, x, u, g)]
+        with saved8(min_numel=1) if inside else nullcontext():
+            h, last = gated_scan(a[0] * 1, a[1], None if layout == "no h0" else a[2] * 1, offsets=off, checkpoint="int8")
+            y, n = norm_residual(a[3] * 1, a[4] * 1, w, w, gate=a[5] * 1, checkpoint="int8")
+        loss = h.double().sin().sum() + last.sum() + y.double().sin().sum() + n.double().cos().sum()
+        return torch.autograd.grad(loss, a, allow_unused=True)
+
+    for a, b in zip(grads(True), grads(False)):
+        assert a is b is None or torch.equal(a, b)
