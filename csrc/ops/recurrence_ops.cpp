@@ -288,6 +288,13 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
   }
 };
 
+// Nothing here carries a tangent on: refused, as a second derivative is.
+void check_no_tangent(const char* name, std::initializer_list<at::Tensor> ts) {
+  for (const auto& t : ts)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), name,
+                ": forward-mode differentiation is not supported on CUDA");
+}
+
 bool wants_grad(std::initializer_list<at::Tensor> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const auto& t : ts)
@@ -306,6 +313,7 @@ std::tuple<at::Tensor, at::Tensor> gated_scan(const at::Tensor& p_in, const at::
   const at::Tensor decay = decay_in.contiguous();
   const at::Tensor h0 = given(h0_in) ? h0_in->to(at::kFloat).contiguous() : at::Tensor();
   const bool time_major = !given(offsets) && p.stride(1) > p.stride(0);
+  check_no_tangent("gated_scan", {p, decay, h0});
   if (wants_grad({p, decay, h0})) {
     auto out = GatedScan::apply(p, decay, maybe(h0), mask, offsets, rate, time_major, keep8);
     return {out[0], out[1]};
@@ -598,6 +606,7 @@ std::tuple<OptTensor, OptTensor> norm_residual(const at::Tensor& x, const OptTen
   for (const auto& t : {u, gate})
     TORCH_CHECK(!t.defined() || (t.sizes() == x.sizes() && t.scalar_type() == x.scalar_type() && t.device() == x.device()),
                 "norm_residual: u and gate must have x's shape, type and device");
+  check_no_tangent("norm_residual", {x, u, gate, w_post, w_pre, scale});
   at::Tensor y, n;
   if (wants_grad({x, u, gate, w_post, w_pre, scale})) {
     auto out = NormResidual::apply(x, maybe(u), maybe(gate), maybe(w_post), maybe(w_pre), maybe(scale), eps, keep8);

@@ -111,3 +111,25 @@ def test_rows_without_a_sequence_are_refused():
     for off in (one[:0], one[0]):
         with pytest.raises(RuntimeError, match="offsets must be"):
             gated_scan(p, d, offsets=off)
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor among the inputs, whether or not a gradient is wanted; values outside of it as before."""
+    import torch.autograd.forward_ad as fwd
+
+    from starry_unigraph.ops.norm import norm_residual, rms_norm
+    from starry_unigraph.ops.recurrence import gated_scan
+
+    p, d, h0 = torch.randn(2, 3, 12, device="cuda"), torch.randn(4, device="cuda"), torch.randn(2, 4, device="cuda")
+    x, w = torch.randn(3, 8, device="cuda"), torch.randn(8, device="cuda")
+    calls = [(gated_scan, (p, d, h0)), (lambda *a: gated_scan(*a, checkpoint="int8"), (p, d, h0)), (rms_norm, (x, w)),
+             (lambda x, u, g, a, b, s: norm_residual(x, u, a, b, gate=g, scale=s), (x, x, x, w, w, w))]
+    for f, args in calls:
+        for grad in (False, True):
+            for k in range(len(args)):
+                with fwd.dual_level():
+                    a = [t.clone().requires_grad_(grad) for t in args]
+                    a[k] = fwd.make_dual(a[k], torch.ones_like(a[k]))
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        f(*a)
+        f(*args)
