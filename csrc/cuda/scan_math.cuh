@@ -11,7 +11,8 @@
 //   dr = dz z (1 - sigmoid(r))             ddecay = -c sigmoid(decay) sum dz sigmoid(r)
 //
 // Everything is computed in fp32. 1 - a comes from the series of 1 - exp(z) where z is
-// small, so that a close to 1 (memories of thousands of steps) loses nothing:
+// small, so that a close to 1 (memories of thousands of steps) loses nothing, and a from
+// the exponential where it is not, so that neither does an a close to 0:
 // s = sqrt((1 - a)(1 + a)). Where s^2 is 0 or subnormal (a closed gate) 1 / s is held
 // at its value for the smallest normal s^2: its product with z tends to 0.
 #pragma once
@@ -109,29 +110,38 @@ __device__ __forceinline__ Vf<V> sigmoid(const Vf<V>& a) {
 }
 
 
-// 1 - exp(-y) for V values y >= 0. Taylor's series up to y^6 where y <= 0.25 (remainder below
-// 0.25^6 / 7! = 5e-8 of the result), else the difference, which cancels at most two bits. A
-// thread whose V values are all small, the rule for a memory of many steps, branches past
-// the exponentials: the special-function unit is what bounds bf16 inputs.
+// a = exp(-y) and em = 1 - a for V values y >= 0, each to a few units of its own last place: the
+// gradients are multiples of a where it is small and of em where that is. Where y <= 0.25 em is Taylor's
+// series up to y^6 (remainder below 0.25^6 / 7! = 5e-8 of it) and a the rest, above 0.77; elsewhere a is
+// the exponential and em the rest, above 0.22. A thread whose V values are all small, the rule for
+// a memory of many steps, branches past the exponentials: the special-function unit is what
+// bounds bf16 inputs.
 template <int V>
-__device__ __forceinline__ Vf<V> one_minus_exp(const Vf<V>& y) {
+struct Decay {
+  Vf<V> a, em;
+};
+template <int V>
+__device__ __forceinline__ Decay<V> decay_from(const Vf<V>& y) {
   Vf<V> t = fma(y, splat<V>(-1.f / 720.f), splat<V>(1.f / 120.f));
   t = fma(y, t, splat<V>(-1.f / 24.f));
   t = fma(y, t, splat<V>(1.f / 6.f));
   t = fma(y, t, splat<V>(-0.5f));
   t = fma(y, t, splat<V>(1.f));
-  Vf<V> em = y * t;
+  Decay<V> d;
+  d.em = y * t;
+  d.a = rest_of(d.em);
   float most = y.v[0];
 #pragma unroll
   for (int i = 1; i < V; ++i) most = fmaxf(most, y.v[i]);
   if (most > 0.25f) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float e = 1.f - ex2_f(-kLog2e * y.v[i]);
-      em.v[i] = y.v[i] > 0.25f ? e : em.v[i];
+      const float e = ex2_f(-kLog2e * y.v[i]);
+      d.a.v[i] = y.v[i] > 0.25f ? e : d.a.v[i];
+      d.em.v[i] = y.v[i] > 0.25f ? 1.f - e : d.em.v[i];
     }
   }
-  return em;
+  return d;
 }
 
 // c softplus(decay), so that z = -k sigmoid(r)
@@ -146,10 +156,10 @@ struct Step {
 };
 template <int V>
 __device__ __forceinline__ Step<V> step_of(const Vf<V>& x, const Vf<V>& r, const Vf<V>& i, const Vf<V>& k) {
-  const Vf<V> em = one_minus_exp(k * sigmoid(r));
+  const Decay<V> d = decay_from(k * sigmoid(r));
   Step<V> g;
-  g.a = rest_of(em);
-  Vf<V> s = fma(em, g.a, em);
+  g.a = d.a;
+  Vf<V> s = fma(d.em, d.a, d.em);
 #pragma unroll
   for (int v = 0; v < V; ++v) s.v[v] = sqrt_f(s.v[v]);
   g.add = s * sigmoid(i) * x;
@@ -157,7 +167,7 @@ __device__ __forceinline__ Step<V> step_of(const Vf<V>& x, const Vf<V>& r, const
 }
 template <int V>
 __device__ __forceinline__ Vf<V> decay_of(const Vf<V>& r, const Vf<V>& k) {
-  return rest_of(one_minus_exp(k * sigmoid(r)));
+  return decay_from(k * sigmoid(r)).a;
 }
 
 // One step's gradients are products with g, the gradient at h_t: dx = g x, dr = g r,
@@ -173,9 +183,9 @@ __device__ __forceinline__ Gate<V> gate_of(const Vf<V>& x, const Vf<V>& r, const
   g.sr = sigmoid(r);
   const Vf<V> si = sigmoid(i);
   const Vf<V> y = k * g.sr;  // -z
-  const Vf<V> em = one_minus_exp(y);
-  g.a = rest_of(em);
-  const Vf<V> ss = fma(em, g.a, em);
+  const Decay<V> d = decay_from(y);
+  g.a = d.a;
+  const Vf<V> ss = fma(d.em, d.a, d.em);
   Vf<V> rs;
 #pragma unroll
   for (int v = 0; v < V; ++v) rs.v[v] = rsqrt_f(fmaxf(ss.v[v], 1.2e-38f));  // finite where the gate is closed: s, z 0

@@ -133,3 +133,52 @@ def test_forward_mode_is_refused():
                     with pytest.raises(RuntimeError, match="forward-mode"):
                         f(*a)
         f(*args)
+
+
+@pytest.mark.parametrize("decay", [-9.0, -3.0, 0.0, 2.0, 3.0, 4.0, 5.0])
+@pytest.mark.parametrize("batch,steps", [(2, 2000), (4000, 8)])
+def test_gradients_of_fast_and_slow_decays(batch, steps, decay):
+    """dr, ddecay and dh0 are multiples of a = exp(-y): they keep their relative precision channel by channel
+    where a is small too. y, in the middle 4 softplus(decay), comes from the exponential and the reciprocal
+    of a sigmoid (2^-22 and 2^-23 at most), softplus and three products (2^-24 each), 2^-22 of it taken
+    together, and a loses as much as y does: y 2^-22 beside the fp32 bound. A dr holds the difference of
+    two terms: twice that at the median; ddecay goes by the sum of its terms' magnitudes. A slow channel's
+    state gathers the errors of hundreds of steps: four times the fp32 bound."""
+    from starry_unigraph.ops.recurrence import gated_scan
+
+    g = torch.Generator().manual_seed(int(decay) + batch)
+    H = 8
+    p, dh = torch.randn(batch, steps, 3 * H, generator=g), torch.randn(batch, steps, H, generator=g)
+    d, h0 = torch.full((H,), decay), torch.randn(batch, H, generator=g)
+
+    def run(device, dtype):
+        a = [t.to(device, dtype).requires_grad_() for t in (p, d, h0)]
+        return [t.double().cpu() for t in torch.autograd.grad(gated_scan(*a)[0], a, dh.to(device, dtype))]
+
+    (gp, gd, g0), (wp, wd, w0) = run("cuda", torch.float32), run("cpu", torch.float64)
+    r, soft = p[..., H:2 * H].double(), torch.nn.functional.softplus(d.double())
+    tol = F32 * (4 if decay < 0 else 1) + 4 * float(soft[0]) * 2.0 ** -22
+    dr, wr = gp[..., H:2 * H], wp[..., H:2 * H]
+    assert ((dr - wr).abs() / wr.abs()).flatten(0, 1).median(0).values.max() < 2 * tol
+    terms = wr / (soft * (1 - torch.sigmoid(r))) * torch.sigmoid(d.double())  # -dz c sigmoid(r) sigmoid(decay)
+    torch.testing.assert_close(terms.sum((0, 1)), wd, rtol=1e-9, atol=1e-9 * float(terms.abs().sum()))
+    assert ((gd - wd).abs() / terms.abs().sum((0, 1))).max() < tol
+    assert ((g0 - w0).norm(dim=0) / w0.norm(dim=0)).max() < tol
+
+
+def test_small_decays_reach_the_first_state():
+    """dh0 after one step is a dh: precise relative to itself down to a near 2^-80, 0 below fp32's normal
+    numbers. Softplus (2^-23), its product with the rate and the exponent's (2^-24 each) and the
+    constant are off by less than 2^-21 of y together, the exponential and its product by 2^-22 each."""
+    from starry_unigraph.ops.recurrence import gated_scan
+
+    y = torch.tensor([1e-30, 1e-6, 0.2, 0.25, 0.26, 1, 5, 10, 17, 20, 40, 55, 100])  # -log a at an open gate
+    H = len(y)
+    p = torch.zeros(1, 1, 3 * H)
+    p[..., H:2 * H] = 200.0  # sigmoid(r) = 1
+    decay = torch.where(y > 15, y, torch.log(torch.expm1(y.double())).float())  # softplus(decay) = y
+    h0 = torch.ones(1, H, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(gated_scan(p.cuda(), decay.cuda(), h0, rate=1.0)[0].sum(), h0)
+    want = torch.exp(-torch.nn.functional.softplus(decay.double()))
+    want[want < 2.0 ** -126] = 0
+    assert ((g.double().cpu()[0] - want).abs() <= (2.0 ** -21 + 2.0 ** -21 * y.double()) * want).all()
