@@ -293,9 +293,14 @@ __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs
           held.d[j].get(dy.v);
         }
         const Vf<V> g = dy + E;
-        const Vf<V> dx = g * f[j].x, dr = g * f[j].r, di = g * f[j].i;
-        dl = fma(g, f[j].l, dl);
-        E = g * f[j].a;
+        Vf<V> dx = g * f[j].x, dr = g * f[j].r, di = g * f[j].i;
+        if (WHOLE || (on >> j & 1)) {
+          dl = fma(g, f[j].l, dl);
+          E = g * f[j].a;
+        } else {  // the factors are 0 times the state, and g need not be finite either
+          dx = dr = di = splat<V>(0.f);
+          E = g;
+        }
         Pack<T, V> o;
         o.set(dx.v);
         o.store(out);

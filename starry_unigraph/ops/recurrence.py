@@ -57,8 +57,11 @@ def _scan_torch(p, decay, h0, mask, offsets, rate):
                       torch.zeros_like(z)) * torch.sigmoid(i) * x
     outs = []
     for t in range(p.size(1)):
-        new = a[:, t] * h + add[:, t]
-        h = new if mask is None else torch.where(mask[:, t].unsqueeze(-1), new, h)
+        if mask is None:
+            h = a[:, t] * h + add[:, t]
+        else:  # a step that does not count gives no gradient, whatever the state holds
+            on = mask[:, t].unsqueeze(-1)
+            h = torch.where(on, a[:, t] * torch.where(on, h, torch.zeros_like(h)) + add[:, t], h)
         outs.append(h)
     out = torch.stack(outs, 1) if outs else x
     return out.to(p.dtype), h

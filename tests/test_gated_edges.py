@@ -66,3 +66,30 @@ def test_codes_and_states_are_not_packed_again(layout, dtype):
 
     for a, b in zip(grads(True), grads(False)):
         assert a is b is None or torch.equal(a, b)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_masked_steps_get_no_gradient_whatever_the_state(checkpoint):
+    """A sequence without a valid step whose first state is NaN or infinite, and one whose state becomes so,
+    with gradients at h that are not finite there: zeros at the masked steps, the decay's sum untouched by them."""
+    torch.manual_seed(3)
+    for bad in (float("nan"), float("inf")):
+        p, d, h0 = torch.randn(3, 20, 12), torch.randn(4), torch.randn(3, 4)
+        mask = torch.rand(3, 20) < 0.5
+        mask[1], mask[2, 9], mask[2, 10:] = False, True, False
+        h0[1] = bad
+        a = [t.clone().requires_grad_() for t in (p, d, h0)]
+        gh = torch.randn(3, 20, 4)
+        gh[1] = bad
+        h, _ = gated_scan(*a, mask=mask, checkpoint=checkpoint)
+        dp, dd, d0 = torch.autograd.grad(h, a, gh)
+        assert torch.equal(dp[~mask], torch.zeros_like(dp[~mask]))
+        b = [t.clone().requires_grad_() for t in (p[[0, 2]], d, h0[[0, 2]])]
+        want = torch.autograd.grad(gated_scan(*b, mask=mask[[0, 2]], checkpoint=checkpoint)[0], b, gh[[0, 2]])
+        for x, y in zip((dp[[0, 2]], dd, d0[[0, 2]]), want):
+            torch.testing.assert_close(x, y)
+        assert torch.equal(h[1].detach().nan_to_num(1.0, 2.0), torch.full((20, 4), bad).nan_to_num(1.0, 2.0))
+        p[2, 9, :4] = bad  # the state of the steps behind it
+        a = [t.clone().requires_grad_() for t in (p, d)]
+        dp, = torch.autograd.grad(gated_scan(*a, h0, mask=mask, checkpoint=checkpoint)[0].sum(), a[:1])
+        assert torch.equal(dp[~mask], torch.zeros_like(dp[~mask]))

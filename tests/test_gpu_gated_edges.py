@@ -182,3 +182,42 @@ def test_small_decays_reach_the_first_state():
     want = torch.exp(-torch.nn.functional.softplus(decay.double()))
     want[want < 2.0 ** -126] = 0
     assert ((g.double().cpu()[0] - want).abs() <= (2.0 ** -21 + 2.0 ** -21 * y.double()) * want).all()
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("layout", ["time", "batch", "packed"])
+@pytest.mark.parametrize("steps,H", [(3, 8), (20, 4), (20, 6), (90, 5), (300, 100)])
+def test_masked_steps_get_no_gradient_whatever_the_state(steps, H, layout, checkpoint):
+    """A sequence without a valid step whose first state is NaN or infinite, and one whose state becomes so,
+    with gradients at h that are not finite there: zeros at the masked steps, no share in the decay's sum."""
+    from starry_unigraph.ops.recurrence import gated_scan
+
+    g = torch.Generator(device="cuda").manual_seed(steps + H)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    B, T = 3, steps
+    p, d, h0, gh = r(B, T, 3 * H), r(H) - 3, r(B, H), r(B, T, H)
+    mask = torch.rand(B, T, device="cuda", generator=g) < 0.5
+    mask[1], mask[2, T // 2], mask[2, T // 2 + 1:] = False, True, False
+    off = torch.arange(B + 1, device="cuda") * T if layout == "packed" else None
+
+    def run(p, h0, gh):
+        a = [p.clone().requires_grad_(), d.clone().requires_grad_(), h0.clone().requires_grad_()]
+        q, m, e = a[0], mask, gh
+        if layout == "time":
+            q, m, e = (t.transpose(0, 1).contiguous().transpose(0, 1) for t in (q, m, e))
+        if layout == "packed":
+            q, m, e = (t.flatten(0, 1) for t in (q, m, e))
+        h, _ = gated_scan(q, a[1], a[2], mask=m, offsets=off, checkpoint=checkpoint)
+        return [h.detach().reshape(B, T, H), *torch.autograd.grad(h, a, e)]
+
+    clean = run(p, h0, gh.clone().index_fill_(0, torch.tensor([1], device="cuda"), 0.0))
+    for bad in (float("nan"), float("inf")):
+        h1, g1, p1 = h0.clone(), gh.clone(), p.clone()
+        h1[1], g1[1] = bad, bad
+        h, dp, dd, d0 = run(p, h1, g1)
+        assert torch.equal(dp[~mask], torch.zeros_like(dp[~mask])) and torch.equal(dp, clean[1])
+        assert torch.equal(dd, clean[2]) and torch.equal(d0[[0, 2]], clean[3][[0, 2]])
+        assert not torch.isfinite(h[1]).any() and not torch.isfinite(d0[1]).any()
+        p1[2, T // 2, :H] = bad  # the state of the steps behind it
+        dp = run(p1, h0, gh)[1]
+        assert torch.equal(dp[~mask], torch.zeros_like(dp[~mask]))
