@@ -198,23 +198,30 @@ static std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptT
   a.vec = z.width % 4 == 0 ? 4 : z.width % 2 == 0 ? 2 : 1;
   if (given(scales)) {
     TORCH_CHECK(like.scalar_type() == at::kChar, "gated_scan: 8-bit codes must be int8");
+    TORCH_CHECK(scales->device() == dev && scales->numel() == like.numel() / (3 * z.width) * 3 * groups_of(z.width),
+                "gated_scan: scales do not fit the 8-bit codes");
     a.codes = like.data_ptr<int8_t>();
     a.scales = scales->data_ptr<float>();
   } else {
     TORCH_CHECK(like.scalar_type() == type, "gated_scan: p must have the type of h");
+    TORCH_CHECK(unit_last(like), "gated_scan: p must have unit stride along its last dimension");
     a.p = like.data_ptr();
     a.p_sb = z.packed ? 0 : like.stride(0);
     a.p_st = like.stride(z.packed ? 0 : 1);
     a.vec = std::min(a.vec, row_unit(like, z.width));
   }
-  TORCH_CHECK(states.numel() == (z.packed ? 1 : z.batch) * a.n_states * z.width, "gated_scan: kept states do not fit");
+  TORCH_CHECK(states.device() == dev && states.is_contiguous() &&
+                  states.numel() == (z.packed ? 1 : z.batch) * a.n_states * z.width,
+              "gated_scan: kept states do not fit");
   a.states = const_cast<float*>(states.data_ptr<float>());
   if (z.packed) {
-    TORCH_CHECK(given(marks) && marks->numel() == z.steps, "gated_scan: packed sequences need the forward's marks");
+    TORCH_CHECK(given(marks) && marks->device() == dev && marks->is_contiguous() && marks->numel() == z.steps,
+                "gated_scan: packed sequences need the forward's marks");
     a.marks = marks->data_ptr<int>();
   }
   if (given(dh)) {
     TORCH_CHECK(dh->device() == dev && dh->scalar_type() == type && dh->dim() == like.dim() &&
+                    dh->sizes().slice(0, like.dim() - 1) == like.sizes().slice(0, like.dim() - 1) &&
                     dh->size(-1) == z.width && unit_last(*dh),
                 "gated_scan: the gradient of h must have its type, shape and unit last stride");
     a.dh = dh->data_ptr();
@@ -223,7 +230,8 @@ static std::vector<at::Tensor> gated_scan_bwd(const at::Tensor& like, const OptT
     a.vec = std::min(a.vec, row_unit(*dh, z.width));
   }
   if (given(dlast)) {
-    TORCH_CHECK(dlast->scalar_type() == at::kFloat && dlast->is_contiguous() && dlast->numel() == z.batch * z.width,
+    TORCH_CHECK(dlast->device() == dev && dlast->scalar_type() == at::kFloat && dlast->is_contiguous() &&
+                    dlast->numel() == z.batch * z.width,
                 "gated_scan: the gradient of the last state must be contiguous float32");
     a.dlast = dlast->data_ptr<float>();
   }
@@ -257,6 +265,14 @@ at::Tensor shown(const at::Tensor& t) { return t.defined() ? t.view(at::kFloat) 
 OptTensor maybe(const at::Tensor& t) { return t.defined() ? OptTensor(t) : c10::nullopt; }
 at::Tensor value(const OptTensor& t) { return given(t) ? *t : at::Tensor(); }
 
+// What was saved comes back from a user's saved-tensor hooks with its values, but in any layout (pinned
+// copies on the host are contiguous).
+at::Tensor plain(const at::Tensor& t) { return t.defined() ? t.contiguous() : t; }
+// dense rows in the order of the layout (see dense_rows)
+at::Tensor dense(const at::Tensor& t, bool time_major) {
+  return time_major && t.defined() ? t.transpose(0, 1).contiguous().transpose(0, 1) : plain(t);
+}
+
 void check_once(const char* name) {
   TORCH_CHECK(!at::GradMode::is_enabled(), name, ": its gradient cannot be differentiated again (create_graph)");
 }
@@ -279,10 +295,14 @@ struct GatedScan : public torch::autograd::Function<GatedScan> {
     const auto v = ctx->get_saved_variables();
     at::Tensor dh = grads[0], dlast = grads[1];
     if (dh.defined() && !unit_last(dh)) dh = dh.contiguous();
-    if (dlast.defined()) dlast = dlast.contiguous();
-    auto g = gated_scan_bwd(v[0], maybe(shown(v[1])), shown(v[2]), v[3], maybe(shown(v[4])), maybe(v[5]), maybe(v[6]),
-                            maybe(v[7]), maybe(dh), maybe(dlast), ctx->saved_data["rate"].toDouble(),
-                            ctx->saved_data["time_major"].toBool(), ctx->saved_data["bf16"].toBool(),
+    dlast = plain(dlast);
+    const bool time_major = ctx->saved_data["time_major"].toBool();
+    const bool keep8 = v[1].defined();
+    const at::Tensor in = keep8 ? dense(v[0], time_major) : unit_last(v[0]) ? v[0] : v[0].contiguous();
+    auto g = gated_scan_bwd(in, maybe(shown(dense(v[1], time_major))), shown(plain(v[2])), plain(v[3]),
+                            maybe(shown(plain(v[4]))), maybe(v[5]), maybe(plain(v[6])), maybe(plain(v[7])), maybe(dh),
+                            maybe(dlast), ctx->saved_data["rate"].toDouble(), time_major,
+                            ctx->saved_data["bf16"].toBool(),
                             v[4].defined() && ctx->needs_input_grad(2));  // p, decay, h0: the tensors given
     return {g[0], g[1], g[2], {}, {}, {}, {}, {}};
   }
@@ -472,7 +492,9 @@ static std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const OptT
   a.vec8 = H % 8 == 0;
   bool has_u, has_gate;
   if (given(scales)) {
-    TORCH_CHECK(x.scalar_type() == at::kChar && x.dim() == 3, "norm_residual: malformed 8-bit inputs");
+    TORCH_CHECK(x.scalar_type() == at::kChar && x.dim() == 3 && x.is_contiguous() && scales->device() == x.device() &&
+                    scales->is_contiguous() && scales->numel() == x.size(0) * x.size(1) * groups_of(H),
+                "norm_residual: malformed 8-bit inputs");
     a.codes = x.data_ptr<int8_t>();
     a.scales = scales->data_ptr<float>();
     a.x = x.data_ptr();
@@ -481,7 +503,7 @@ static std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const OptT
     if (has_u) a.u = a.x;  // only whether they exist is read
     if (has_gate) a.gate = a.x;
   } else {
-    TORCH_CHECK(x.scalar_type() == type && x.dim() == 2, "norm_residual: x must have the type of y");
+    TORCH_CHECK(x.scalar_type() == type && x.dim() == 2 && unit_last(x), "norm_residual: x must have the type of y");
     a.x = x.data_ptr();
     a.x_ld = x.stride(0);
     a.vec = a.vec && rows_of_four(x);
@@ -489,12 +511,14 @@ static std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const OptT
     has_u = given(u);
     has_gate = given(gate);
     if (has_u) {
+      check_rows(*u, "norm_residual: u", x);
       a.u = u->data_ptr();
       a.u_ld = u->stride(0);
       a.vec = a.vec && rows_of_four(*u);
       a.vec8 = a.vec8 && rows_of(8, *u);
     }
     if (has_gate) {
+      check_rows(*gate, "norm_residual: gate", x);
       a.gate = gate->data_ptr();
       a.gate_ld = gate->stride(0);
       a.vec = a.vec && rows_of_four(*gate);
@@ -503,7 +527,8 @@ static std::vector<at::Tensor> norm_residual_bwd(const at::Tensor& x, const OptT
   }
   auto grad = [&](const OptTensor& t, const void*& ptr, int64_t& ld) {
     if (!given(t)) return;
-    TORCH_CHECK(t->scalar_type() == type && t->dim() == 2 && t->size(0) == a.rows && t->size(1) == H && unit_last(*t),
+    TORCH_CHECK(t->device() == x.device() && t->scalar_type() == type && t->dim() == 2 && t->size(0) == a.rows &&
+                    t->size(1) == H && unit_last(*t),
                 "norm_residual: gradients must have the type and shape of the outputs and unit last stride");
     ptr = t->data_ptr();
     ld = t->stride(0);
@@ -584,8 +609,8 @@ struct NormResidual : public torch::autograd::Function<NormResidual> {
     const bool has_y = ctx->saved_data["has_y"].toBool();
     const at::Tensor dy = has_y ? grads[0] : at::Tensor();
     const at::Tensor dn = has_y ? (grads.size() > 1 ? grads[1] : at::Tensor()) : grads[0];
-    auto g = norm_residual_bwd(keep8 ? v[0] : as_rows(v[0], H), maybe(as_rows(v[1], H)), maybe(as_rows(v[2], H)),
-                               maybe(shown(v[3])), maybe(v[4]), maybe(v[5]), maybe(v[6]),
+    auto g = norm_residual_bwd(keep8 ? plain(v[0]) : as_rows(v[0], H), maybe(as_rows(v[1], H)), maybe(as_rows(v[2], H)),
+                               maybe(shown(plain(v[3]))), maybe(plain(v[4])), maybe(plain(v[5])), maybe(plain(v[6])),
                                ctx->saved_data["eps"].toDouble(), maybe(as_rows(dy, H)), maybe(as_rows(dn, H)),
                                ctx->saved_data["bf16"].toBool());
     return {like_shape(g[0], shape), like_shape(g[1], shape), like_shape(g[2], shape), g[3], g[4], g[5], {}, {}};

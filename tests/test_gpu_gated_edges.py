@@ -221,3 +221,40 @@ def test_masked_steps_get_no_gradient_whatever_the_state(steps, H, layout, check
         p1[2, T // 2, :H] = bad  # the state of the steps behind it
         dp = run(p1, h0, gh)[1]
         assert torch.equal(dp[~mask], torch.zeros_like(dp[~mask]))
+
+
+def _turned(t):
+    """The same values with the last two dimensions' memory exchanged, as a hook may bring a tensor back."""
+    return t.transpose(-1, -2).contiguous().transpose(-1, -2) if t.dim() > 1 else t
+
+
+@pytest.mark.parametrize("hooks", ["pinned", "contiguous", "turned"])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("layout", ["time", "batch", "packed"])
+def test_saved_tensors_come_back_in_any_layout(layout, checkpoint, hooks):
+    """Saved-tensor hooks that move the saved tensors to the host or give them other strides change no bit."""
+    from contextlib import nullcontext
+
+    from starry_unigraph.ops.norm import norm_residual
+    from starry_unigraph.ops.recurrence import gated_scan
+
+    torch.manual_seed(0)
+    p, d, h0 = torch.randn(40, 30, 108, device="cuda"), torch.randn(36, device="cuda"), torch.randn(40, 36, device="cuda")
+    x, w = torch.randn(30, 40, 36, device="cuda"), torch.randn(36, device="cuda")
+    off = torch.arange(0, 1201, 30, device="cuda") if layout == "packed" else None
+    graph = torch.autograd.graph
+    made = {"pinned": lambda: graph.save_on_cpu(pin_memory=True),
+            "contiguous": lambda: graph.saved_tensors_hooks(lambda t: t.contiguous().clone(), lambda t: t),
+            "turned": lambda: graph.saved_tensors_hooks(_turned, lambda t: t)}[hooks]
+
+    def grads(ctx):
+        a = [t.clone().requires_grad_() for t in (p, d, h0, x, w)]
+        with ctx:
+            q = a[0] if layout == "batch" else a[0].flatten(0, 1) if layout == "packed" else \
+                a[0].transpose(0, 1).contiguous().transpose(0, 1)
+            h, last = gated_scan(q, a[1], a[2], offsets=off, checkpoint=checkpoint)
+            y, n = norm_residual(a[3], a[3].sin(), a[4], a[4], gate=a[3].cos(), scale=a[4], checkpoint=checkpoint)
+        return torch.autograd.grad(h.square().sum() + last.sum() + y.square().sum() + n.sin().sum(), a)
+
+    for a, b in zip(grads(made()), grads(nullcontext())):
+        assert torch.equal(a, b)
