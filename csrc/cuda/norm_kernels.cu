@@ -593,12 +593,23 @@ int64_t round_count(const NormArgs& a, const Shape& s) {
 }
 
 constexpr int kMostBlocks = 8;  // per SM
-// fits[block / 32]: blocks that an SM takes, asked once per kernel and block size
+// Blocks that an SM takes, asked once per kernel and team: block size and shared memory go by the
+// team (8-bit backward pass, fp32: 88 KB and two blocks with teams of 16 in blocks of 256, 123 KB and
+// one block with a team of 256), and so must the grid, whose blocks are the vectors' partial sums.
+struct Fits {
+  int of[39] = {};  // teams of 4 to 32 lanes in larger blocks, then teams of 32 k that are blocks
+  int& at(const Team& t) {
+    if (t.size == t.block) return of[6 + t.size / 32];
+    int k = 0;
+    while (1 << k < t.size) ++k;
+    return of[k];
+  }
+};
 template <class K>
-void run(K kernel, int (&fits)[33], uint64_t& allowed, const NormArgs& a, const Shape& s, size_t smem, int sms, cudaStream_t st,
+void run(K kernel, Fits& fits, uint64_t& allowed, const NormArgs& a, const Shape& s, size_t smem, int sms, cudaStream_t st,
          int* grid) {
   allow_smem(kernel, smem, allowed);
-  int& per_sm = fits[s.team.block / 32];
+  int& per_sm = fits.at(s.team);
   if (per_sm == 0) {
     int n = 1;
     cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, s.team.block, smem);
@@ -616,7 +627,7 @@ void run(K kernel, int (&fits)[33], uint64_t& allowed, const NormArgs& a, const 
 // blocks above 256 threads do not fit.
 template <class T, int V, int NV, int MAXT, bool CODES, bool BWD, bool AHEAD>
 void run_case(const NormArgs& a, const Shape& s, int sms, cudaStream_t st, int* grid) {
-  static int fits[33] = {};
+  static Fits fits;
   static uint64_t allowed = 0;
   const size_t threads = s.team.block;
   if constexpr (BWD) {
@@ -630,7 +641,7 @@ void run_case(const NormArgs& a, const Shape& s, int sms, cudaStream_t st, int* 
     constexpr int kCodes = !CODES ? kNoCodes : kWide;
     if constexpr (CODES && NV == 1) {
       if (a.width < kGroup8) {
-        static int narrow_fits[33] = {};
+        static Fits narrow_fits;
         return run(norm_fwd_kernel<T, V, NV, MAXT, kNarrow, AHEAD>, narrow_fits, allowed, a, s, smem, sms, st, grid);
       }
     }

@@ -258,3 +258,36 @@ def test_saved_tensors_come_back_in_any_layout(layout, checkpoint, hooks):
 
     for a, b in zip(grads(made()), grads(nullcontext())):
         assert torch.equal(a, b)
+
+
+_ORDER = """
+import sys
+import torch
+from starry_unigraph.ops.norm import norm_residual
+out = {}
+for H in map(int, sys.argv[2:]):
+    g = torch.Generator(device="cuda").manual_seed(H)
+    x, u, gate, dy = (torch.randn(20_000, H, device="cuda", generator=g) for _ in range(4))
+    ws = [torch.randn(H, device="cuda", generator=g).requires_grad_() for _ in range(3)]
+    y, n = norm_residual(x, u, ws[0], ws[1], gate=gate, scale=ws[2], checkpoint="int8")
+    out[H] = [t.cpu() for t in torch.autograd.grad((y, n), ws, (dy, dy))]
+torch.save(out, sys.argv[1])
+"""
+
+
+def test_results_do_not_depend_on_which_width_ran_first(tmp_path):
+    """172 and 3,000 columns with 8-bit inputs share a kernel and a block size, but not a block's memory."""
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = str(Path(__file__).resolve().parents[1])
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([root, os.environ.get("PYTHONPATH", "")]))
+    res = []
+    for order in (["172", "3000"], ["3000", "172"]):
+        path = str(tmp_path / ("-".join(order) + ".pt"))
+        subprocess.run([sys.executable, "-c", _ORDER, path, *order], check=True, cwd=root, env=env, timeout=300)
+        res.append(torch.load(path))
+    for H in (172, 3000):
+        assert all(torch.equal(a, b) for a, b in zip(res[0][H], res[1][H]))
