@@ -55,6 +55,13 @@ void check_rows(const at::Tensor& t, const char* name, const at::Tensor& like) {
   TORCH_CHECK(unit_last(t), name, " must have unit stride along its last dimension");
 }
 
+// a rate or eps that kernels hold in fp32
+float positive(double v, const char* name) {
+  const float f = static_cast<float>(v);
+  TORCH_CHECK(f > 0 && std::isfinite(f), name, " must be positive and finite in float32");
+  return f;
+}
+
 struct ScanSizes {
   bool packed;
   int64_t batch, steps, width;
@@ -83,8 +90,7 @@ ScanArgs scan_args(const ScanSizes& z, const at::Tensor& decay, const OptTensor&
   a.batch = z.batch;
   a.steps = z.steps;
   a.width = static_cast<int>(z.width);
-  TORCH_CHECK(rate > 0 && std::isfinite(rate), "gated_scan: rate must be positive and finite");
-  a.rate = static_cast<float>(rate);
+  a.rate = positive(rate, "gated_scan: rate");
   check_param(decay, "gated_scan: decay", z.width, dev);
   a.decay = decay.data_ptr();
   a.decay_bf16 = decay.scalar_type() == at::kBFloat16;
@@ -351,7 +357,7 @@ at::Tensor gated_scan_step(const at::Tensor& p_in, const at::Tensor& decay, at::
               "gated_scan_step: p must be [rows, 3H] with unit stride along its last dimension");
   const int64_t n = p.size(0), H = p.size(1) / 3;
   TORCH_CHECK(H <= (1 << 18), "gated_scan_step: H above 2^18");
-  TORCH_CHECK(rate > 0 && std::isfinite(rate), "gated_scan_step: rate must be positive and finite");
+  const float rate32 = positive(rate, "gated_scan_step: rate");
   c10::cuda::CUDAGuard guard(p.device());
   check_param(decay, "gated_scan_step: decay", H, p.device());
   TORCH_CHECK(state.device() == p.device() && state.scalar_type() == at::kFloat && state.dim() == 2 &&
@@ -377,7 +383,7 @@ at::Tensor gated_scan_step(const at::Tensor& p_in, const at::Tensor& decay, at::
   a.rows = n;
   a.table_rows = state.size(0);
   a.width = static_cast<int>(H);
-  a.rate = static_cast<float>(rate);
+  a.rate = rate32;
   a.p = p.data_ptr();
   a.p_sb = p.stride(0);
   a.decay = decay.data_ptr();
@@ -399,10 +405,9 @@ namespace {
 NormArgs norm_args(const at::Tensor& x, int64_t width, const OptTensor& w_post, const OptTensor& w_pre,
                    const OptTensor& scale, double eps) {
   TORCH_CHECK(width >= 1 && width <= kNormMaxWidth, "norm_residual: the width must be 1 to ", str(kNormMaxWidth));
-  TORCH_CHECK(eps > 0 && std::isfinite(eps), "norm_residual: eps must be positive and finite");
   NormArgs a;
   a.width = static_cast<int>(width);
-  a.eps = static_cast<float>(eps);
+  a.eps = positive(eps, "norm_residual: eps");
   auto param = [&](const OptTensor& t, const char* name, const void*& ptr, int& bf16) {
     if (!given(t)) return;
     check_param(*t, name, width, x.device());

@@ -39,6 +39,15 @@ def check_checkpoint(value: str | None) -> bool:
     return value == "int8"
 
 
+def check_positive(value: float, name: str, dtype: torch.dtype) -> float:
+    """A rate or eps as a float: positive and finite once rounded to the type that the formulas run in."""
+    value = float(value)
+    least, most = (0.0, float("inf")) if dtype == torch.float64 else (2.0 ** -150, 2.0 ** 128 - 2.0 ** 103)
+    if not least < value < most:
+        raise ValueError(f"{name} must be positive and finite, got {value}")
+    return value
+
+
 def _quantize_torch(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Codes and scales of [rows, H] with torch operations (fp32; fp64 inputs stay fp64)."""
     v = x if x.dtype == torch.float64 else x.float()

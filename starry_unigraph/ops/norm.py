@@ -15,7 +15,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from starry_unigraph.ops import cuda_ext
-from starry_unigraph.ops.checkpoint8 import _hidden, _shown, check_checkpoint, quantize8
+from starry_unigraph.ops.checkpoint8 import _hidden, _shown, check_checkpoint, check_positive, quantize8
 
 
 def _norm_torch(x, u, gate, w_post, w_pre, scale, eps):
@@ -93,8 +93,7 @@ def _call(x, u, gate, w_post, w_pre, scale, eps, checkpoint):
     H = x.size(-1) if x.dim() else 0
     if H == 0:
         raise ValueError("norm_residual: x needs a last dimension of at least one value")
-    if not eps > 0:
-        raise ValueError(f"norm_residual: eps must be positive, got {eps}")
+    eps = check_positive(eps, "norm_residual: eps", x.dtype)
     for name, t in (("u", u), ("gate", gate)):
         if t is not None and (t.shape != x.shape or t.dtype != x.dtype):
             raise ValueError(f"norm_residual: {name} must have x's shape {tuple(x.shape)} and type {x.dtype}, got "

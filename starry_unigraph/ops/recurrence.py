@@ -24,7 +24,8 @@ import torch.nn.functional as F
 from torch.autograd.function import once_differentiable
 
 from starry_unigraph.ops import cuda_ext
-from starry_unigraph.ops.checkpoint8 import _dequantize_torch, _hidden, _quantize_torch, _shown, check_checkpoint
+from starry_unigraph.ops.checkpoint8 import (_dequantize_torch, _hidden, _quantize_torch, _shown, check_checkpoint,
+                                             check_positive)
 
 STATE_EVERY = 16  # checkpoint="int8": steps between the fp32 states kept for the backward pass
 
@@ -144,8 +145,7 @@ def gated_scan(p: torch.Tensor, decay: torch.Tensor, h0: torch.Tensor | None = N
         return cuda_ext().gated_scan(p, decay, h0, mask, offsets, rate, keep8)
     if p.dim() != (3 if offsets is None else 2) or p.size(-1) == 0 or p.size(-1) % 3:
         raise ValueError("gated_scan: p must be [batch, steps, 3H], or [rows, 3H] with offsets")
-    if not rate > 0:
-        raise ValueError(f"gated_scan: rate must be positive, got {rate}")
+    rate = check_positive(rate, "gated_scan: rate", p.dtype)
     H = p.size(-1) // 3
     if tuple(decay.shape) != (H,):
         raise ValueError(f"gated_scan: decay must have shape ({H},), got {tuple(decay.shape)}")
@@ -155,8 +155,8 @@ def gated_scan(p: torch.Tensor, decay: torch.Tensor, h0: torch.Tensor | None = N
     if mask is not None and (mask.dtype != torch.bool or mask.shape != p.shape[:-1]):
         raise ValueError(f"gated_scan: mask must be bool of shape {tuple(p.shape[:-1])}")
     if keep8:
-        return _ThroughCodes.apply(p, decay, h0, mask, offsets, float(rate))
-    return _scan_torch(p, decay, h0, mask, offsets, float(rate))
+        return _ThroughCodes.apply(p, decay, h0, mask, offsets, rate)
+    return _scan_torch(p, decay, h0, mask, offsets, rate)
 
 
 def gated_scan_step(p: torch.Tensor, decay: torch.Tensor, state: torch.Tensor, rows: torch.Tensor | None = None, *,
@@ -171,14 +171,13 @@ def gated_scan_step(p: torch.Tensor, decay: torch.Tensor, state: torch.Tensor, r
         return cuda_ext().gated_scan_step(p, decay, state, rows, rate)
     if p.dim() != 2 or p.size(1) == 0 or p.size(1) % 3:
         raise ValueError("gated_scan_step: p must be [rows, 3H]")
-    if not rate > 0:
-        raise ValueError(f"gated_scan_step: rate must be positive, got {rate}")
+    rate = check_positive(rate, "gated_scan_step: rate", p.dtype)
     if state.dtype not in (torch.float32, torch.float64) or state.dim() != 2 or state.size(1) * 3 != p.size(1):
         raise ValueError(f"gated_scan_step: state must be float32 [table rows, {p.size(1) // 3}]")
     if (state.size(0) if rows is None else rows.numel()) != p.size(0):
         raise ValueError("gated_scan_step: one place of the table per row of p is wanted")
     with torch.no_grad():
-        h, last = _scan_torch(p.unsqueeze(1), decay, state if rows is None else state[rows], None, None, float(rate))
+        h, last = _scan_torch(p.unsqueeze(1), decay, state if rows is None else state[rows], None, None, rate)
         if rows is None:
             state.copy_(last)
         else:

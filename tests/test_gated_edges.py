@@ -6,8 +6,8 @@ import pytest
 import torch
 
 from starry_unigraph.ops.checkpoint8 import quantize8, saved8
-from starry_unigraph.ops.norm import norm_residual
-from starry_unigraph.ops.recurrence import gated_scan
+from starry_unigraph.ops.norm import norm_residual, rms_norm
+from starry_unigraph.ops.recurrence import gated_scan, gated_scan_step
 
 
 def test_saved8_leaves_weights_alone():
@@ -93,3 +93,15 @@ def test_masked_steps_get_no_gradient_whatever_the_state(checkpoint):
         a = [t.clone().requires_grad_() for t in (p, d)]
         dp, = torch.autograd.grad(gated_scan(*a, h0, mask=mask, checkpoint=checkpoint)[0].sum(), a[:1])
         assert torch.equal(dp[~mask], torch.zeros_like(dp[~mask]))
+
+
+def test_rates_and_eps_that_fp32_cannot_hold_are_refused():
+    p, d, x, w = torch.randn(2, 3, 12), torch.randn(4), torch.zeros(3, 8), torch.ones(8)
+    for bad in (2.0 ** -150, 1e-60, 3.5e38, 1e300, float("inf"), float("nan"), 0.0, -1.0):
+        for f in (lambda: gated_scan(p, d, rate=bad), lambda: gated_scan_step(p[0], d, torch.zeros(3, 4), rate=bad),
+                  lambda: rms_norm(x, w, eps=bad), lambda: norm_residual(x, x, w, eps=bad)):
+            with pytest.raises(ValueError):
+                f()
+    for good in (2.0 ** -149, 1e-40, 3.4e38):
+        assert torch.equal(rms_norm(x, w, eps=good), x) and torch.isfinite(gated_scan(p, d - 50, rate=good)[0]).all()
+    assert torch.equal(rms_norm(x.double(), w.double(), eps=1e-60), x.double())

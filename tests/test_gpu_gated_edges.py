@@ -291,3 +291,20 @@ def test_results_do_not_depend_on_which_width_ran_first(tmp_path):
         res.append(torch.load(path))
     for H in (172, 3000):
         assert all(torch.equal(a, b) for a, b in zip(res[0][H], res[1][H]))
+
+
+def test_rates_and_eps_that_fp32_cannot_hold_are_refused():
+    """An eps that rounds to 0 made NaN of rows of zeros, a rate that rounds to infinity of closed gates."""
+    from starry_unigraph.ops.norm import norm_residual, rms_norm
+    from starry_unigraph.ops.recurrence import gated_scan, gated_scan_step
+
+    p, d = torch.randn(2, 3, 12, device="cuda"), torch.randn(4, device="cuda")
+    x, w, t = torch.zeros(3, 8, device="cuda"), torch.ones(8, device="cuda"), torch.zeros(3, 4, device="cuda")
+    for bad in (2.0 ** -150, 1e-60, 3.5e38, 1e300, float("inf"), float("nan"), 0.0, -1.0):
+        for f in (lambda: gated_scan(p, d, rate=bad), lambda: gated_scan_step(p[0], d, t, rate=bad),
+                  lambda: rms_norm(x, w, eps=bad), lambda: norm_residual(x, x, w, eps=bad)):
+            with pytest.raises(RuntimeError, match="positive and finite"):
+                f()
+    assert not t.any()
+    for good in (2.0 ** -149, 1e-40, 3.4e38):
+        assert torch.equal(rms_norm(x, w, eps=good), x) and torch.isfinite(gated_scan(p, d - 50, rate=good)[0]).all()
