@@ -164,9 +164,9 @@ def gated_scan_step(p: torch.Tensor, decay: torch.Tensor, state: torch.Tensor, r
     """One step for each row of p ``[n, 3H]``; returns h ``[n, H]`` in p's type.
 
     state: fp32 table ``[table rows, H]``, updated in place: row ``rows[j]`` (int64, no row
-    twice; None: row j) holds the state of row j. A place outside the table is reported by
-    ``check_status()``; its row of h is zero and nothing is written. No gradient flows
-    through a step."""
+    twice; None: row j) holds the state of row j. On CUDA a place outside the table is reported
+    by ``check_status()``, its row of h is zero and nothing is written for it; on CPU it raises
+    before anything is written. No gradient flows through a step."""
     if p.is_cuda:
         return cuda_ext().gated_scan_step(p, decay, state, rows, rate)
     if p.dim() != 2 or p.size(1) == 0 or p.size(1) % 3:
@@ -176,6 +176,13 @@ def gated_scan_step(p: torch.Tensor, decay: torch.Tensor, state: torch.Tensor, r
         raise ValueError(f"gated_scan_step: state must be float32 [table rows, {p.size(1) // 3}]")
     if (state.size(0) if rows is None else rows.numel()) != p.size(0):
         raise ValueError("gated_scan_step: one place of the table per row of p is wanted")
+    if tuple(decay.shape) != (state.size(1),):
+        raise ValueError(f"gated_scan_step: decay must have shape ({state.size(1)},), got {tuple(decay.shape)}")
+    if rows is not None:
+        if rows.dtype not in (torch.int64, torch.int32) or rows.dim() != 1:
+            raise ValueError("gated_scan_step: rows must be an int64 vector, one place per row of p")
+        if rows.numel() and not 0 <= int(rows.min()) <= int(rows.max()) < state.size(0):
+            raise IndexError(f"gated_scan_step: rows must be places of the table, 0 to {state.size(0) - 1}")
     with torch.no_grad():
         h, last = _scan_torch(p.unsqueeze(1), decay, state if rows is None else state[rows], None, None, rate)
         if rows is None:

@@ -105,3 +105,19 @@ def test_rates_and_eps_that_fp32_cannot_hold_are_refused():
     for good in (2.0 ** -149, 1e-40, 3.4e38):
         assert torch.equal(rms_norm(x, w, eps=good), x) and torch.isfinite(gated_scan(p, d - 50, rate=good)[0]).all()
     assert torch.equal(rms_norm(x.double(), w.double(), eps=1e-60), x.double())
+
+
+def test_step_refuses_places_outside_the_table():
+    """Nothing is written, of the valid places neither; -1 is no last row."""
+    torch.manual_seed(4)
+    p, d = torch.randn(3, 12), torch.randn(4)
+    for rows in ([0, 1, -1], [0, 1, 5], [-5, 1, 2]):
+        table = torch.ones(5, 4)
+        with pytest.raises(IndexError):
+            gated_scan_step(p, d, table, torch.tensor(rows))
+        assert torch.equal(table, torch.ones(5, 4))
+    for rows, decay in ((torch.tensor([True, True, True]), d), (torch.tensor([[0], [1], [2]]), d),
+                        (torch.tensor([0, 1, 2]), d[:1])):
+        with pytest.raises(ValueError):
+            gated_scan_step(p, decay, table, rows)
+    assert gated_scan_step(p[:0], d, table, torch.zeros(0, dtype=torch.long)).shape == (0, 4)
