@@ -36,7 +36,7 @@ def _scan_torch(p, decay, h0, mask, offsets, rate):
     dec = decay.to(wide.dtype)
     if offsets is not None:
         bounds = offsets.tolist()
-        if bounds[0] != 0 or bounds[-1] != p.size(0) or any(b < a for a, b in zip(bounds, bounds[1:])):
+        if not bounds or bounds[0] != 0 or bounds[-1] != p.size(0) or any(b < a for a, b in zip(bounds, bounds[1:])):
             raise ValueError("gated_scan: offsets must rise from 0 to the number of rows")
         outs, lasts = [], []
         for s, (a, b) in enumerate(zip(bounds, bounds[1:])):

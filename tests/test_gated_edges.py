@@ -121,3 +121,10 @@ def test_step_refuses_places_outside_the_table():
         with pytest.raises(ValueError):
             gated_scan_step(p, decay, table, rows)
     assert gated_scan_step(p[:0], d, table, torch.zeros(0, dtype=torch.long)).shape == (0, 4)
+
+
+def test_scan_refuses_empty_offsets():
+    for keep in (None, "int8"):
+        for off in (torch.zeros(0, dtype=torch.long), torch.zeros(1, dtype=torch.long)):
+            with pytest.raises(ValueError):
+                gated_scan(torch.randn(3, 6), torch.randn(2), offsets=off, checkpoint=keep)
