@@ -10,7 +10,8 @@ The norm after a block, its gate and residual scale and the norm before the next
 one kernel (``norm_residual``); the recurrence runs over all steps at once (``gated_scan``)
 instead of one cell call per snapshot, and ``step`` advances every layer by one token on a
 table of states. With ``checkpoint="int8"`` the recurrence and the norms keep their inputs
-in 8 bits for the backward pass.
+in 8 bits for the backward pass. Rows are taken in the type of the parameters (float32 or
+bfloat16, on CPU float64 too); states are float32 (of float64 blocks float64).
 """
 from __future__ import annotations
 
@@ -48,12 +49,14 @@ class GatedRecurrentStack(nn.Module):
         return len(self.proj)
 
     def init_state(self, rows: int, device=None) -> list[torch.Tensor]:
-        """Zero states, one fp32 table [rows, width] per layer."""
+        """Zero states, one table [rows, width] per layer."""
         device = self.decay[0].device if device is None else device
-        return [torch.zeros(rows, self.width, device=device) for _ in range(self.num_layers)]
+        dtype = torch.float64 if self.decay[0].dtype == torch.float64 else torch.float32
+        return [torch.zeros(rows, self.width, device=device, dtype=dtype) for _ in range(self.num_layers)]
 
     def _layers(self, x, recur):
         """x [rows, width] through every layer; recur(layer, p) gives h."""
+        x = x.to(self.pre[0].dtype)
         y, n = x, rms_norm(x, self.pre[0], eps=self.eps, checkpoint=self.checkpoint)
         for k in range(self.num_layers):
             p = linear(n, self.proj[k].weight, self.proj[k].bias)
@@ -81,11 +84,11 @@ class GatedRecurrentStack(nn.Module):
             states.append(last)
             return h.transpose(0, 1).reshape(steps * rows, width)
 
-        n = self._layers(x.float().reshape(steps * rows, width), recur)
+        n = self._layers(x.reshape(steps * rows, width), recur)
         return n.view(steps, rows, width), states
 
     @torch.no_grad()
     def step(self, x: torch.Tensor, state: list[torch.Tensor], rows: torch.Tensor | None = None) -> torch.Tensor:
         """One new token x [n, width] per row; the layers' tables `state` advance in place at
         `rows` (every row when None). Returns the normed output [n, width]."""
-        return self._layers(x.float(), lambda k, p: gated_scan_step(p, self.decay[k], state[k], rows, rate=self.rate))
+        return self._layers(x, lambda k, p: gated_scan_step(p, self.decay[k], state[k], rows, rate=self.rate))

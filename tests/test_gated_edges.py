@@ -1,10 +1,12 @@
 """Edges of the gated recurrence, the norms around a block and 8-bit activations on CPU: what
 8-bit saved tensors leave alone, values that are not finite, arguments that are refused."""
+import copy
 from contextlib import nullcontext
 
 import pytest
 import torch
 
+from starry_unigraph.lib_stable import GatedRecurrentStack
 from starry_unigraph.ops.checkpoint8 import quantize8, saved8
 from starry_unigraph.ops.norm import norm_residual, rms_norm
 from starry_unigraph.ops.recurrence import gated_scan, gated_scan_step
@@ -128,3 +130,23 @@ def test_scan_refuses_empty_offsets():
         for off in (torch.zeros(0, dtype=torch.long), torch.zeros(1, dtype=torch.long)):
             with pytest.raises(ValueError):
                 gated_scan(torch.randn(3, 6), torch.randn(2), offsets=off, checkpoint=keep)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_stack_runs_in_the_type_of_its_parameters(checkpoint):
+    """float64 blocks whole and token by token to 64 bits, and the fp32 blocks' results to 32."""
+    torch.manual_seed(5)
+    m = GatedRecurrentStack(12, num_layers=2, checkpoint=checkpoint)
+    x = torch.randn(7, 5, 12)
+    n, last = m(x)
+    m64 = copy.deepcopy(m).double()
+    n64, last64 = m64(x)
+    assert n64.dtype == last64[0].dtype == torch.float64 and n.dtype == last[0].dtype == torch.float32
+    torch.testing.assert_close(n64.float(), n, rtol=1e-4, atol=1e-5)
+    state = m64.init_state(5)
+    out = torch.stack([m64.step(row, state) for row in x])
+    torch.testing.assert_close(out, n64, rtol=1e-12, atol=1e-12)
+    torch.testing.assert_close(state, last64, rtol=1e-12, atol=1e-12)
+    n64.square().sum().backward()
+    assert all(torch.isfinite(p.grad).all() and p.grad.dtype == torch.float64 for p in m64.parameters() if p.grad is not None)
+    assert m.bfloat16()(x)[0].dtype == torch.bfloat16
