@@ -330,3 +330,62 @@ def test_stack_in_bf16():
     state = m.init_state(30)
     out = torch.stack([m.step(row, state) for row in x])
     assert err(out, exact) < 3e-2 and all(err(a, b) < 3e-2 for a, b in zip(state, end))
+
+
+def test_step_on_another_stream_advances_the_whole_table():
+    from starry_unigraph.ops.recurrence import gated_scan_step
+
+    torch.manual_seed(7)
+    p, d, table = torch.randn(400, 96, device="cuda"), torch.randn(32, device="cuda"), torch.randn(500, 32, device="cuda")
+    rows = torch.randperm(500, device="cuda")[:400]
+    want = table.clone()
+    h = gated_scan_step(p, d, want, rows)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    got = table.clone()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = gated_scan_step(p, d, got, rows)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(out, h) and torch.equal(got, want) and not torch.equal(got, table)
+    rest = torch.ones(500, dtype=torch.bool, device="cuda").index_fill_(0, rows, False)
+    assert torch.equal(got[rest], table[rest])
+
+
+def test_bytes_kept_in_8_bits():
+    """What lives between the forward and the backward pass: 1.125 bytes a value of p, x, u and gate instead of
+    four, beside the outputs and the states kept every 16 (8) steps, as asked of the allocator."""
+    from starry_unigraph.ops.checkpoint8 import saved8
+    from starry_unigraph.ops.norm import norm_residual
+    from starry_unigraph.ops.recurrence import gated_scan
+
+    B, T, H = 2000, 33, 64
+    n = B * T * H
+    p, x = torch.randn(B, T, 3 * H, device="cuda", requires_grad=True), torch.randn(B * T, H, device="cuda", requires_grad=True)
+    d, w = torch.randn(H, device="cuda"), torch.randn(H, device="cuda")
+
+    def asked():  # (whole blocks would count up to 1 MB a tensor more)
+        return torch.cuda.memory_stats()["requested_bytes.all.current"]
+
+    def kept(f):
+        before = asked()
+        out = f()
+        assert all(t.grad_fn is not None for t in out)
+        return asked() - before
+
+    def scan(keep):
+        return kept(lambda: gated_scan(p * 1, d, checkpoint=keep))
+
+    def norm(keep):
+        return kept(lambda: norm_residual(x * 1, x * 2, w, w, gate=x * 3, checkpoint=keep))
+
+    def packed():
+        with saved8():
+            return (torch.sin(x * 1),)
+
+    out = 4 * n + 4 * B * H  # h and the last states
+    assert scan("int8") == out + 3.375 * n + 4 * B * 2 * H
+    assert scan(None) == out + 12 * n + 4 * B * 4 * H
+    assert norm("int8") == 8 * n + 3.375 * n
+    assert norm(None) == 8 * n + 12 * n
+    assert kept(packed) == 4 * n + 1.125 * n
