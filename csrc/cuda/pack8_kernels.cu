@@ -1,7 +1,8 @@
 // Activations in 8 bits: per group of 32 values of a row, scale = amax / 127 and
 // code = rint(v * (127 / amax)). Bound by bytes: each value is read once, and one byte
 // is written for it and four for the group's scale. 1,600,000 x 64 fp32: 101 us to codes
-// (5.2 TB/s; five exchanges a group and the rounding cost issue), 84 us back (6.3 TB/s).
+// (5.2 TB/s; three exchanges a group, a division on each of its eight lanes and the rounding cost
+// issue), 84 us back (6.3 TB/s).
 #include "scan_shape.cuh"
 
 namespace su {

@@ -145,9 +145,9 @@ struct Held {
 // registers, and then backwards for g. The gates are evaluated once.
 //
 // Bound by the loads under way: three blocks of 128 threads fit an SM with their factors and
-// slots (74 KB a block with packed fp32). 200,000 x 8 x 64 fp32 557 us, 5.1 TB/s; 2 x 65,537 x 256
-// bf16 131 us, where the gates' special functions and issue bound it; 1,000,000 x 100 packed
-// fp32 700 us, 4.1 TB/s, the marks' branches on top; 400,000 x 4 x 128 from 8-bit codes 798 us.
+// slots (74 KB a block with packed fp32). 200,000 x 8 x 64 fp32 567 us, 5.1 TB/s; 2 x 65,537 x 256
+// bf16 128 us, where the gates' special functions and issue bound it; 1,000,000 x 100 packed
+// fp32 704 us, 4.1 TB/s, the marks' branches on top; 400,000 x 4 x 128 from 8-bit codes 802 us.
 constexpr int kBwdThreads = 128;
 template <class T, int V, int CH, bool CODES, int KIND>
 __global__ void __launch_bounds__(kBwdThreads, 3) scan_bwd_kernel(const ScanArgs A, const ScanPlan P, const Lanes L) {

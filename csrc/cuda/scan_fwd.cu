@@ -27,7 +27,7 @@ struct Unit {
 // fp32 (two channels) 68 and 63.
 //
 // Bound by bytes at fp32: 200,000 x 8 x 64 takes 262 us, 6.3 TB/s. With codes the encoding's
-// instructions bound it (400,000 x 4 x 128 fp32: 698 us), in bf16 the gates' as well.
+// instructions bound it (400,000 x 4 x 128 fp32: 693 us), in bf16 the gates' as well.
 template <class T, int V, int KIND>
 constexpr bool kAsyncOf = V == 4 && (sizeof(T) == 4 || KIND == kPlain);
 
